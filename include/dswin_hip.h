@@ -648,6 +648,65 @@ int dsw_layernorm_bwd(const void *dy, int dy_dtype, long long ld_dy, const float
                       const float *mean, const float *rstd, long long M, int C, float *dx, const float *dx_add,
                       const float *dx_add2, long long ld_add2, int cols2, float *partial, void *stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Attention over token sequences (no counterpart in the reference, whose attention ends at the border of an
+ * 8x8 / 16x16 window).  Tensors are [B, tokens, heads, D] with D contiguous; the other three strides, in elements,
+ * are passed as a dsw_strides in HOST memory (read before the call returns), so that slices of a packed q|k|v
+ * projection and caches of any order are read in place.  Strides of results must not let two elements coincide.
+ */
+typedef struct { long long b, l, h; } dsw_strides;
+
+/* Norm of every head's query and key row and the rotation by position, one launch for both:
+ *     u = w * x / sqrt(mean(x^2) + eps);  pair c = a * pairs + i of the first 2 * axes * pairs columns -
+ *     (c, c + axes * pairs), interleaved: (2c, 2c + 1) - turns by pos[b, l, a] * freqs[a, i] radians.
+ * q, oq [B,L,Hq,D], k, ok [B,L,Hkv,D], dtype for all four; 1 <= D <= 128, 2 * axes * pairs <= D.  wq, wk [D] fp32 or
+ * NULL (ones); freqs [axes, pairs] fp32 (NULL with axes * pairs = 0: norm only); pos int32 or int64 (pos_bytes 4 or 8)
+ * [.., L, axes] with pos_batch elements between sequences (0: one set for all), NULL: the token's index on every axis. */
+int dsw_qk_norm_rotary_fwd(const void *q, const dsw_strides *sq, const void *k, const dsw_strides *sk, int dtype, int B,
+                           int L, int Hq, int Hkv, int D, const float *wq, const float *wk, float eps, const float *freqs,
+                           int axes, int pairs, const void *pos, int pos_bytes, long long pos_batch, int interleaved, void *oq,
+                           const dsw_strides *soq, void *ok, const dsw_strides *sok, void *stream);
+/* Its backward: dq, dk from the gradients dyq, dyk of oq, ok (q, k: the inputs of the forward).  partial: NULL, or
+ * fp32 [dsw_qk_norm_rotary_blocks(B, L)][2][D], whose column sums (dsw_colsum) are the gradients of wq and wk. */
+int dsw_qk_norm_rotary_blocks(int B, int L);
+int dsw_qk_norm_rotary_bwd(const void *q, const dsw_strides *sq, const void *k, const dsw_strides *sk, const void *dyq,
+                           const dsw_strides *sdyq, const void *dyk, const dsw_strides *sdyk, int dtype, int B, int L,
+                           int Hq, int Hkv, int D, const float *wq, const float *wk, float eps, const float *freqs, int axes,
+                           int pairs, const void *pos, int pos_bytes, long long pos_batch, int interleaved, void *dq, const dsw_strides *sdq,
+                           void *dk, const dsw_strides *sdk, float *partial, void *stream);
+
+/* Softmax attention with a sliding window of keys and a few first keys (sinks) that stay visible.  Query row i of
+ * sequence b stands at p = k_len - q_len + i (q_len <= Lq rows, k_len <= Lk keys); key j < k_len is visible to it when
+ * j <= p + right and (j >= p - left or j < sinks).  out = softmax over the visible keys of scale * q.k + bias, times v;
+ * rows without a visible key and rows from q_len on are zeros, and so are their gradients.  Query head h reads key head
+ * h / (Hq / Hkv).  The description is read before the call returns (it lies in HOST memory, the pointers in it do not). */
+typedef struct {
+    int dtype;                 /* of q, k, v, out and their gradients: DSW_F32 or DSW_BF16 */
+    int B, Lq, Lk, Hq, Hkv, D; /* Hq a multiple of Hkv, 1 <= D <= 128 */
+    int left, right;           /* keys before / behind the row's own position, -1: all */
+    int sinks;
+    float scale;               /* > 0 */
+    const int *q_lens, *k_lens; /* int32 [B] or NULL (all Lq rows / Lk keys); values are clamped to 0..Lq / 0..Lk */
+    const float *bias_table;   /* fp32 [n_buckets, Hq] or NULL: bias[j - p] = table[bias_buckets[clip(j - p, +-M) + M]] */
+    const int *bias_buckets;   /* int32 [2 M + 1], values are clamped to 0..n_buckets - 1 */
+    int n_buckets, max_distance; /* M <= 512 */
+} dsw_band_desc;
+
+/* lse: fp32 [B, Hq, Lq] for the backward or NULL; out32: NULL, or (bf16 calls with a bias table that wants a gradient)
+ * fp32 [B, Lq, Hq, D], the result before its rounding, which the table's gradient needs.  Without either, calls of few
+ * query rows (new tokens over a cache) split the keys over workgroups; workspace holds their shares. */
+size_t dsw_band_attn_fwd_workspace(const dsw_band_desc *d);
+int dsw_band_attn_fwd(const dsw_band_desc *d, const void *q, const dsw_strides *sq, const void *k, const dsw_strides *sk,
+                      const void *v, const dsw_strides *sv, void *out, const dsw_strides *so, float *lse, float *out32,
+                      void *workspace, size_t workspace_bytes, void *stream);
+/* Backward: dq, dk, dv, and d_table fp32 [n_buckets, Hq] (or NULL).  out, out32, lse as the forward left them. */
+size_t dsw_band_attn_bwd_workspace(const dsw_band_desc *d);
+int dsw_band_attn_bwd(const dsw_band_desc *d, const void *q, const dsw_strides *sq, const void *k, const dsw_strides *sk,
+                      const void *v, const dsw_strides *sv, const void *out, const dsw_strides *so, const float *out32,
+                      const void *dout, const dsw_strides *sdo, const float *lse, void *dq, const dsw_strides *sdq, void *dk,
+                      const dsw_strides *sdk, void *dv, const dsw_strides *sdv, float *d_table, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

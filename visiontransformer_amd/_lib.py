@@ -22,6 +22,19 @@ _I = ctypes.c_int
 _F = ctypes.c_float
 _Z = ctypes.c_size_t
 
+
+class Strides(ctypes.Structure):
+    """dsw_strides: elements between batches, tokens and heads"""
+    _fields_ = [("b", ctypes.c_longlong), ("l", ctypes.c_longlong), ("h", ctypes.c_longlong)]
+
+
+class BandDesc(ctypes.Structure):
+    """dsw_band_desc"""
+    _fields_ = [("dtype", _I), ("B", _I), ("Lq", _I), ("Lk", _I), ("Hq", _I), ("Hkv", _I), ("D", _I), ("left", _I), ("right", _I),
+                ("sinks", _I), ("scale", _F), ("q_lens", _P), ("k_lens", _P), ("bias_table", _P), ("bias_buckets", _P),
+                ("n_buckets", _I), ("max_distance", _I)]
+
+
 # name -> (restype, argtypes); must list every symbol include/dswin_hip.h declares
 SIGNATURES = {
     "dswin_version": (_I, []),
@@ -115,6 +128,13 @@ SIGNATURES = {
     "dsw_sparse_disc_bwd_scratch": (_Z, [_I, _I, _I, _I, _I]),
     "dsw_sparse_disc_bwd": (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I,
                                  _P, _P, _P, _P, _P, _P, _P, _P]),
+    "dsw_qk_norm_rotary_fwd": (_I, [_P, _P, _P, _P] + [_I] * 6 + [_P, _P, _F, _P, _I, _I, _P, _I, ctypes.c_longlong, _I] + [_P] * 5),
+    "dsw_qk_norm_rotary_blocks": (_I, [_I, _I]),
+    "dsw_band_attn_fwd_workspace": (_Z, [_P]),
+    "dsw_band_attn_fwd": (_I, [_P] * 12 + [_Z, _P]),
+    "dsw_band_attn_bwd_workspace": (_Z, [_P]),
+    "dsw_band_attn_bwd": (_I, [_P] * 21 + [_Z, _P]),
+    "dsw_qk_norm_rotary_bwd": (_I, [_P] * 8 + [_I] * 6 + [_P, _P, _F, _P, _I, _I, _P, _I, ctypes.c_longlong, _I] + [_P] * 6),
 }
 
 

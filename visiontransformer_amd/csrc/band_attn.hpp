@@ -1,0 +1,337 @@
+// Shared pieces of the attention over token sequences (band_attn_fwd.hip, band_attn_step.hip, band_attn_bwd.hip).
+//
+//   query row i of sequence b stands at p = k_len - q_len + i; key j < k_len is visible when j <= p + right and
+//   (j >= p - left or j < sinks);  x_j = log2(e) * (scale * q.k_j + bias[clip(j - p)]);  out = sum 2^(x_j - lse) v_j
+//
+// All products run on 32x32 MFMA tiles with the softmax rows on the lane axis of the accumulators, so that the
+// probabilities of a tile are, as they stand in the registers, the second operand of the product behind them.
+#pragma once
+#include "attn_common.hpp"
+
+namespace dsw {
+
+constexpr int BAND_TILE = 64;    // keys (forward, dQ) or query rows (dK, dV) staged at a time
+constexpr int BAND_ROWS = 128;   // query rows (forward, dQ) or keys (dK, dV) of a workgroup: 4 waves x 32
+constexpr int BAND_MARGIN = 96;  // a tile of 64 x 32 spans 95 distances: entries past the clip distance in the LDS bias
+constexpr int BAND_MAX_DISTANCE = 512;
+constexpr int BAND_FAR = 1 << 29;  // "unlimited": beyond every length, and sums of two stay inside 32 bits
+
+struct BandTensor {
+    const void *p;
+    dsw_strides s;
+    int mode;  // 0: whole 16-byte pieces; 1: 4-byte pieces; 2: single elements
+};
+
+struct BandArgs {
+    BandTensor q, k, v, out, dout, dq, dk, dv;
+    int B, Lq, Lk, Hq, Hkv, G, D;
+    int left, right, sinks;
+    float c, scale;  // scale * log2(e), scale
+    const int *q_lens, *k_lens;
+    const float *table;  // [n_buckets][Hq] or null
+    const int *buckets;  // [2 M + 1]
+    int n_buckets, M;
+    float *lse;          // [B][Hq][Lq], base 2; +inf for rows without a visible key (2^(x - inf) = 0 in the backward)
+    float *out32;        // [B][Lq][Hq][D] or null
+    float *delta;        // [B][Hq][Lq]
+    float *partial;      // step kernel: see there; dQ kernel: bias gradients by distance
+    int nsplit, nrb;
+};
+
+// ---- element types ------------------------------------------------------------------------------------------
+// A fragment is the 8 elements a lane hands to one 32x32x16 product: row (or column) lane % 32, k = 8 * (lane / 32)...
+template <typename T> struct band_t;
+template <> struct band_t<bf16_t> {
+    typedef uint4 frag;
+    template <int DP> static constexpr int elems(int rows) { return rows * DP; }
+    static constexpr int nbuf(int) { return 2; }
+};
+template <> struct band_t<float> {
+    struct frag { float4 lo, hi; };
+    template <int DP> static constexpr int elems(int rows) { return rows * (DP + 4); }
+    static constexpr int nbuf(int dp) { return dp == 128 ? 1 : 2; }
+};
+
+__device__ __forceinline__ f32x16 band_mma(const uint4 &a, const uint4 &b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 band_mma(const band_t<float>::frag &a, const band_t<float>::frag &b, f32x16 c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.lo.x, b.lo.x, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.lo.y, b.lo.y, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.lo.z, b.lo.z, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.lo.w, b.lo.w, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.hi.x, b.hi.x, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.hi.y, b.hi.y, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.hi.z, b.hi.z, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.hi.w, b.hi.w, c, 0, 0, 0);
+    return c;
+}
+
+__device__ __forceinline__ f32x16 band_zero() {
+    f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.f;
+    return z;
+}
+
+// registers 8c .. 8c+7 of a 32x32 result as a fragment (bf16: rounded to nearest even)
+__device__ __forceinline__ void band_pack(const f32x16 &s, int c, uint4 &f) {
+    f = make_uint4(pack_bf16(s[8 * c], s[8 * c + 1]), pack_bf16(s[8 * c + 2], s[8 * c + 3]),
+                   pack_bf16(s[8 * c + 4], s[8 * c + 5]), pack_bf16(s[8 * c + 6], s[8 * c + 7]));
+}
+__device__ __forceinline__ void band_pack(const f32x16 &s, int c, band_t<float>::frag &f) {
+    f.lo = make_float4(s[8 * c], s[8 * c + 1], s[8 * c + 2], s[8 * c + 3]);
+    f.hi = make_float4(s[8 * c + 4], s[8 * c + 5], s[8 * c + 6], s[8 * c + 7]);
+}
+// what the rounding of band_pack left behind, rounded in its turn: the two together carry 16 bits
+__device__ __forceinline__ uint32_t band_rest2(float a, float b, uint32_t rounded) {
+    return pack_bf16(a - __uint_as_float(rounded << 16), b - __uint_as_float(rounded & 0xffff0000u));
+}
+__device__ __forceinline__ void band_pack_rest(const f32x16 &s, int c, const uint4 &f, uint4 &rest) {
+    rest = make_uint4(band_rest2(s[8 * c], s[8 * c + 1], f.x), band_rest2(s[8 * c + 2], s[8 * c + 3], f.y),
+                      band_rest2(s[8 * c + 4], s[8 * c + 5], f.z), band_rest2(s[8 * c + 6], s[8 * c + 7], f.w));
+}
+
+// ---- global memory: 8 consecutive elements of a row, zero past D -------------------------------------------------
+__device__ __forceinline__ uint4 band_load8(const bf16_t *row, int col, int D, int mode) {
+    if (mode == 0) return col < D ? *reinterpret_cast<const uint4 *>(row + col) : make_uint4(0u, 0u, 0u, 0u);
+    if (mode == 1) return load_slot(row + col, slot_dwords(D, col >> 3));
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = col + 2 * i < D ? row[col + 2 * i] : 0u, hi = col + 2 * i + 1 < D ? row[col + 2 * i + 1] : 0u;
+        w[i] = lo | (hi << 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ band_t<float>::frag band_load8(const float *row, int col, int D, int mode) {
+    band_t<float>::frag f;
+    if (mode == 0) {
+        f.lo = col < D ? *reinterpret_cast<const float4 *>(row + col) : f4zero();
+        f.hi = col + 4 < D ? *reinterpret_cast<const float4 *>(row + col + 4) : f4zero();
+        return f;
+    }
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = col + i < D ? row[col + i] : 0.f;
+    f.lo = make_float4(v[0], v[1], v[2], v[3]);
+    f.hi = make_float4(v[4], v[5], v[6], v[7]);
+    return f;
+}
+__device__ __forceinline__ void band_clear(uint4 &f) { f = make_uint4(0u, 0u, 0u, 0u); }
+__device__ __forceinline__ void band_clear(band_t<float>::frag &f) { f.lo = f4zero(), f.hi = f4zero(); }
+
+__device__ __forceinline__ void band_store8(bf16_t *row, int col, const float *v, int D, int mode) {
+    const uint4 u = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    if (mode == 0) {
+        if (col < D) *reinterpret_cast<uint4 *>(row + col) = u;
+    } else if (mode == 1) {
+        store_slot(row + col, u, slot_dwords(D, col >> 3));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (col + i < D) row[col + i] = f32_to_bf16(v[i]);
+    }
+}
+__device__ __forceinline__ void band_store8(float *row, int col, const float *v, int D, int mode) {
+    if (mode == 0) {
+        if (col < D) *reinterpret_cast<float4 *>(row + col) = make_float4(v[0], v[1], v[2], v[3]);
+        if (col + 4 < D) *reinterpret_cast<float4 *>(row + col + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (col + i < D) row[col + i] = v[i];
+    }
+}
+
+template <typename T> __device__ __forceinline__ const T *band_row(const BandTensor &t, int b, long long l, int h) {
+    return static_cast<const T *>(t.p) + b * t.s.b + l * t.s.l + h * t.s.h;
+}
+
+// Transposed result tiles (accumulator rows = head-dim columns, lane = row of the tensor): 8 consecutive columns per
+// lane by an exchange of the two lane halves, then one store per 16 columns.  All lanes must call it (the exchange);
+// `on` says whether this lane's row is written.
+template <typename T, int DP>
+__device__ __forceinline__ void band_store_row(T *row, const f32x16 *acc, float mul, int D, int mode, int hh, bool on) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[db][8 * p + i] * mul),
+                                                                __float_as_uint(acc[db][8 * p + 4 + i] * mul), false, false);
+                v[i] = __uint_as_float(r[0]);
+                v[4 + i] = __uint_as_float(r[1]);
+            }
+            if (on) band_store8(row, 32 * db + 16 * p + 8 * hh, v, D, mode);
+        }
+}
+
+// ---- LDS images of [rows][DP] tiles --------------------------------------------------------------------------------
+// bf16: 16-byte slots XORed with a pattern of the row, such that 16 rows' reads of one slot and the transposing reads of
+// 4 rows x 32 columns fall on distinct banks; fp32: rows padded by 16 bytes.
+template <int DP> __device__ __forceinline__ int band_flip(int row) {
+    if constexpr (DP == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else return slot_flip<DP>(row);
+}
+template <typename T, int DP> __device__ __forceinline__ int band_at(int row, int col) {
+    if constexpr (sizeof(T) == 2) return row * DP + (((col >> 3) ^ band_flip<DP>(row)) << 3) + (col & 7);
+    else return row * (DP + 4) + col;
+}
+template <int DP> __device__ __forceinline__ void band_put(bf16_t *m, int row, int slot, const uint4 &f) {
+    *reinterpret_cast<uint4 *>(m + band_at<bf16_t, DP>(row, 8 * slot)) = f;
+}
+template <int DP> __device__ __forceinline__ void band_put(float *m, int row, int slot, const band_t<float>::frag &f) {
+    float *p = m + band_at<float, DP>(row, 8 * slot);
+    *reinterpret_cast<float4 *>(p) = f.lo;
+    *reinterpret_cast<float4 *>(p + 4) = f.hi;
+}
+// rows of the image as the first operand: row row0 + lane % 32, columns 16 c + 8 (lane / 32) ..
+template <int DP> __device__ __forceinline__ uint4 band_rows(const bf16_t *m, int row, int c, int hh) {
+    return *reinterpret_cast<const uint4 *>(m + band_at<bf16_t, DP>(row, 16 * c + 8 * hh));
+}
+template <int DP> __device__ __forceinline__ band_t<float>::frag band_rows(const float *m, int row, int c, int hh) {
+    const float *p = m + band_at<float, DP>(row, 16 * c + 8 * hh);
+    band_t<float>::frag f;
+    f.lo = *reinterpret_cast<const float4 *>(p);
+    f.hi = *reinterpret_cast<const float4 *>(p + 4);
+    return f;
+}
+// columns of the image as the first operand: column 32 db + lane % 32; element e is row row0 + (e & 3) + 8 (e >> 2) +
+// 4 (lane / 32), the rows that registers 8c .. 8c+7 of a 32x32 result hold for row0 = 16 c
+template <int DP> __device__ __forceinline__ uint4 band_cols(const bf16_t *m, int row0, int db, int lane) {
+    const int row = row0 + 4 * (lane >> 5) + ((lane >> 2) & 3), col = 32 * db + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const uint2 a = lds_read_tr16(m + band_at<bf16_t, DP>(row, col)), b = lds_read_tr16(m + band_at<bf16_t, DP>(row + 8, col));
+    return make_uint4(a.x, a.y, b.x, b.y);
+}
+template <int DP> __device__ __forceinline__ band_t<float>::frag band_cols(const float *m, int row0, int db, int lane) {
+    const float *p = m + band_at<float, DP>(row0 + 4 * (lane >> 5), 32 * db + (lane & 31));
+    constexpr int S = DP + 4;
+    band_t<float>::frag f;
+    f.lo = make_float4(p[0], p[S], p[2 * S], p[3 * S]);
+    f.hi = make_float4(p[8 * S], p[9 * S], p[10 * S], p[11 * S]);
+    return f;
+}
+
+// ---- staging of 64-row tiles by the whole workgroup: global memory -> registers -> LDS -----------------------------
+template <typename T, int DP> struct BandStage {
+    static constexpr int N = DP / 32, SLOTS = DP / 8, STEP = 256 / SLOTS;  // pieces per thread, per row; rows between a thread's pieces
+    typename band_t<T>::frag f[N];
+    // rows row0 .. row0+63 of the slice at `base` (row stride ld); rows from `limit` on read as zero
+    __device__ __forceinline__ void load(const T *base, long long ld, int row0, int limit, int D, int mode) {
+        const int r = threadIdx.x / SLOTS, col = 8 * (threadIdx.x % SLOTS);
+        const T *p = base + (long long)(row0 + r) * ld;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (row0 + r + i * STEP < limit) f[i] = band_load8(p + (long long)(i * STEP) * ld, col, D, mode);
+            else band_clear(f[i]);
+        }
+    }
+    __device__ __forceinline__ void put(T *m) const {
+        const int r = threadIdx.x / SLOTS, slot = threadIdx.x % SLOTS;
+#pragma unroll
+        for (int i = 0; i < N; ++i) band_put<DP>(m, r + i * STEP, slot, f[i]);
+    }
+};
+
+// ---- lengths, tiles -----------------------------------------------------------------------------------------------------
+struct BandSeq {
+    int kn, qn, off;  // keys, query rows, position of row 0
+};
+__device__ __forceinline__ BandSeq band_seq(const BandArgs &a, int b) {
+    BandSeq s;
+    s.kn = a.k_lens ? min(max(a.k_lens[b], 0), a.Lk) : a.Lk;
+    s.qn = a.q_lens ? min(max(a.q_lens[b], 0), a.Lq) : a.Lq;
+    s.off = s.kn - s.qn;
+    return s;
+}
+// Tiles of `size` keys that rows at positions p_lo..p_hi need: the sinks' tiles, then the window's without a gap.
+struct BandTiles {
+    int n_sink, first, count;
+    __device__ __forceinline__ int at(int i) const { return i < n_sink ? i : first + i - n_sink; }
+};
+template <int SIZE> __device__ __forceinline__ BandTiles band_tiles(const BandArgs &a, int kn, int p_lo, int p_hi) {
+    BandTiles t;
+    const int j_hi = min(kn - 1, p_hi + a.right);
+    t.n_sink = t.first = t.count = 0;
+    if (j_hi < 0 || p_hi < p_lo) return t;
+    t.first = max(0, p_lo - a.left) / SIZE;
+    const int last = j_hi / SIZE;
+    if (last < t.first) return t;
+    t.n_sink = min((a.sinks + SIZE - 1) / SIZE, t.first);
+    t.count = t.n_sink + last - t.first + 1;
+    return t;
+}
+
+// the bias of one head by distance, times log2(e), in LDS: entry e is distance sign * (e - M - BAND_MARGIN), clipped
+__device__ __forceinline__ float band_bias_at(const BandArgs &a, int head, int rel) {
+    const int m = min(max(rel, -a.M), a.M) + a.M;
+    const int bucket = min(max(a.buckets[m], 0), a.n_buckets - 1);
+    return a.table[(size_t)bucket * a.Hq + head] * LOG2E;
+}
+__device__ __forceinline__ void band_stage_bias(const BandArgs &a, int head, int sign, float *dst, int threads) {
+    const int n = 2 * (a.M + BAND_MARGIN) + 1;
+    for (int e = threadIdx.x; e < n; e += threads) dst[e] = band_bias_at(a, head, sign * (e - a.M - BAND_MARGIN));
+}
+// Which keys of a tile a row sees: key base + off is visible when off <= hi and (off >= lo or off < first).  Decided with
+// selects on scalars throughout: branches that write single elements of the 16-wide accumulators were seen to be
+// compiled wrongly (an element's store was lost).
+struct BandMask {
+    int hi, lo, first;
+    __device__ __forceinline__ bool sees(int off) const { return (off <= hi) & ((off >= lo) | (off < first)); }
+};
+// one row at position p against keys from `base` on
+__device__ __forceinline__ BandMask band_row_mask(const BandArgs &a, int p, int kn, int base) {
+    return {min(kn - 1, p + a.right) - base, p - a.left - base, a.sinks - base};
+}
+
+// Non-finite values in keys or values that a row does not see must not reach it: a probability of zero times an
+// infinity is not zero.  The tiles' products cannot tell, so a wave that ends with a non-finite result (seen nowhere
+// else) does its tiles again key by key, touching only what each row sees.  Lane = row as in the kernels; m, l and acc
+// as they leave them (l of one lane half).
+template <typename T, int DP, bool BIAS, int SIZE>
+__device__ __forceinline__ void band_careful(const BandArgs &a, const T *qrow, const T *kbase, const T *vbase, int head, int p,
+                                             bool on, int kn, const BandTiles &tiles, int t_begin, int t_end, int t_step, int hh,
+                                             float &m, float &l, f32x16 *acc) {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) acc[db] = band_zero();
+    for (int t = t_begin; t < t_end; t += t_step)
+        for (int j = tiles.at(t) * SIZE; j < min(tiles.at(t) * SIZE + SIZE, kn); ++j) {
+            const bool vis = on & band_row_mask(a, p, kn, j).sees(0);
+            if (!__any(vis)) continue;
+            const T *kr = kbase + (long long)j * a.k.s.l, *vr = vbase + (long long)j * a.v.s.l;
+            float s = 0.f;
+            if (vis)
+                for (int d = hh; d < a.D; d += 2) s = __builtin_fmaf(io<T>::ld(qrow + d), io<T>::ld(kr + d), s);
+            s += __shfl_xor(s, 32, 64);
+            float x = s * a.c;
+            if constexpr (BIAS) x += vis ? band_bias_at(a, head, j - p) : 0.f;
+            const float mn = vis ? fmaxf(m, x) : m;
+            const float alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            const float e = vis ? __builtin_amdgcn_exp2f(x - mn) : 0.f;
+            m = mn;
+            l = l * alpha + (hh == 0 ? e : 0.f);
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int d = 32 * db + rho(r) + 4 * hh;
+                    const bool take = vis & (d < a.D);
+                    const float v = take ? io<T>::ld(vr + d) : 0.f, sum = __builtin_fmaf(e, v, acc[db][r] * alpha);
+                    acc[db][r] = take ? sum : acc[db][r];
+                }
+        }
+}
+
+int band_make_args(const char *who, const dsw_band_desc *d, BandArgs &a);
+int band_tensor(const char *who, const char *name, const void *p, const dsw_strides *s, int dtype, int D, bool null_ok, BandTensor &t);
+// launches the kernel for few query rows (band_attn_step.hip) and the one that joins its splits
+int band_launch_step(BandArgs &a, int dtype, hipStream_t st);
+// whether a call goes there, and how many row blocks and splits it has
+bool band_step_plan(const dsw_band_desc &d, int &nrb, int &nsplit);
+
+}  // namespace dsw

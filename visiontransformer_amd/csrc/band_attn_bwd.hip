@@ -1,0 +1,423 @@
+// Attention over token sequences, backward (see band_attn.hpp for the mathematics and the register layouts).
+//
+//   delta_i = dout_i . out_i        P = 2^(x - lse)        dS = P (dout v^T - delta)
+//   dq = scale dS k     dk = scale dS^T q     dv = P^T dout     dtable[b, head] = sum of dS over the pairs of bucket b
+//
+// Two kernels that each own what they write, so that no sum depends on the order in which workgroups run: one over
+// key blocks (dk, dv; the query heads that share a key head are walked one after the other and meet in the
+// accumulators), one over row blocks (dq, and the bias gradient by distance).  Both recompute the scores.  Layouts as in
+// the forward: the 16 registers of a tile's P and dS are the second operand of the products that follow.
+#include "band_attn.hpp"
+
+namespace dsw {
+
+// ---- delta: 16 lanes a row ---------------------------------------------------------------------------------------
+template <typename T> __global__ __launch_bounds__(256) void band_attn_delta_kernel(const BandArgs a) {
+    const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int lane = threadIdx.x & 15;
+    const long long rows = (long long)a.B * a.Lq * a.Hq;
+    float s = 0.f;
+    int b = 0, i = 0, h = 0;
+    if (row < rows) {
+        h = (int)(row % a.Hq);
+        const long long t = row / a.Hq;
+        i = (int)(t % a.Lq), b = (int)(t / a.Lq);
+        if (i < band_seq(a, b).qn) {
+            const T *g = band_row<T>(a.dout, b, i, h), *o = band_row<T>(a.out, b, i, h);
+            const float *o32 = a.out32 ? a.out32 + (size_t)row * a.D : nullptr;
+            if (a.dout.mode == 0 && a.out.mode == 0 && a.D % 8 == 0 && o32 == nullptr) {
+                for (int d = 8 * lane; d < a.D; d += 128) {
+                    const float4 g0 = io<T>::ld4(g + d), g1 = io<T>::ld4(g + d + 4), o0 = io<T>::ld4(o + d), o1 = io<T>::ld4(o + d + 4);
+                    s += ((g0.x * o0.x + g0.y * o0.y) + (g0.z * o0.z + g0.w * o0.w)) + ((g1.x * o1.x + g1.y * o1.y) + (g1.z * o1.z + g1.w * o1.w));
+                }
+            } else {
+                for (int d = lane; d < a.D; d += 16) s = __builtin_fmaf(io<T>::ld(g + d), o32 ? o32[d] : io<T>::ld(o + d), s);
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 8; k > 0; k >>= 1) s += __shfl_xor(s, k, 64);
+    if (row < rows && lane == 0) a.delta[((size_t)b * a.Hq + h) * a.Lq + i] = s;
+}
+
+// ---- dk, dv: 128 keys of a workgroup, 32 per wave -----------------------------------------------------------------
+template <typename T, int DP, bool BIAS>
+__global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void band_attn_dkv_kernel(const BandArgs a) {
+    constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE);
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    T *const lds = reinterpret_cast<T *>(smem);                        // [NB][Q | dO]
+    float *const stats = reinterpret_cast<float *>(lds + NB * 2 * ELEMS);  // [NB][lse | delta][64]
+    float *const bias = stats + NB * 2 * BAND_TILE;
+
+    const int nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS;
+    const int idx = xcd_remap(blockIdx.x, gridDim.x);
+    const int kb = idx % nkb, bh = idx / nkb, hk = bh % a.Hkv, b = bh / a.Hkv;
+    const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const BandSeq sq = band_seq(a, b);
+    const int k_lo = kb * BAND_ROWS, k_hi = min(k_lo + BAND_ROWS, sq.kn) - 1;
+    const int j_lo = k_lo + 32 * wave, j_hi = j_lo + 31, j = j_lo + l31;
+    const bool key_on = j < sq.kn;
+
+    // query rows that see a key of this block
+    const int first = max(0, k_lo - a.right - sq.off) / BAND_TILE;
+    const int last_row = k_lo < a.sinks ? sq.qn - 1 : min(sq.qn - 1, k_hi + a.left - sq.off);
+    const int n_tiles = k_lo < sq.kn && last_row >= 0 ? max(0, last_row / BAND_TILE - first + 1) : 0;
+
+    typename band_t<T>::frag kf[DP / 16], vf[DP / 16];
+    const T *const krow = band_row<T>(a.k, b, j, hk), *const vrow = band_row<T>(a.v, b, j, hk);
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        if (key_on) {
+            kf[c] = band_load8(krow, 16 * c + 8 * hh, a.D, a.k.mode);
+            vf[c] = band_load8(vrow, 16 * c + 8 * hh, a.D, a.v.mode);
+        } else {
+            band_clear(kf[c]);
+            band_clear(vf[c]);
+        }
+    }
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) dk[db] = dv[db] = band_zero();
+
+    const int steps = n_tiles * a.G;  // tiles of the first head, of the second, ...
+    BandStage<T, DP> qs, gs;
+    float st = 0.f;
+    auto load = [&](int step) {
+        const int g = step / n_tiles, i0 = (first + step - g * n_tiles) * BAND_TILE, h = hk * a.G + g;
+        qs.load(band_row<T>(a.q, b, 0, h), a.q.s.l, i0, sq.qn, a.D, a.q.mode);
+        gs.load(band_row<T>(a.dout, b, 0, h), a.dout.s.l, i0, sq.qn, a.D, a.dout.mode);
+        if (threadIdx.x < 2 * BAND_TILE) {
+            const int i = i0 + (threadIdx.x & (BAND_TILE - 1));
+            const float *src = (threadIdx.x < BAND_TILE ? a.lse : a.delta) + ((size_t)b * a.Hq + h) * a.Lq;
+            st = i < sq.qn ? src[i] : threadIdx.x < BAND_TILE ? INFINITY : 0.f;
+        }
+    };
+    if (steps) load(0);
+    for (int step = 0; step < steps; ++step) {
+        T *const Q = lds + (NB == 2 ? (step & 1) : 0) * 2 * ELEMS, *const G = Q + ELEMS;
+        float *const S = stats + (NB == 2 ? (step & 1) : 0) * 2 * BAND_TILE;
+        const int g = step / n_tiles, i0 = (first + step - g * n_tiles) * BAND_TILE;
+        if constexpr (NB == 1) lds_barrier();
+        if constexpr (BIAS) {
+            if (step == g * n_tiles) {  // another head's bias
+                lds_barrier();          // the last head's readers are done
+                band_stage_bias(a, hk * a.G + g, -1, bias, 256);
+            }
+        }
+        qs.put(Q);
+        gs.put(G);
+        if (threadIdx.x < 2 * BAND_TILE) S[threadIdx.x] = st;
+        if (step + 1 < steps) load(step + 1);
+        lds_barrier();
+#pragma unroll 1
+        for (int u = 0; u < 2; ++u) {
+            const int r0 = i0 + 32 * u, p_lo = sq.off + r0, p_hi = sq.off + min(r0 + 31, sq.qn - 1);
+            if (r0 >= sq.qn || j_lo >= sq.kn || j_lo > p_hi + a.right || (j_hi < p_lo - a.left && j_lo >= a.sinks)) continue;
+            const bool full = j_hi < sq.kn && j_hi <= p_lo + a.right && (j_lo >= p_hi - a.left || j_hi < a.sinks);
+            f32x16 s = band_zero(), dp = band_zero();
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) s = band_mma(band_rows<DP>(Q, 32 * u + l31, c, hh), kf[c], s);
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) dp = band_mma(band_rows<DP>(G, 32 * u + l31, c, hh), vf[c], dp);
+            float bu = 0.f;
+            bool near = false;
+            if constexpr (BIAS) {
+                near = j_lo - p_hi < a.M && j_hi - p_lo > -a.M;
+                if (!near) bu = bias[j_lo > p_hi ? 0 : 2 * (a.M + BAND_MARGIN)];
+            }
+            const float *br = bias + (p_lo + 4 * hh - j + a.M + BAND_MARGIN);
+            // the mask from the key's side: position p sees key j when p >= j - right and (p <= j + left or j < sinks)
+            const int p_min = key_on ? j - a.right - p_lo - 4 * hh : BAND_FAR, p_max = j < a.sinks ? BAND_FAR : j + a.left - p_lo - 4 * hh;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float4 ls = *reinterpret_cast<const float4 *>(S + 32 * u + 8 * k + 4 * hh);
+                const float4 de = *reinterpret_cast<const float4 *>(S + BAND_TILE + 32 * u + 8 * k + 4 * hh);
+                const float lse[4] = {ls.x, ls.y, ls.z, ls.w}, del[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * k + e;
+                    float add = bu;
+                    if constexpr (BIAS) {
+                        if (near) add = br[rho(r)];
+                    }
+                    float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, add - lse[e]));
+                    if (!full) pr = (int)(rho(r) >= p_min) & (int)(rho(r) <= p_max) ? pr : 0.f;
+                    s[r] = pr;
+                    dp[r] = pr == 0.f ? 0.f : pr * (dp[r] - del[e]);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                typename band_t<T>::frag pf, sf;
+                band_pack(s, k, pf);
+                band_pack(dp, k, sf);
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db) {
+                    dv[db] = band_mma(band_cols<DP>(G, 32 * u + 16 * k, db, lane), pf, dv[db]);
+                    dk[db] = band_mma(band_cols<DP>(Q, 32 * u + 16 * k, db, lane), sf, dk[db]);
+                }
+            }
+        }
+    }
+    // (keys behind the sequence: their P and dS are zero, and so are these rows)
+    const bool store = j < a.Lk;
+    band_store_row<T, DP>(const_cast<T *>(band_row<T>(a.dk, b, j, hk)), dk, a.scale, a.D, a.dk.mode, hh, store);
+    band_store_row<T, DP>(const_cast<T *>(band_row<T>(a.dv, b, j, hk)), dv, 1.f, a.D, a.dv.mode, hh, store);
+}
+
+// ---- dq: 128 rows of a workgroup, 32 per wave; bias gradient by distance ---------------------------------------------
+template <typename T, int DP, bool BIAS, bool DTABLE>
+__global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void band_attn_dq_kernel(const BandArgs a) {
+    constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE);
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    T *const lds = reinterpret_cast<T *>(smem);  // [NB][K | V]
+    float *const bias = reinterpret_cast<float *>(lds + NB * 2 * ELEMS);
+    const int BL = 2 * (a.M + BAND_MARGIN) + 1;
+    float *const sums = bias + BL;  // [4 waves][2 lane halves][BL]: dS by distance
+
+    const int nqb = (a.Lq + BAND_ROWS - 1) / BAND_ROWS;
+    const int idx = xcd_remap(blockIdx.x, gridDim.x);
+    const int g = idx % a.G, rest = idx / a.G;
+    const int qb = nqb - 1 - rest % nqb, bh = rest / nqb;
+    const int hk = bh % a.Hkv, b = bh / a.Hkv, h = hk * a.G + g;
+    const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const BandSeq sq = band_seq(a, b);
+    const int i_lo = qb * BAND_ROWS, i0 = i_lo + 32 * wave, i = i0 + l31;
+    const bool row_on = i < sq.qn, wave_on = i0 < sq.qn;
+    const int p = sq.off + i, w_lo = sq.off + i0, w_hi = sq.off + min(i0 + 31, sq.qn - 1);
+    const BandTiles tiles = band_tiles<BAND_TILE>(a, sq.kn, sq.off + i_lo, sq.off + min(i_lo + BAND_ROWS, sq.qn) - 1);
+
+    const T *const kbase = band_row<T>(a.k, b, 0, hk), *const vbase = band_row<T>(a.v, b, 0, hk);
+    if constexpr (BIAS) band_stage_bias(a, h, 1, bias, 256);
+    if constexpr (DTABLE) {
+        for (int e = threadIdx.x; e < 8 * BL; e += 256) sums[e] = 0.f;
+    }
+    typename band_t<T>::frag qf[DP / 16], gf[DP / 16];
+    const T *const qrow = band_row<T>(a.q, b, i, h), *const grow = band_row<T>(a.dout, b, i, h);
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        if (row_on) {
+            qf[c] = band_load8(qrow, 16 * c + 8 * hh, a.D, a.q.mode);
+            gf[c] = band_load8(grow, 16 * c + 8 * hh, a.D, a.dout.mode);
+        } else {
+            band_clear(qf[c]);
+            band_clear(gf[c]);
+        }
+    }
+    const size_t at = ((size_t)b * a.Hq + h) * a.Lq + i;
+    const float lse = row_on ? a.lse[at] : INFINITY, del = row_on ? a.delta[at] : 0.f;
+    f32x16 dq[DP / 32];
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) dq[db] = band_zero();
+    float far_lo = 0.f, far_hi = 0.f;
+
+    BandStage<T, DP> ks, vs;
+    if (tiles.count) {
+        const int j0 = tiles.at(0) * BAND_TILE;
+        ks.load(kbase, a.k.s.l, j0, sq.kn, a.D, a.k.mode);
+        vs.load(vbase, a.v.s.l, j0, sq.kn, a.D, a.v.mode);
+    }
+    for (int it = 0; it < tiles.count; ++it) {
+        T *const K = lds + (NB == 2 ? (it & 1) : 0) * 2 * ELEMS, *const V = K + ELEMS;
+        if constexpr (NB == 1) lds_barrier();
+        ks.put(K);
+        vs.put(V);
+        if (it + 1 < tiles.count) {
+            const int j1 = tiles.at(it + 1) * BAND_TILE;
+            ks.load(kbase, a.k.s.l, j1, sq.kn, a.D, a.k.mode);
+            vs.load(vbase, a.v.s.l, j1, sq.kn, a.D, a.v.mode);
+        }
+        lds_barrier();
+#pragma unroll 1
+        for (int u = 0; u < 2; ++u) {
+            const int j0 = tiles.at(it) * BAND_TILE + 32 * u, j9 = j0 + 31;
+            if (!wave_on || j0 >= sq.kn || j0 > w_hi + a.right || (j9 < w_lo - a.left && j0 >= a.sinks)) continue;
+            const bool full = j9 < sq.kn && j9 <= w_lo + a.right && (j0 >= w_hi - a.left || j9 < a.sinks);
+            f32x16 s = band_zero(), dp = band_zero();
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) s = band_mma(band_rows<DP>(K, 32 * u + l31, c, hh), qf[c], s);
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) dp = band_mma(band_rows<DP>(V, 32 * u + l31, c, hh), gf[c], dp);
+            float bu = 0.f;
+            bool near = false;
+            if constexpr (BIAS) {
+                near = j9 - w_lo > -a.M && j0 - w_hi < a.M;
+                if (!near) bu = bias[j0 > w_hi ? BL - 1 : 0];
+            }
+            const int e0 = j0 + 4 * hh - p + a.M + BAND_MARGIN;
+            const BandMask mask = band_row_mask(a, p, sq.kn, j0 + 4 * hh);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float add = bu;
+                if constexpr (BIAS) {
+                    if (near) add = bias[e0 + rho(r)];
+                }
+                float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, add - lse));
+                if (!full) pr = mask.sees(rho(r)) ? pr : 0.f;
+                s[r] = pr == 0.f ? 0.f : pr * (dp[r] - del);
+            }
+            if constexpr (DTABLE) {
+                // the 32 lanes of a half hold one key each time: 32 different distances, in a table that only this wave's
+                // half adds to, one instruction after the other - the order of the sums is fixed
+                if (near) {
+                    float *const mine = sums + (2 * wave + hh) * BL + e0;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        __hip_atomic_fetch_add(mine + rho(r), s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                } else {
+                    float t = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) t += s[r];
+                    if (j0 > w_hi) far_hi += t;
+                    else far_lo += t;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                typename band_t<T>::frag sf;
+                band_pack(s, k, sf);
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db) dq[db] = band_mma(band_cols<DP>(K, 32 * u + 16 * k, db, lane), sf, dq[db]);
+            }
+        }
+    }
+    band_store_row<T, DP>(const_cast<T *>(band_row<T>(a.dq, b, i, h)), dq, a.scale, a.D, a.dq.mode, hh, i < a.Lq);
+
+    if constexpr (DTABLE) {
+        // clipped distances meet in the two end entries, then the eight tables are added
+        far_lo = wave_sum(far_lo);
+        far_hi = wave_sum(far_hi);
+        __syncthreads();
+        if (threadIdx.x < 16) {
+            float *const t = sums + (threadIdx.x >> 1) * BL;
+            const int e = threadIdx.x & 1 ? BL - 1 - BAND_MARGIN : BAND_MARGIN, dir = threadIdx.x & 1 ? 1 : -1;
+            float v = t[e];
+            for (int k = 1; k <= BAND_MARGIN; ++k) v += t[e + dir * k];
+            t[e] = v;
+        }
+        __syncthreads();
+        if (lane == 0) {
+            sums[2 * wave * BL + BAND_MARGIN] += far_lo;
+            sums[2 * wave * BL + BL - 1 - BAND_MARGIN] += far_hi;
+        }
+        __syncthreads();
+        const int n = 2 * a.M + 1;
+        float *const dst = a.partial + ((size_t)h * a.B * nqb + (size_t)b * nqb + qb) * n;
+        for (int e = threadIdx.x; e < n; e += 256) {
+            float v = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v += sums[k * BL + BAND_MARGIN + e];
+            dst[e] = v;
+        }
+    }
+}
+
+// by_distance[head][2 M + 1] = sum over the head's row blocks
+__global__ __launch_bounds__(1024) void band_attn_distance_kernel(const float *__restrict__ partial, int rows, int n, float *__restrict__ dst) {
+    __shared__ float red[32][33];
+    int col;
+    float total;
+    if (column_sum_32<32>(partial + (size_t)blockIdx.y * rows * n, rows, n, red, col, total)) dst[(size_t)blockIdx.y * n + col] = total;
+}
+// one wave per (bucket, head)
+__global__ __launch_bounds__(64) void band_attn_table_kernel(const float *__restrict__ by_distance, const int *__restrict__ buckets, int n,
+                                                             int n_buckets, int heads, float *__restrict__ d_table) {
+    const int bucket = blockIdx.x, h = blockIdx.y;
+    float v = 0.f;
+    for (int e = threadIdx.x; e < n; e += 64)
+        if (min(max(buckets[e], 0), n_buckets - 1) == bucket) v += by_distance[(size_t)h * n + e];
+    v = wave_sum(v);
+    if (threadIdx.x == 0) d_table[(size_t)bucket * heads + h] = v;
+}
+
+template <typename K> static int allow_lds(K kern, size_t lds) {
+    if (lds <= 65536) return DSW_OK;
+    hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    return e == hipSuccess ? DSW_OK : fail(DSW_ELAUNCH, "dsw_band_attn_bwd: %zu bytes of LDS: %s", lds, hipGetErrorString(e));
+}
+
+template <typename T, int DP, bool BIAS, bool DTABLE> static int launch_bwd(const BandArgs &a, hipStream_t st) {
+    const size_t images = (size_t)band_t<T>::nbuf(DP) * 2 * band_t<T>::template elems<DP>(BAND_TILE) * sizeof(T);
+    const size_t bl = BIAS ? (2 * (a.M + BAND_MARGIN) + 1) * sizeof(float) : 0;
+    if (a.Lk) {
+        const size_t lds = images + (size_t)band_t<T>::nbuf(DP) * 2 * BAND_TILE * sizeof(float) + bl;
+        auto kern = band_attn_dkv_kernel<T, DP, BIAS>;
+        if (int rc = allow_lds(kern, lds)) return rc;
+        kern<<<dim3((unsigned)((long long)a.B * a.Hkv * ((a.Lk + BAND_ROWS - 1) / BAND_ROWS))), 256, lds, st>>>(a);
+        if (int rc = check_launch("dsw_band_attn_bwd (dk, dv)")) return rc;
+    }
+    if (a.Lq) {
+        const size_t lds = images + bl + (DTABLE ? 8 * bl : 0);
+        auto kern = band_attn_dq_kernel<T, DP, BIAS, DTABLE>;
+        if (int rc = allow_lds(kern, lds)) return rc;
+        kern<<<dim3((unsigned)((long long)a.B * a.Hq * ((a.Lq + BAND_ROWS - 1) / BAND_ROWS))), 256, lds, st>>>(a);
+        if (int rc = check_launch("dsw_band_attn_bwd (dq)")) return rc;
+    }
+    return DSW_OK;
+}
+
+static size_t round16(size_t n) { return (n + 3) & ~(size_t)3; }
+
+}  // namespace dsw
+
+using namespace dsw;
+
+#define DSW_BAND_DISPATCH(dtype, D, T, DP, ...)                                   \
+    DSW_DISPATCH_DTYPE(dtype, T, {                                                \
+        if ((D) <= 32) { constexpr int DP = 32; __VA_ARGS__; }                    \
+        else if ((D) <= 64) { constexpr int DP = 64; __VA_ARGS__; }               \
+        else { constexpr int DP = 128; __VA_ARGS__; }                             \
+    })
+
+extern "C" size_t dsw_band_attn_bwd_workspace(const dsw_band_desc *d) {
+    BandArgs a;
+    if (band_make_args("dsw_band_attn_bwd_workspace", d, a)) return 0;
+    size_t n = round16((size_t)a.B * a.Hq * a.Lq);
+    if (a.table) n += (size_t)a.Hq * ((size_t)a.B * ((a.Lq + BAND_ROWS - 1) / BAND_ROWS) + 1) * (2 * a.M + 1);
+    return n * sizeof(float);
+}
+
+extern "C" int dsw_band_attn_bwd(const dsw_band_desc *d, const void *q, const dsw_strides *sq, const void *k, const dsw_strides *sk,
+                                 const void *v, const dsw_strides *sv, const void *out, const dsw_strides *so, const float *out32,
+                                 const void *dout, const dsw_strides *sdo, const float *lse, void *dq, const dsw_strides *sdq, void *dk,
+                                 const dsw_strides *sdk, void *dv, const dsw_strides *sdv, float *d_table, void *workspace,
+                                 size_t workspace_bytes, void *stream) {
+    const char *who = "dsw_band_attn_bwd";
+    BandArgs a;
+    int rc = band_make_args(who, d, a);
+    if (rc) return rc;
+    if (a.B == 0 || a.Hq == 0) return DSW_OK;
+    const bool no_rows = a.Lq == 0, no_keys = a.Lk == 0;
+    if ((rc = band_tensor(who, "q", q, sq, d->dtype, a.D, no_rows, a.q)) || (rc = band_tensor(who, "k", k, sk, d->dtype, a.D, no_keys, a.k)) ||
+        (rc = band_tensor(who, "v", v, sv, d->dtype, a.D, no_keys, a.v)) || (rc = band_tensor(who, "out", out, so, d->dtype, a.D, no_rows, a.out)) ||
+        (rc = band_tensor(who, "dout", dout, sdo, d->dtype, a.D, no_rows, a.dout)) || (rc = band_tensor(who, "dq", dq, sdq, d->dtype, a.D, no_rows, a.dq)) ||
+        (rc = band_tensor(who, "dk", dk, sdk, d->dtype, a.D, no_keys, a.dk)) || (rc = band_tensor(who, "dv", dv, sdv, d->dtype, a.D, no_keys, a.dv)))
+        return rc;
+    DSW_REQUIRE(no_rows || lse, "%s: null lse", who);
+    DSW_REQUIRE(d_table == nullptr || a.table, "%s: a gradient for a table that is not there", who);
+    const size_t need = dsw_band_attn_bwd_workspace(d);
+    DSW_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "%s: workspace of %zu bytes, %zu are needed", who, workspace_bytes, need);
+    a.lse = const_cast<float *>(lse);
+    a.out32 = const_cast<float *>(out32);
+    a.delta = static_cast<float *>(workspace);
+    a.partial = a.delta + round16((size_t)a.B * a.Hq * a.Lq);
+    hipStream_t st = as_stream(stream);
+    if (!no_rows) {
+        const long long rows = (long long)a.B * a.Lq * a.Hq;
+        const dim3 grid((unsigned)((rows + 15) / 16));
+        DSW_DISPATCH_DTYPE(d->dtype, T, (band_attn_delta_kernel<T><<<grid, 256, 0, st>>>(a)));
+        if ((rc = check_launch("dsw_band_attn_bwd (delta)"))) return rc;
+    }
+    DSW_BAND_DISPATCH(d->dtype, a.D, T, DP, {
+        rc = d_table ? launch_bwd<T, DP, true, true>(a, st) : a.table ? launch_bwd<T, DP, true, false>(a, st) : launch_bwd<T, DP, false, false>(a, st);
+    });
+    if (rc || d_table == nullptr) return rc;
+    const int n = 2 * a.M + 1, rows = a.B * ((a.Lq + BAND_ROWS - 1) / BAND_ROWS);
+    float *by_distance = a.partial + (size_t)a.Hq * rows * n;
+    band_attn_distance_kernel<<<dim3((n + 31) / 32, a.Hq), 1024, 0, st>>>(a.partial, rows, n, by_distance);
+    if ((rc = check_launch("dsw_band_attn_bwd (distances)"))) return rc;
+    band_attn_table_kernel<<<dim3(a.n_buckets, a.Hq), 64, 0, st>>>(by_distance, a.buckets, n, a.n_buckets, a.Hq, d_table);
+    return check_launch("dsw_band_attn_bwd (table)");
+}

@@ -1,0 +1,241 @@
+// Attention over token sequences for few query rows: new tokens over a cache (see band_attn.hpp for the mathematics).
+//
+// Bound by the bytes of the keys and values, which every query head of a shared key head reads: the Lq * G rows of a key
+// head sit side by side on the lane axis of one 32x32 tile (32 rows to a block).  A workgroup takes one block and one of
+// `nsplit` shares of the key tiles (32 keys); its four waves take every fourth tile each, on their own - K straight
+// from memory into the operand registers, V through a piece of LDS that only the wave touches, no barrier in the loop,
+// the next tile under way meanwhile - and meet at the end.  With more than one share the sums, maxima and denominators
+// go to the workspace, and a second kernel joins them in the order of the shares.
+#include "band_attn.hpp"
+
+namespace dsw {
+
+constexpr int STEP_KEYS = 32;
+
+template <typename T, int DP, bool BIAS>
+__global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void band_attn_step_kernel(const BandArgs a) {
+    constexpr int ELEMS = band_t<T>::template elems<DP>(STEP_KEYS);
+    constexpr int SLOTS = DP / 8, NV = STEP_KEYS * SLOTS / 64, STEP = 64 / SLOTS;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    T *const V = reinterpret_cast<T *>(smem) + wave * ELEMS;
+
+    const int sp = blockIdx.x % a.nsplit, rest = blockIdx.x / a.nsplit;
+    const int rb = rest % a.nrb, bh = rest / a.nrb, hk = bh % a.Hkv, b = bh / a.Hkv;
+    const BandSeq sq = band_seq(a, b);
+    const int row = rb * 32 + l31, R = a.Lq * a.G;
+    const int i = row / a.G, h = hk * a.G + row - i * a.G;
+    const bool row_on = row < R && i < sq.qn;
+    const int p = sq.off + i;
+    const int i_lo = rb * 32 / a.G, i_hi = min((rb * 32 + 31) / a.G, sq.qn - 1);
+    const int p_lo = sq.off + i_lo, p_hi = sq.off + i_hi;
+    const BandTiles tiles = band_tiles<STEP_KEYS>(a, sq.kn, p_lo, p_hi);
+    const int share = (tiles.count + a.nsplit - 1) / a.nsplit, t_end = min((sp + 1) * share, tiles.count);
+    const int t_begin = sp * share + wave;
+
+    const T *const qrow = band_row<T>(a.q, b, i, h);
+    const T *const kbase = band_row<T>(a.k, b, 0, hk);
+    const T *const vbase = band_row<T>(a.v, b, 0, hk);
+    typename band_t<T>::frag qf[DP / 16];
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        if (row_on) qf[c] = band_load8(qrow, 16 * c + 8 * hh, a.D, a.q.mode);
+        else band_clear(qf[c]);
+    }
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) o[db] = band_zero();
+    float m = -INFINITY, l = 0.f;
+
+    typename band_t<T>::frag kf[DP / 16], vf[NV];
+    auto load = [&](int j0) {
+        // (rows that no query of the block sees are not read: they may be uninitialised parts of a cache)
+        auto wanted = [&](int j) { return j < sq.kn && j <= p_hi + a.right && (j >= p_lo - a.left || j < a.sinks); };
+        const int j = j0 + l31;
+        const T *kr = kbase + (long long)j * a.k.s.l;
+        const bool on = wanted(j);
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+            if (on) kf[c] = band_load8(kr, 16 * c + 8 * hh, a.D, a.k.mode);
+            else band_clear(kf[c]);
+        }
+        const int r = lane / SLOTS, col = 8 * (lane % SLOTS);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const int jv = j0 + r + n * STEP;
+            if (wanted(jv)) vf[n] = band_load8(vbase + (long long)jv * a.v.s.l, col, a.D, a.v.mode);
+            else band_clear(vf[n]);
+        }
+    };
+    if (t_begin < t_end) load(tiles.at(t_begin) * STEP_KEYS);
+    for (int t = t_begin; t < t_end; t += 4) {
+        const int j0 = tiles.at(t) * STEP_KEYS;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) band_put<DP>(V, lane / SLOTS + n * STEP, lane % SLOTS, vf[n]);
+        f32x16 s = band_zero();
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) s = band_mma(kf[c], qf[c], s);
+        if (t + 4 < t_end) load(tiles.at(t + 4) * STEP_KEYS);
+        const BandMask mask = band_row_mask(a, p, sq.kn, j0 + 4 * hh);
+        float x = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int j = j0 + rho(r) + 4 * hh;
+            float y = s[r] * a.c;
+            if constexpr (BIAS) y += row < R ? band_bias_at(a, h, j - p) : 0.f;
+            s[r] = mask.sees(rho(r)) ? y : -INFINITY;
+            x = fmaxf(x, s[r]);
+        }
+        x = max_across_halves(x);
+        if (__any(x > m + 8.f)) {
+            const float mn = fmaxf(m, x), alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+        }
+        const float shift = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(s[r] - shift);
+            l += s[r];
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            typename band_t<T>::frag pf;
+            band_pack(s, k, pf);
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db) o[db] = band_mma(band_cols<DP>(V, 16 * k, db, lane), pf, o[db]);
+        }
+    }
+    float bad = 0.f;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bad = __builtin_fmaf(o[db][r], 0.f, bad);
+    if (__any(bad != 0.f))
+        band_careful<T, DP, BIAS, STEP_KEYS>(a, qrow, kbase, vbase, h, p, row_on, sq.kn, tiles, t_begin, t_end, 4, hh, m, l, o);
+
+    // the four waves meet: maxima and denominators first, then the sums, scaled to the common maximum
+    l += __shfl_xor(l, 32, 64);
+    __syncthreads();
+    const int nrow = min(32, R - rb * 32);
+    float *const ml = reinterpret_cast<float *>(smem);  // [4][32][2]
+    float *const os = ml + 4 * 32 * 2;                   // [4][nrow][D]
+    if (hh == 0) ml[(wave * 32 + l31) * 2] = m, ml[(wave * 32 + l31) * 2 + 1] = l;
+    __syncthreads();
+    float mt = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, ml[(w * 32 + l31) * 2]);
+    const float mul = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mt);
+    if (l31 < nrow) {
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = 32 * db + rho(r) + 4 * hh;
+                // (a wave without visible keys holds zeros, or what a row it must not see left there)
+                if (d < a.D) os[(wave * nrow + l31) * a.D + d] = m == -INFINITY ? 0.f : o[db][r] * mul;
+            }
+    }
+    __syncthreads();
+    const int n = nrow * a.D;
+    for (int e = threadIdx.x; e < n; e += 256) {
+        const int rl = e / a.D, d = e - rl * a.D;
+        float mx = -INFINITY, den = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[(w * 32 + rl) * 2]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float mw = ml[(w * 32 + rl) * 2];
+            den += mw == -INFINITY ? 0.f : ml[(w * 32 + rl) * 2 + 1] * __builtin_amdgcn_exp2f(mw - mx);
+        }
+        const float sum = (os[e] + os[n + e]) + (os[2 * n + e] + os[3 * n + e]);
+        if (a.nsplit == 1) {
+            const int ro = rb * 32 + rl, io_ = ro / a.G, ho = hk * a.G + ro - io_ * a.G;
+            io<T>::st(const_cast<T *>(band_row<T>(a.out, b, io_, ho)) + d, den == 0.f || io_ >= sq.qn ? 0.f : sum / den);
+        } else {
+            float *const ws = a.partial + (((size_t)bh * a.nrb + rb) * a.nsplit + sp) * 32 * (a.D + 2);
+            ws[rl * (a.D + 2) + d] = sum;
+            if (d == 0) ws[rl * (a.D + 2) + a.D] = mx, ws[rl * (a.D + 2) + a.D + 1] = den;
+        }
+    }
+}
+
+// one wave joins the shares of one row
+template <typename T> __global__ __launch_bounds__(256) void band_attn_join_kernel(const BandArgs a) {
+    const long long row_all = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, R = a.Lq * a.G;
+    if (row_all >= (long long)a.B * a.Hkv * R) return;
+    const int bh = (int)(row_all / R), row = (int)(row_all - (long long)bh * R), b = bh / a.Hkv, hk = bh % a.Hkv;
+    const int i = row / a.G, h = hk * a.G + row - i * a.G, W = a.D + 2;
+    const float *ws = a.partial + (((size_t)bh * a.nrb + row / 32) * a.nsplit) * 32 * W + (row & 31) * W;
+    float mt = -INFINITY;
+    for (int s = lane; s < a.nsplit; s += 64) mt = fmaxf(mt, ws[(size_t)s * 32 * W + a.D]);
+    mt = wave_max(mt);
+    float den = 0.f, o0 = 0.f, o1 = 0.f;
+    for (int s = 0; s < a.nsplit; ++s) {
+        const float *r = ws + (size_t)s * 32 * W;
+        const float ms = r[a.D];
+        if (ms == -INFINITY) continue;
+        const float f = __builtin_amdgcn_exp2f(ms - mt);
+        den = __builtin_fmaf(r[a.D + 1], f, den);
+        if (lane < a.D) o0 = __builtin_fmaf(r[lane], f, o0);
+        if (lane + 64 < a.D) o1 = __builtin_fmaf(r[lane + 64], f, o1);
+    }
+    const BandSeq sq = band_seq(a, b);
+    const bool off = den == 0.f || i >= sq.qn;
+    T *out = const_cast<T *>(band_row<T>(a.out, b, i, h));
+    if (lane < a.D) io<T>::st(out + lane, off ? 0.f : o0 / den);
+    if (lane + 64 < a.D) io<T>::st(out + lane + 64, off ? 0.f : o1 / den);
+}
+
+// Few rows: at most 32 rows of a key head, or too few of the other kernel's workgroups to fill the chip while the rows
+// of a key head fit four blocks.
+bool band_step_plan(const dsw_band_desc &d, int &nrb, int &nsplit) {
+    if (d.B == 0 || d.Lq == 0 || d.Hq == 0 || d.Hkv == 0) return false;
+    const long long R = (long long)d.Lq * (d.Hq / d.Hkv);
+    if (R > 128) return false;
+    if (R > 32 && (long long)d.B * d.Hq * ((d.Lq + BAND_ROWS - 1) / BAND_ROWS) >= 256) return false;
+    nrb = (int)((R + 31) / 32);
+    const long long span = d.left < 0 ? d.Lk : (long long)d.left + d.Lq + (d.right > 0 ? d.right : 0) + d.sinks + 2 * STEP_KEYS;
+    const long long tiles = ((span < d.Lk ? span : d.Lk) + STEP_KEYS - 1) / STEP_KEYS, units = (long long)d.B * d.Hkv * nrb;
+    long long n = (1024 + units - 1) / units;   // four workgroups a CU
+    const long long most = (tiles + 7) / 8;      // two tiles per wave at least
+    n = n < most ? n : most;
+    nsplit = (int)(n < 1 ? 1 : n > 512 ? 512 : n);
+    return true;
+}
+
+template <typename T, int DP, bool BIAS> static int launch_step(const BandArgs &a, hipStream_t st) {
+    const int R = a.Lq * a.G, nrow = R < 32 ? R : 32;
+    const size_t tile = (size_t)4 * band_t<T>::template elems<DP>(STEP_KEYS) * sizeof(T);
+    const size_t meet = (size_t)(4 * 32 * 2 + 4 * nrow * a.D) * sizeof(float), lds = tile > meet ? tile : meet;
+    auto kern = band_attn_step_kernel<T, DP, BIAS>;
+    if (lds > 65536) {
+        hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return fail(DSW_ELAUNCH, "dsw_band_attn_fwd: %zu bytes of LDS: %s", lds, hipGetErrorString(e));
+    }
+    const long long grid = (long long)a.B * a.Hkv * a.nrb * a.nsplit;
+    if (grid >= (1LL << 31)) return fail(DSW_EUNSUPPORTED, "dsw_band_attn_fwd: %lld workgroups", grid);
+    kern<<<dim3((unsigned)grid), 256, lds, st>>>(a);
+    int rc = check_launch("dsw_band_attn_fwd");
+    if (rc || a.nsplit == 1) return rc;
+    const long long rows = (long long)a.B * a.Hkv * R;
+    band_attn_join_kernel<T><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(a);
+    return check_launch("dsw_band_attn_fwd (join)");
+}
+
+int band_launch_step(BandArgs &a, int dtype, hipStream_t st) {
+    DSW_DISPATCH_DTYPE(dtype, T, {
+        if (a.D <= 32) return a.table ? launch_step<T, 32, true>(a, st) : launch_step<T, 32, false>(a, st);
+        if (a.D <= 64) return a.table ? launch_step<T, 64, true>(a, st) : launch_step<T, 64, false>(a, st);
+        return a.table ? launch_step<T, 128, true>(a, st) : launch_step<T, 128, false>(a, st);
+    });
+    return DSW_OK;
+}
+
+}  // namespace dsw

@@ -1,0 +1,448 @@
+// Norm of every head's query and key row with the rotation by position behind it, one pass forward and one backward.
+//
+//   x: a head's D columns of one token      r = 1 / sqrt(mean(x^2) + eps)      u = w * x * r
+//   y = u with its first 2 * axes * pairs columns turned pair by pair: pair c = a * pairs + i stands in columns
+//   (c, c + axes * pairs), or (2c, 2c + 1) when interleaved, and turns by pos[token][a] * freqs[a][i]
+//   backward: du = dy turned back, dw = sum over rows of du * x * r, dn = du * w, dx = r (dn - x r mean(dn * x r))
+//
+// Memory-bound: forward reads x and writes y, backward reads x and dy and writes dx, with some 20 vector instructions
+// per 16 bytes.  The angles need the accurate path (positions in the millions: the product with the frequency is
+// taken in 64 bits and reduced to a part of one turn before sine and cosine), which costs more than a row's norm; they
+// are the same for all heads of a token, so a workgroup takes all heads of a few tokens and keeps the sines and cosines
+// in LDS.  A row is held by RL lanes in units of two Q-element pieces, chosen so that both columns of a pair are
+// in one lane: the rotation needs no exchange, the norm log2(RL) of them.  Q is the widest piece (16 bytes at most)
+// that the head dim, the pair count, the strides and the addresses allow; Q = 1 takes any of them.
+#include "common.hpp"
+
+namespace dsw {
+
+struct RotOperand {
+    const void *p;
+    dsw_strides s;
+};
+struct RotArgs {
+    RotOperand x[2], dy[2];  // q, k
+    RotOperand y[2];         // forward: results, backward: dx
+    const float *w[2];       // null: ones
+    const float *freqs;
+    const void *pos;         // int32 or int64 [.., axes], or null: the token's index in its sequence on every axis
+    int pos_bytes;
+    long long pos_batch;     // elements between the positions of two sequences (0: shared)
+    float *partial;          // backward: [blocks][2][D] or null
+    long long tokens;
+    int L, Hq, Hkv, D, axes, pairs, rl_log, units, tpw;
+    float eps;
+};
+
+template <typename T, int Q> struct piece;  // Q consecutive elements, aligned to their size (16 bytes at most)
+template <> struct piece<bf16_t, 8> {
+    __device__ static __forceinline__ void ld(const bf16_t *p, float *v) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+    __device__ static __forceinline__ void st(bf16_t *p, const float *v) {
+        *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    }
+};
+template <> struct piece<bf16_t, 4> {
+    __device__ static __forceinline__ void ld(const bf16_t *p, float *v) {
+        const float4 f = io<bf16_t>::ld4(p);
+        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    }
+    __device__ static __forceinline__ void st(bf16_t *p, const float *v) { io<bf16_t>::st4(p, make_float4(v[0], v[1], v[2], v[3])); }
+};
+template <> struct piece<bf16_t, 2> {
+    __device__ static __forceinline__ void ld(const bf16_t *p, float *v) {
+        const uint32_t u = *reinterpret_cast<const uint32_t *>(p);
+        v[0] = __uint_as_float(u << 16), v[1] = __uint_as_float(u & 0xffff0000u);
+    }
+    __device__ static __forceinline__ void st(bf16_t *p, const float *v) { *reinterpret_cast<uint32_t *>(p) = pack_bf16(v[0], v[1]); }
+};
+template <> struct piece<float, 4> {
+    __device__ static __forceinline__ void ld(const float *p, float *v) {
+        const float4 f = *reinterpret_cast<const float4 *>(p);
+        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    }
+    __device__ static __forceinline__ void st(float *p, const float *v) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+};
+template <> struct piece<float, 2> {
+    __device__ static __forceinline__ void ld(const float *p, float *v) {
+        const float2 f = *reinterpret_cast<const float2 *>(p);
+        v[0] = f.x, v[1] = f.y;
+    }
+    __device__ static __forceinline__ void st(float *p, const float *v) { *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]); }
+};
+template <typename T> struct piece<T, 1> {
+    __device__ static __forceinline__ void ld(const T *p, float *v) { v[0] = io<T>::ld(p); }
+    __device__ static __forceinline__ void st(T *p, const float *v) { io<T>::st(p, v[0]); }
+};
+
+constexpr int ROT_THREADS = 256;
+
+// cosines and sines of nt tokens' angles, [token][pair], and the two weights [2][D] behind them (forward and backward
+// read both per row)
+__device__ __forceinline__ void rot_tables(const RotArgs &a, long long token0, int nt, float2 *cs, float *w) {
+    const int n = a.axes * a.pairs;
+    for (int e = threadIdx.x; e < nt * n; e += ROT_THREADS) {
+        const int t = e / n, c = e - t * n, ax = c / a.pairs;
+        const long long token = token0 + t, b = token / a.L;
+        const int l = (int)(token - b * a.L);
+        const long long at = b * a.pos_batch + (long long)l * a.axes + ax;
+        const long long pos = !a.pos ? l : a.pos_bytes == 8 ? static_cast<const long long *>(a.pos)[at] : static_cast<const int *>(a.pos)[at];
+        // in turns; two roundings in 64 bits leave less than 2^-24 of a turn up to 2^28 turns
+        double turns = (double)pos * ((double)a.freqs[c] * 0.15915494309189533577);
+        turns -= rint(turns);
+        float s, co;
+        sincospif(2.f * (float)turns, &s, &co);
+        cs[e] = make_float2(co, s);
+    }
+    if (w)
+        for (int e = threadIdx.x; e < 2 * a.D; e += ROT_THREADS) {
+            const float *src = a.w[e >= a.D];
+            w[e] = src ? src[e >= a.D ? e - a.D : e] : 1.f;
+        }
+}
+
+// columns of unit u: two pieces of Q elements; returns whether the second one exists
+template <int Q, bool INTER> __device__ __forceinline__ bool rot_columns(int u, int n, int D, int &ca, int &cb, bool &turned) {
+    turned = Q * u < n;
+    if (turned) {
+        ca = INTER ? 2 * Q * u : Q * u;
+        cb = INTER ? ca + Q : n + Q * u;
+    } else {
+        ca = 2 * n + 2 * (Q * u - n);
+        cb = ca + Q;
+    }
+    return cb < D;
+}
+// turn the pairs of a unit; inv: back
+template <int Q, bool INTER> __device__ __forceinline__ void rot_turn(float *x, const float2 *cs, bool inv) {
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+        const float2 t = cs[i];
+        const float s = inv ? -t.y : t.y;
+        float &p = x[INTER ? 2 * i : i], &q = x[INTER ? 2 * i + 1 : Q + i];
+        const float p0 = p, q0 = q;
+        p = __builtin_fmaf(p0, t.x, -(q0 * s));
+        q = __builtin_fmaf(p0, s, q0 * t.x);
+    }
+}
+
+template <typename T, int Q, int NU, bool INTER>
+__global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_fwd_kernel(const RotArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int n = a.axes * a.pairs, D = a.D, H = a.Hq + a.Hkv;
+    const long long token0 = (long long)blockIdx.x * a.tpw;
+    const int nt = (int)(a.tokens - token0 < a.tpw ? a.tokens - token0 : a.tpw);
+    float *w = reinterpret_cast<float *>(smem);
+    float2 *cs = reinterpret_cast<float2 *>(w + ((2 * D + 3) & ~3));
+    const int RL = 1 << a.rl_log, lane = threadIdx.x & (RL - 1), grp = threadIdx.x >> a.rl_log, G = ROT_THREADS >> a.rl_log;
+    const int rows = nt * H;
+    const float inv_d = 1.f / (float)D;
+    constexpr int AHEAD = Q == 8 ? 2 : 1;  // rows whose loads are under way together
+    bool first = true;
+    for (int r0 = grp; first || r0 < rows; r0 += AHEAD * G) {
+        float x[AHEAD][NU][2 * Q];
+        T *dst[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int row = r0 + k * G;
+            dst[k] = nullptr;
+#pragma unroll
+            for (int j = 0; j < NU; ++j)
+#pragma unroll
+                for (int i = 0; i < 2 * Q; ++i) x[k][j][i] = 0.f;
+            if (row >= rows) continue;
+            const int t = row / H;
+            int h = row - t * H;
+            const int which = h >= a.Hq;
+            h -= which ? a.Hq : 0;
+            const long long token = token0 + t, b = token / a.L, l = token - b * a.L;
+            const dsw_strides &si = a.x[which].s, &so = a.y[which].s;
+            const T *src = static_cast<const T *>(a.x[which].p) + b * si.b + l * si.l + h * si.h;
+            dst[k] = static_cast<T *>(const_cast<void *>(a.y[which].p)) + b * so.b + l * so.l + h * so.h;
+#pragma unroll
+            for (int j = 0; j < NU; ++j) {
+                const int u = lane + j * RL;
+                int ca, cb;
+                bool turned;
+                if (u < a.units) {
+                    const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
+                    piece<T, Q>::ld(src + ca, x[k][j]);
+                    if (two) piece<T, Q>::ld(src + cb, x[k][j] + Q);
+                }
+            }
+        }
+        if (first) {  // the tables are made while the first rows are on their way
+            rot_tables(a, token0, nt, cs, w);
+            __syncthreads();
+            first = false;
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (dst[k] == nullptr) continue;
+            const int row = r0 + k * G, t = row / H;
+            const float *wr = w + (row - t * H >= a.Hq ? D : 0);
+            float ss = 0.f;
+#pragma unroll
+            for (int j = 0; j < NU; ++j)
+#pragma unroll
+                for (int i = 0; i < 2 * Q; ++i) ss = __builtin_fmaf(x[k][j][i], x[k][j][i], ss);
+            for (int o = RL >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+            const float r = rsqrtf(ss * inv_d + a.eps);
+#pragma unroll
+            for (int j = 0; j < NU; ++j) {
+                const int u = lane + j * RL;
+                if (u >= a.units) continue;
+                int ca, cb;
+                bool turned;
+                const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
+                float *v = x[k][j];
+#pragma unroll
+                for (int i = 0; i < Q; ++i) {
+                    v[i] = v[i] * r * wr[ca + i];
+                    v[Q + i] = two ? v[Q + i] * r * wr[cb + i] : 0.f;
+                }
+                if (turned) rot_turn<Q, INTER>(v, cs + t * n + Q * u, false);
+                piece<T, Q>::st(dst[k] + ca, v);
+                if (two) piece<T, Q>::st(dst[k] + cb, v + Q);
+            }
+        }
+    }
+}
+
+// One workgroup walks token tiles blockIdx.x, + gridDim.x, ...; its share of the weights' gradients stays in registers
+// until the end and leaves as one row of `partial`, so that the sums have a fixed order.
+template <typename T, int Q, int NU, bool INTER>
+__global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_bwd_kernel(const RotArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int n = a.axes * a.pairs, D = a.D;
+    float *w = reinterpret_cast<float *>(smem);
+    float2 *cs = reinterpret_cast<float2 *>(w + ((2 * D + 3) & ~3));
+    const int RL = 1 << a.rl_log, lane = threadIdx.x & (RL - 1), grp = threadIdx.x >> a.rl_log, G = ROT_THREADS >> a.rl_log;
+    const float inv_d = 1.f / (float)D;
+    float dw[2][NU][2 * Q];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int j = 0; j < NU; ++j)
+#pragma unroll
+            for (int i = 0; i < 2 * Q; ++i) dw[m][j][i] = 0.f;
+    const long long tiles = (a.tokens + a.tpw - 1) / a.tpw;
+    for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const long long token0 = tile * a.tpw;
+        const int nt = (int)(a.tokens - token0 < a.tpw ? a.tokens - token0 : a.tpw);
+        __syncthreads();  // the last tile's readers are done
+        rot_tables(a, token0, nt, cs, tile == blockIdx.x ? w : nullptr);
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const int H = m ? a.Hkv : a.Hq, rows = nt * H;
+            const dsw_strides &sx = a.x[m].s, &sg = a.dy[m].s, &so = a.y[m].s;
+            for (int row = grp; row < rows; row += G) {
+                const int t = row / H, h = row - t * H;
+                const long long token = token0 + t, b = token / a.L, l = token - b * a.L;
+                const T *src = static_cast<const T *>(a.x[m].p) + b * sx.b + l * sx.l + h * sx.h;
+                const T *grd = static_cast<const T *>(a.dy[m].p) + b * sg.b + l * sg.l + h * sg.h;
+                T *dst = static_cast<T *>(const_cast<void *>(a.y[m].p)) + b * so.b + l * so.l + h * so.h;
+                float x[NU][2 * Q], g[NU][2 * Q];
+                float ss = 0.f;
+#pragma unroll
+                for (int j = 0; j < NU; ++j) {
+                    const int u = lane + j * RL;
+#pragma unroll
+                    for (int i = 0; i < 2 * Q; ++i) x[j][i] = 0.f, g[j][i] = 0.f;
+                    if (u >= a.units) continue;
+                    int ca, cb;
+                    bool turned;
+                    const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
+                    piece<T, Q>::ld(src + ca, x[j]);
+                    piece<T, Q>::ld(grd + ca, g[j]);
+                    if (two) {
+                        piece<T, Q>::ld(src + cb, x[j] + Q);
+                        piece<T, Q>::ld(grd + cb, g[j] + Q);
+                    }
+                    if (turned) rot_turn<Q, INTER>(g[j], cs + t * n + Q * u, true);
+                }
+#pragma unroll
+                for (int j = 0; j < NU; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2 * Q; ++i) ss = __builtin_fmaf(x[j][i], x[j][i], ss);
+                for (int o = RL >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+                const float r = rsqrtf(ss * inv_d + a.eps);
+                float dot = 0.f;
+#pragma unroll
+                for (int j = 0; j < NU; ++j) {
+                    const int u = lane + j * RL;
+                    if (u >= a.units) continue;
+                    int ca, cb;
+                    bool turned;
+                    const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
+#pragma unroll
+                    for (int i = 0; i < 2 * Q; ++i) {
+                        if (i >= Q && !two) continue;
+                        x[j][i] *= r;
+                        dw[m][j][i] = __builtin_fmaf(g[j][i], x[j][i], dw[m][j][i]);
+                        g[j][i] *= w[m * D + (i < Q ? ca + i : cb + i - Q)];
+                        dot = __builtin_fmaf(g[j][i], x[j][i], dot);
+                    }
+                }
+                for (int o = RL >> 1; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
+                dot *= inv_d;
+#pragma unroll
+                for (int j = 0; j < NU; ++j) {
+                    const int u = lane + j * RL;
+                    if (u >= a.units) continue;
+                    int ca, cb;
+                    bool turned;
+                    const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
+#pragma unroll
+                    for (int i = 0; i < 2 * Q; ++i) g[j][i] = r * __builtin_fmaf(-x[j][i], dot, g[j][i]);
+                    piece<T, Q>::st(dst + ca, g[j]);
+                    if (two) piece<T, Q>::st(dst + cb, g[j] + Q);
+                }
+            }
+        }
+    }
+    if (a.partial == nullptr) return;
+    // the groups of a wave, then the four waves
+    __syncthreads();
+    float *red = reinterpret_cast<float *>(smem);  // [4][2][D]
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int j = 0; j < NU; ++j)
+#pragma unroll
+            for (int i = 0; i < 2 * Q; ++i) {
+                float v = dw[m][j][i];
+                for (int o = RL; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+                const int u = lane + j * RL;
+                int ca, cb;
+                bool turned;
+                if ((threadIdx.x & 63) < RL && u < a.units) {
+                    const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
+                    if (i < Q || two) red[((threadIdx.x >> 6) * 2 + m) * D + (i < Q ? ca + i : cb + i - Q)] = v;
+                }
+            }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 2 * D; e += ROT_THREADS)
+        a.partial[(size_t)blockIdx.x * 2 * D + e] = (red[e] + red[2 * D + e]) + (red[4 * D + e] + red[6 * D + e]);
+}
+
+constexpr int ROT_MAX_D = 128, ROT_BWD_BLOCKS = 2048;
+
+// tokens of a workgroup: eight where that still leaves two thousand workgroups (the angles of a token are computed
+// once per workgroup, whatever it is), fewer for short calls, down to one per new token
+static int rot_tokens_per_wg(long long tokens) {
+    const long long t = tokens / 2048;
+    return t < 1 ? 1 : t > 8 ? 8 : (int)t;
+}
+
+static bool operand_ok(const RotOperand &o, int heads, long long q, int size) {
+    return heads == 0 || (reinterpret_cast<uintptr_t>(o.p) % (q * size) == 0 && o.s.b % q == 0 && o.s.l % q == 0 && o.s.h % q == 0);
+}
+
+static int rot_check(const char *who, RotArgs &a, int dtype, int B, bool bwd, int &Q) {
+    DSW_REQUIRE(B >= 0 && a.L >= 0 && a.Hq >= 0 && a.Hkv >= 0 && a.axes >= 0 && a.pairs >= 0, "%s: negative size", who);
+    if (dtype != DSW_F32 && dtype != DSW_BF16) return fail(DSW_EUNSUPPORTED, "%s: dtype code %d", who, dtype);
+    if (a.D < 1 || a.D > ROT_MAX_D) return fail(DSW_EUNSUPPORTED, "%s: head dim %d outside 1..%d", who, a.D, ROT_MAX_D);
+    // (64-bit product: two large factors must not wrap into an accepted one)
+    DSW_REQUIRE(2LL * a.axes * a.pairs <= a.D, "%s: %d axes of %d pairs need more than the head dim %d", who, a.axes, a.pairs, a.D);
+    if (a.axes == 0 || a.pairs == 0) a.axes = a.pairs = 0;
+    if ((long long)B * a.L >= (1LL << 31)) return fail(DSW_EUNSUPPORTED, "%s: %lld tokens", who, (long long)B * a.L);
+    a.tokens = (long long)B * a.L;
+    if (a.tokens == 0 || a.Hq + a.Hkv == 0) return DSW_OK;
+    if ((long long)a.Hq + a.Hkv > 4096) return fail(DSW_EUNSUPPORTED, "%s: %d + %d heads", who, a.Hq, a.Hkv);
+    DSW_REQUIRE(a.axes == 0 || a.freqs, "%s: null freqs", who);
+    DSW_REQUIRE(a.pos == nullptr || a.pos_bytes == 4 || a.pos_bytes == 8, "%s: positions of %d bytes", who, a.pos_bytes);
+    for (int m = 0; m < 2; ++m) {
+        const int h = m ? a.Hkv : a.Hq;
+        DSW_REQUIRE(h == 0 || (a.x[m].p && a.y[m].p && (!bwd || a.dy[m].p)), "%s: null pointer", who);
+    }
+    const int n = a.axes * a.pairs, size = dtype == DSW_F32 ? 4 : 2;
+    for (Q = dtype == DSW_F32 ? 4 : 8; Q > 1; Q >>= 1) {
+        bool ok = a.D % Q == 0 && n % Q == 0;
+        for (int m = 0; m < 2 && ok; ++m) {
+            const int h = m ? a.Hkv : a.Hq;
+            ok = operand_ok(a.x[m], h, Q, size) && operand_ok(a.y[m], h, Q, size) && (!bwd || operand_ok(a.dy[m], h, Q, size));
+        }
+        if (ok) break;
+    }
+    a.units = (a.D + 2 * Q - 1) / (2 * Q);
+    a.rl_log = 0;
+    while ((1 << a.rl_log) < a.units && a.rl_log < 4) ++a.rl_log;
+    a.tpw = rot_tokens_per_wg(a.tokens);
+    return DSW_OK;
+}
+
+template <typename T, int Q, int NU>
+static int rot_launch(const RotArgs &a, bool bwd, bool interleaved, hipStream_t st) {
+    const long long tiles = (a.tokens + a.tpw - 1) / a.tpw;
+    size_t lds = ((2 * a.D + 3) & ~3) * 4 + (size_t)a.tpw * a.axes * a.pairs * 8;
+    if (bwd) {
+        if (lds < (size_t)8 * a.D * 4) lds = (size_t)8 * a.D * 4;
+        const dim3 grid((unsigned)(tiles < ROT_BWD_BLOCKS ? tiles : ROT_BWD_BLOCKS));
+        if (interleaved) qk_norm_rotary_bwd_kernel<T, Q, NU, true><<<grid, ROT_THREADS, lds, st>>>(a);
+        else qk_norm_rotary_bwd_kernel<T, Q, NU, false><<<grid, ROT_THREADS, lds, st>>>(a);
+    } else {
+        const dim3 grid((unsigned)tiles);
+        if (interleaved) qk_norm_rotary_fwd_kernel<T, Q, NU, true><<<grid, ROT_THREADS, lds, st>>>(a);
+        else qk_norm_rotary_fwd_kernel<T, Q, NU, false><<<grid, ROT_THREADS, lds, st>>>(a);
+    }
+    return check_launch(bwd ? "dsw_qk_norm_rotary_bwd" : "dsw_qk_norm_rotary_fwd");
+}
+
+static int rot_dispatch(const RotArgs &a, int dtype, int Q, bool bwd, bool interleaved, hipStream_t st) {
+    if (dtype == DSW_BF16 && Q == 8) return rot_launch<bf16_t, 8, 1>(a, bwd, interleaved, st);
+    DSW_DISPATCH_DTYPE(dtype, T, {
+        if (Q == 4) return rot_launch<T, 4, 1>(a, bwd, interleaved, st);
+        if (Q == 2) return rot_launch<T, 2, 2>(a, bwd, interleaved, st);
+        return rot_launch<T, 1, 4>(a, bwd, interleaved, st);
+    });
+    return DSW_OK;
+}
+
+}  // namespace dsw
+
+using namespace dsw;
+
+extern "C" int dsw_qk_norm_rotary_fwd(const void *q, const dsw_strides *sq, const void *k, const dsw_strides *sk, int dtype, int B,
+                                      int L, int Hq, int Hkv, int D, const float *wq, const float *wk, float eps, const float *freqs,
+                                      int axes, int pairs, const void *pos, int pos_bytes, long long pos_batch, int interleaved, void *oq,
+                                      const dsw_strides *soq, void *ok, const dsw_strides *sok, void *stream) {
+    DSW_REQUIRE(sq && sk && soq && sok, "dsw_qk_norm_rotary_fwd: null strides");
+    RotArgs a = {};
+    a.x[0] = {q, *sq}, a.x[1] = {k, *sk}, a.y[0] = {oq, *soq}, a.y[1] = {ok, *sok};
+    a.w[0] = wq, a.w[1] = wk, a.freqs = freqs, a.pos = pos, a.pos_bytes = pos_bytes, a.pos_batch = pos_batch;
+    a.L = L, a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.axes = axes, a.pairs = pairs, a.eps = eps;
+    int Q = 1;
+    const int rc = rot_check("dsw_qk_norm_rotary_fwd", a, dtype, B, false, Q);
+    if (rc || a.tokens == 0 || Hq + Hkv == 0) return rc;
+    return rot_dispatch(a, dtype, Q, false, interleaved != 0, as_stream(stream));
+}
+
+extern "C" int dsw_qk_norm_rotary_blocks(int B, int L) {
+    const long long tokens = (long long)B * L;
+    if (B < 0 || L < 0 || tokens >= (1LL << 31)) return 0;
+    const int tpw = rot_tokens_per_wg(tokens);
+    const long long tiles = (tokens + tpw - 1) / tpw;
+    return (int)(tiles < ROT_BWD_BLOCKS ? tiles : ROT_BWD_BLOCKS);
+}
+
+extern "C" int dsw_qk_norm_rotary_bwd(const void *q, const dsw_strides *sq, const void *k, const dsw_strides *sk, const void *dyq,
+                                      const dsw_strides *sdyq, const void *dyk, const dsw_strides *sdyk, int dtype, int B, int L,
+                                      int Hq, int Hkv, int D, const float *wq, const float *wk, float eps, const float *freqs,
+                                      int axes, int pairs, const void *pos, int pos_bytes, long long pos_batch, int interleaved, void *dq,
+                                      const dsw_strides *sdq, void *dk, const dsw_strides *sdk, float *partial, void *stream) {
+    DSW_REQUIRE(sq && sk && sdyq && sdyk && sdq && sdk, "dsw_qk_norm_rotary_bwd: null strides");
+    RotArgs a = {};
+    a.x[0] = {q, *sq}, a.x[1] = {k, *sk}, a.dy[0] = {dyq, *sdyq}, a.dy[1] = {dyk, *sdyk}, a.y[0] = {dq, *sdq}, a.y[1] = {dk, *sdk};
+    a.w[0] = wq, a.w[1] = wk, a.freqs = freqs, a.pos = pos, a.pos_bytes = pos_bytes, a.pos_batch = pos_batch, a.partial = partial;
+    a.L = L, a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.axes = axes, a.pairs = pairs, a.eps = eps;
+    int Q = 1;
+    const int rc = rot_check("dsw_qk_norm_rotary_bwd", a, dtype, B, true, Q);
+    if (rc || a.tokens == 0 || Hq + Hkv == 0) return rc;
+    return rot_dispatch(a, dtype, Q, true, interleaved != 0, as_stream(stream));
+}

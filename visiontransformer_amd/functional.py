@@ -17,6 +17,7 @@ from ._lib import call, dtype_code, ptr, stream
 
 _c_int = ctypes.c_int
 _c_float = ctypes.c_float
+_c_void_p = ctypes.c_void_p
 
 
 class _NoGradCtx:
@@ -2380,3 +2381,255 @@ def layer_norm(x, norm, for_projection=False, sink=None, pending=None):
     act = autocast_dtype(x.dtype)
     to_act = for_projection and act == torch.bfloat16
     return _run(_LayerNormFn, x, norm.weight, norm.bias, norm.eps, act if to_act else torch.float32, to_act, sink, pending)
+
+
+# ---------------------------------------------------------------------------------------------
+# token sequences: norm + rotation of queries and keys, attention in a sliding window with sinks
+# ---------------------------------------------------------------------------------------------
+def _fail(who, text):
+    raise RuntimeError("visiontransformer_amd: %s: %s" % (who, text))
+
+
+def _call_on(device, name, *args):
+    """call() with `device` as the current one: the tensors' device need not be"""
+    if torch.cuda.current_device() == device.index:
+        return call(name, *args)
+    with torch.cuda.device(device):
+        return call(name, *args)
+
+
+def _head_rows(t):
+    """[B, L, H, D] with D contiguous (a copy where it is not), its dsw_strides and address"""
+    if t.stride(3) != 1 and t.shape[3] > 1:
+        t = t.contiguous()
+    # (strides of dimensions of one element mean nothing, but would count against the alignment)
+    s = _lib.Strides(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
+    return t, ctypes.byref(s), _c_void_p(t.data_ptr())
+
+
+def _same_kind(who, named):
+    """all tensors 4-D, of one supported dtype, on one GPU"""
+    first = next(iter(named.values()))
+    _lib.require_cuda(*named.values())
+    for name, t in named.items():
+        if t.dim() != 4:
+            _fail(who, "%s must be [batch, tokens, heads, head dim], got %s" % (name, tuple(t.shape)))
+        if t.dtype != first.dtype or t.device != first.device:
+            _fail(who, "%s is %s on %s, the others %s on %s" % (name, t.dtype, t.device, first.dtype, first.device))
+    dtype_code(first.dtype)
+
+
+def _device_ints(who, name, t, device, shapes):
+    if t is None:
+        return None
+    if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) not in shapes or t.device != device:
+        _fail(who, "%s must be int32 or int64 of shape %s on %s, got %s %s on %s" % (
+            name, " or ".join(str(s) for s in shapes), device, t.dtype, tuple(t.shape), t.device))
+    return t
+
+
+class _QKNormRotaryFn(torch.autograd.Function):
+    @staticmethod
+    def _spec(q, Hkv, wq, wk, freqs, positions, eps, interleaved):
+        """the arguments that both directions share (addresses taken anew: a hook may have moved saved tensors)"""
+        B, L, Hq, D = q.shape
+        axes, pairs = (0, 0) if freqs is None else freqs.shape
+        return (dtype_code(q.dtype), B, L, Hq, Hkv, D, ptr(wq), ptr(wk), _c_float(eps), ptr(freqs), axes, pairs, ptr(positions),
+                0 if positions is None else positions.element_size(),
+                0 if positions is None or positions.dim() == 2 else L * axes, int(interleaved))
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, freqs, positions, eps, interleaved):
+        B, L, Hq, D = q.shape
+        Hkv, dev = k.shape[2], q.device
+        q, sq, pq = _head_rows(q)
+        k, sk, pk = _head_rows(k)
+        wq, wk = (None if w is None else w.detach().float().contiguous() for w in (q_weight, k_weight))
+        oq, soq, poq = _head_rows(torch.empty(B, L, Hq, D, dtype=q.dtype, device=dev))
+        ok, sok, pok = _head_rows(torch.empty(B, L, Hkv, D, dtype=q.dtype, device=dev))
+        if B * L:
+            spec = _QKNormRotaryFn._spec(q, Hkv, wq, wk, freqs, positions, eps, interleaved)
+            _call_on(dev, "dsw_qk_norm_rotary_fwd", pq, sq, pk, sk, *spec, poq, soq, pok, sok, stream(dev))
+        ctx.save_for_backward(q, k, wq, wk, freqs, positions)
+        ctx.settings = (eps, interleaved)
+        ctx.weight_dtypes = (None if q_weight is None else q_weight.dtype, None if k_weight is None else k_weight.dtype)
+        return oq, ok
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dyq, dyk):
+        q, k, wq, wk, freqs, positions = ctx.saved_tensors
+        B, L, Hq, D = q.shape
+        Hkv, dev = k.shape[2], q.device
+        _, sq, pq = _head_rows(q)
+        _, sk, pk = _head_rows(k)
+        dyq, sdyq, pdyq = _head_rows(dyq.to(q.dtype))
+        dyk, sdyk, pdyk = _head_rows(dyk.to(q.dtype))
+        dq, sdq, pdq = _head_rows(torch.empty(B, L, Hq, D, dtype=q.dtype, device=dev))
+        dk, sdk, pdk = _head_rows(torch.empty(B, L, Hkv, D, dtype=q.dtype, device=dev))
+        want_w = (wq is not None and ctx.needs_input_grad[2]) or (wk is not None and ctx.needs_input_grad[3])
+        blocks = _lib.load().dsw_qk_norm_rotary_blocks(B, L)
+        partial = torch.empty(blocks, 2 * D, dtype=torch.float32, device=dev) if want_w and blocks else None
+        if B * L:
+            spec = _QKNormRotaryFn._spec(q, Hkv, wq, wk, freqs, positions, *ctx.settings)
+            _call_on(dev, "dsw_qk_norm_rotary_bwd", pq, sq, pk, sk, pdyq, sdyq, pdyk, sdyk, *spec, pdq, sdq, pdk, sdk,
+                     ptr(partial), stream(dev))
+        dw = (None, None)
+        if want_w:
+            with torch.cuda.device(dev):
+                both = torch.zeros(2 * D, device=dev) if partial is None else colsum(partial)
+            dw = tuple(both[i * D:(i + 1) * D].to(t) if w is not None else None for i, (w, t) in enumerate(zip((wq, wk), ctx.weight_dtypes)))
+        return dq, dk, dw[0], dw[1], None, None, None, None
+
+
+def qk_norm_rotary(q, k, q_weight=None, k_weight=None, freqs=None, positions=None, eps=1e-6, interleaved=False):
+    """RMS norm of every head's query and key row (u = weight * x / sqrt(mean(x^2) + eps)) and the rotation of the result
+    by position, in one launch; returns new contiguous tensors.
+
+    q [B, L, Hq, D], k [B, L, Hkv, D]: fp32 or bf16, D <= 128, any strides (slices of a packed q|k|v projection are read
+    in place).  q_weight, k_weight: [D] or None.  freqs: fp32 radians per step - [P] (one position per token, positions
+    [L] or [B, L]) or [A, P] (A coordinates per token, e.g. row and column of a map; positions [L, A] or [B, L, A]);
+    pair c = a * P + i of the first 2 A P columns turns by positions[..., a] * freqs[a, i], where a pair is the columns
+    (c, c + A P), or (2 c, 2 c + 1) when interleaved; the columns behind them are only normalised.  None: norm only.
+    positions: int32 or int64, None: the token's index on every axis.  Angles are taken in 64 bits.
+    Gradients: q, k and the two weights (not freqs)."""
+    who = "qk_norm_rotary"
+    _same_kind(who, {"q": q, "k": k})
+    B, L, _, D = q.shape
+    if k.shape[0] != B or k.shape[1] != L or k.shape[3] != D:
+        _fail(who, "q %s and k %s differ in more than their heads" % (tuple(q.shape), tuple(k.shape)))
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (tuple(w.shape) != (D,) or not w.is_floating_point() or w.device != q.device):
+            _fail(who, "%s must be a floating [%d] tensor on %s, got %s %s on %s" % (name, D, q.device, w.dtype, tuple(w.shape), w.device))
+    if freqs is None:
+        if positions is not None:
+            _fail(who, "positions without freqs")
+    else:
+        if freqs.dim() not in (1, 2) or freqs.dtype != torch.float32 or freqs.device != q.device:
+            _fail(who, "freqs must be fp32 [pairs] or [axes, pairs] on %s, got %s %s on %s" % (q.device, freqs.dtype, tuple(freqs.shape), freqs.device))
+        flat = freqs.dim() == 1
+        freqs = freqs.detach().reshape((1, -1) if flat else freqs.shape).contiguous()
+        A = freqs.shape[0]
+        if 2 * freqs.numel() > D:
+            _fail(who, "%d pairs on %d axes need more than the %d columns of a head" % (freqs.shape[1], A, D))
+        positions = _device_ints(who, "positions", positions, q.device, ((L,), (B, L)) if flat else ((L, A), (B, L, A)))
+        if positions is not None:
+            positions = (positions.unsqueeze(-1) if flat else positions).contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        return _QKNormRotaryFn.apply(q, k, q_weight, k_weight, freqs, positions, float(eps), bool(interleaved))
+    return _QKNormRotaryFn.forward(_NO_GRAD, q, k, q_weight, k_weight, freqs, positions, float(eps), bool(interleaved))
+
+
+class _BandAttnFn(torch.autograd.Function):
+    @staticmethod
+    def _desc(q, k, tab, buckets, q_lens, k_lens, left, right, sinks, scale):
+        B, Lq, Hq, D = q.shape
+        return _lib.BandDesc(dtype_code(q.dtype), B, Lq, k.shape[1], Hq, k.shape[2], D, left, right, sinks, scale, ptr(q_lens), ptr(k_lens),
+                             ptr(tab), ptr(buckets), 0 if tab is None else tab.shape[0], 0 if tab is None else buckets.numel() // 2)
+
+    @staticmethod
+    def forward(ctx, q, k, v, table, buckets, q_lens, k_lens, left, right, sinks, scale):
+        B, Lq, Hq, D = q.shape
+        dev = q.device
+        q, sq, pq = _head_rows(q)
+        k, sk, pk = _head_rows(k)
+        v, sv, pv = _head_rows(v)
+        tab = None if table is None else table.detach().float().contiguous()
+        out, so, po = _head_rows(torch.empty(B, Lq, Hq, D, dtype=q.dtype, device=dev))
+        settings = (left, right, sinks, scale)
+        desc = _BandAttnFn._desc(q, k, tab, buckets, q_lens, k_lens, *settings)
+        train = any(ctx.needs_input_grad[:4])
+        lse = torch.empty(B, Hq, Lq, dtype=torch.float32, device=dev) if train else None
+        exact = train and ctx.needs_input_grad[3] and q.dtype == torch.bfloat16
+        out32 = torch.empty(B, Lq, Hq, D, dtype=torch.float32, device=dev) if exact else None
+        if B * Lq * Hq:
+            ws, n = None, 0
+            if not train:
+                n = int(_lib.load().dsw_band_attn_fwd_workspace(ctypes.byref(desc)))
+                ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+            _call_on(dev, "dsw_band_attn_fwd", ctypes.byref(desc), pq, sq, pk, sk, pv, sv, po, so, ptr(lse), ptr(out32), ptr(ws), n, stream(dev))
+        if train:
+            ctx.save_for_backward(q, k, v, tab, buckets, q_lens, k_lens, out, out32, lse)
+            ctx.settings = settings
+            ctx.table_dtype = None if table is None else table.dtype
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, tab, buckets, q_lens, k_lens, out, out32, lse = ctx.saved_tensors
+        dev = q.device
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v)]
+        d_tab = torch.empty_like(tab) if tab is not None and ctx.needs_input_grad[3] else None
+        if q.shape[0] * q.shape[2] * max(q.shape[1], k.shape[1]):
+            operands = []
+            for t in (q, k, v, out):
+                operands += _head_rows(t)[:0:-1]
+            operands.append(ptr(out32))
+            dout, s, p = _head_rows(dout.to(q.dtype))
+            operands += [p, s, ptr(lse)]
+            for t in grads:
+                operands += _head_rows(t)[:0:-1]
+            desc = _BandAttnFn._desc(q, k, tab, buckets, q_lens, k_lens, *ctx.settings)
+            n = int(_lib.load().dsw_band_attn_bwd_workspace(ctypes.byref(desc)))
+            ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+            _call_on(dev, "dsw_band_attn_bwd", ctypes.byref(desc), *operands, ptr(d_tab), ptr(ws), n, stream(dev))
+        elif d_tab is not None:
+            d_tab.zero_()
+        return grads[0], grads[1], grads[2], None if d_tab is None else d_tab.to(ctx.table_dtype), None, None, None, None, None, None, None
+
+
+def band_attention(q, k, v, window=(None, None), sinks=0, scale=None, q_lens=None, k_lens=None, bias_table=None, bias_buckets=None):
+    """Softmax attention of token sequences over a sliding window of keys in which the first `sinks` keys stay visible.
+
+    q [B, Lq, Hq, D], k, v [B, Lk, Hkv, D]: fp32 or bf16, D <= 128, Hq a multiple of Hkv (query head h reads key head
+    h // (Hq // Hkv)), any strides with D contiguous.  Returns [B, Lq, Hq, D].
+
+    Query row i stands at position p = k_len - q_len + i: the rows are the last ones of their sequence, which is what both
+    a whole sequence (Lq = Lk) and new tokens behind a cache need.  k_lens, q_lens: int32 (or int64) [B] on the GPU, None:
+    all Lk keys, all Lq rows; values are clamped to the tensors' sizes.  window = (left, right): key j is visible when
+    p - left <= j <= p + right; None: no limit on that side ((None, 0): causal).  sinks: keys j < sinks stay visible when the
+    window has passed them (j <= p + right still holds).  Rows from q_len on and rows without a visible key give zeros.
+    Keys and values from k_len on are never read into a result, and a non-finite value in a key that a row does not see
+    never reaches that row's output.
+
+    bias_table [n, Hq] with bias_buckets int32 [2 M + 1], M <= 512: table[bias_buckets[clip(j - p, -M, M) + M], head] is
+    added to the scaled logits (sequence.BucketedPositionBias holds both).  scale: D ** -0.5 by default, positive.
+    Gradients: q, k, v, bias_table.  Calls of few query rows without gradients split the keys over the chip."""
+    who = "band_attention"
+    _same_kind(who, {"q": q, "k": k, "v": v})
+    B, Lq, Hq, D = q.shape
+    Lk, Hkv = k.shape[1:3]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        _fail(who, "q %s, k %s and v %s do not go together" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if Hq and (Hkv == 0 or Hq % Hkv):
+        _fail(who, "%d query heads over %d key heads" % (Hq, Hkv))
+    if D == 0:
+        _fail(who, "heads of no columns")
+    left, right = window
+    for name, n in (("window's left", left), ("window's right", right), ("sinks", sinks)):
+        if n is not None and (n != int(n) or not 0 <= n < 2 ** 31):
+            _fail(who, "%s must be a whole number >= 0%s, got %r" % (name, "" if name == "sinks" else " or None", n))
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        _fail(who, "scale must be positive, got %r" % scale)
+    lens = [_device_ints(who, name, t, q.device, ((B,),)) for name, t in (("q_lens", q_lens), ("k_lens", k_lens))]
+    # (int64 lengths are clamped before they are narrowed, so that none comes back as another)
+    q_lens, k_lens = (t if t is None else (t.clamp(0, n) if t.dtype == torch.int64 else t).to(torch.int32).contiguous()
+                      for t, n in zip(lens, (Lq, Lk)))
+    if (bias_table is None) != (bias_buckets is None):
+        _fail(who, "bias_table and bias_buckets go together")
+    if bias_table is not None:
+        if bias_table.dim() != 2 or bias_table.shape[1] != Hq or bias_table.shape[0] < 1 or not bias_table.is_floating_point() or bias_table.device != q.device:
+            _fail(who, "bias_table must be a floating [buckets, %d] tensor on %s, got %s %s on %s" % (
+                Hq, q.device, bias_table.dtype, tuple(bias_table.shape), bias_table.device))
+        n = bias_buckets.numel()
+        _device_ints(who, "bias_buckets", bias_buckets, q.device, ((n,),))
+        if n % 2 == 0 or not 3 <= n <= 1025:
+            _fail(who, "bias_buckets must have 2 M + 1 entries with 1 <= M <= 512, got %d" % n)
+        bias_buckets = bias_buckets.to(torch.int32).contiguous()
+    args = (q, k, v, bias_table, bias_buckets, q_lens, k_lens, -1 if left is None else int(left), -1 if right is None else int(right),
+            int(sinks), scale)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias_table)):
+        return _BandAttnFn.apply(*args)
+    return _BandAttnFn.forward(_NO_GRAD, *args)
