@@ -19,8 +19,11 @@ constexpr int BAND_FAR = 1 << 29;  // "unlimited": beyond every length, and sums
 struct BandTensor {
     const void *p;
     dsw_strides s;
-    int mode;  // 0: whole 16-byte pieces; 1: 4-byte pieces; 2: single elements
 };
+// How a call's tensors are accessed, a template argument of the kernels (a branch per access cost more than the access):
+// 0  16-byte pieces: D and all strides multiples of 16 bytes, rows 16-byte aligned; bf16 tiles go to LDS without registers
+// 1  pieces at any element offset; the last piece of a row is the one that ends with it (8 <= D)
+// 2  single elements (D < 8, or rows so far apart that a tile spans 2 GiB)
 
 struct BandArgs {
     BandTensor q, k, v, out, dout, dq, dk, dv;
@@ -67,6 +70,19 @@ __device__ __forceinline__ f32x16 band_mma(const band_t<float>::frag &a, const b
     return c;
 }
 
+// l + the sum of a fragment's elements, as they enter the product behind it
+typedef __bf16 band_bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float band_sum(const uint4 &f, float l) {
+    const band_bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+    l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(band_bf16x2, f.x), one, l, false);
+    l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(band_bf16x2, f.y), one, l, false);
+    l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(band_bf16x2, f.z), one, l, false);
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(band_bf16x2, f.w), one, l, false);
+}
+__device__ __forceinline__ float band_sum(const band_t<float>::frag &f, float l) {
+    return l + (((f.lo.x + f.lo.y) + (f.lo.z + f.lo.w)) + ((f.hi.x + f.hi.y) + (f.hi.z + f.hi.w)));
+}
+
 __device__ __forceinline__ f32x16 band_zero() {
     f32x16 z;
 #pragma unroll
@@ -93,9 +109,11 @@ __device__ __forceinline__ void band_pack_rest(const f32x16 &s, int c, const uin
 }
 
 // ---- global memory: 8 consecutive elements of a row, zero past D -------------------------------------------------
-__device__ __forceinline__ uint4 band_load8(const bf16_t *row, int col, int D, int mode) {
-    if (mode == 0) return col < D ? *reinterpret_cast<const uint4 *>(row + col) : make_uint4(0u, 0u, 0u, 0u);
-    if (mode == 1) return load_slot(row + col, slot_dwords(D, col >> 3));
+struct __attribute__((packed, aligned(2))) band_u16x8 { uint32_t x, y, z, w; };   // (unaligned vector accesses are legal)
+struct __attribute__((packed, aligned(4))) band_f32x4 { float x, y, z, w; };
+
+template <int MODE> __device__ __forceinline__ uint4 band_load8(const bf16_t *row, int col, int D) {
+    if constexpr (MODE == 0) return col < D ? *reinterpret_cast<const uint4 *>(row + col) : make_uint4(0u, 0u, 0u, 0u);
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -104,9 +122,9 @@ __device__ __forceinline__ uint4 band_load8(const bf16_t *row, int col, int D, i
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ band_t<float>::frag band_load8(const float *row, int col, int D, int mode) {
+template <int MODE> __device__ __forceinline__ band_t<float>::frag band_load8(const float *row, int col, int D) {
     band_t<float>::frag f;
-    if (mode == 0) {
+    if constexpr (MODE == 0) {
         f.lo = col < D ? *reinterpret_cast<const float4 *>(row + col) : f4zero();
         f.hi = col + 4 < D ? *reinterpret_cast<const float4 *>(row + col + 4) : f4zero();
         return f;
@@ -118,23 +136,39 @@ __device__ __forceinline__ band_t<float>::frag band_load8(const float *row, int 
     f.hi = make_float4(v[4], v[5], v[6], v[7]);
     return f;
 }
+// the piece at column `at` itself, at any alignment, all 8 elements inside the row
+__device__ __forceinline__ uint4 band_piece(const bf16_t *p) {
+    const band_u16x8 t = *reinterpret_cast<const band_u16x8 *>(p);
+    return make_uint4(t.x, t.y, t.z, t.w);
+}
+__device__ __forceinline__ band_t<float>::frag band_piece(const float *p) {
+    const band_f32x4 a = *reinterpret_cast<const band_f32x4 *>(p), b = *reinterpret_cast<const band_f32x4 *>(p + 4);
+    band_t<float>::frag f;
+    f.lo = make_float4(a.x, a.y, a.z, a.w);
+    f.hi = make_float4(b.x, b.y, b.z, b.w);
+    return f;
+}
 __device__ __forceinline__ void band_clear(uint4 &f) { f = make_uint4(0u, 0u, 0u, 0u); }
 __device__ __forceinline__ void band_clear(band_t<float>::frag &f) { f.lo = f4zero(), f.hi = f4zero(); }
 
-__device__ __forceinline__ void band_store8(bf16_t *row, int col, const float *v, int D, int mode) {
+template <int MODE> __device__ __forceinline__ void band_store8(bf16_t *row, int col, const float *v, int D) {
     const uint4 u = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-    if (mode == 0) {
-        if (col < D) *reinterpret_cast<uint4 *>(row + col) = u;
-    } else if (mode == 1) {
-        store_slot(row + col, u, slot_dwords(D, col >> 3));
+    if (MODE == 0 || col + 8 <= D) {
+        if (MODE != 0) {
+            band_u16x8 t;
+            t.x = u.x, t.y = u.y, t.z = u.z, t.w = u.w;
+            *reinterpret_cast<band_u16x8 *>(row + col) = t;
+        } else if (col < D) {
+            *reinterpret_cast<uint4 *>(row + col) = u;
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (col + i < D) row[col + i] = f32_to_bf16(v[i]);
     }
 }
-__device__ __forceinline__ void band_store8(float *row, int col, const float *v, int D, int mode) {
-    if (mode == 0) {
+template <int MODE> __device__ __forceinline__ void band_store8(float *row, int col, const float *v, int D) {
+    if constexpr (MODE == 0) {
         if (col < D) *reinterpret_cast<float4 *>(row + col) = make_float4(v[0], v[1], v[2], v[3]);
         if (col + 4 < D) *reinterpret_cast<float4 *>(row + col + 4) = make_float4(v[4], v[5], v[6], v[7]);
     } else {
@@ -151,8 +185,8 @@ template <typename T> __device__ __forceinline__ const T *band_row(const BandTen
 // Transposed result tiles (accumulator rows = head-dim columns, lane = row of the tensor): 8 consecutive columns per
 // lane by an exchange of the two lane halves, then one store per 16 columns.  All lanes must call it (the exchange);
 // `on` says whether this lane's row is written.
-template <typename T, int DP>
-__device__ __forceinline__ void band_store_row(T *row, const f32x16 *acc, float mul, int D, int mode, int hh, bool on) {
+template <typename T, int DP, int MODE>
+__device__ __forceinline__ void band_store_row(T *row, const f32x16 *acc, float mul, int D, int hh, bool on) {
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
@@ -165,7 +199,7 @@ __device__ __forceinline__ void band_store_row(T *row, const f32x16 *acc, float 
                 v[i] = __uint_as_float(r[0]);
                 v[4 + i] = __uint_as_float(r[1]);
             }
-            if (on) band_store8(row, 32 * db + 16 * p + 8 * hh, v, D, mode);
+            if (on) band_store8<MODE>(row, 32 * db + 16 * p + 8 * hh, v, D);
         }
 }
 
@@ -215,24 +249,83 @@ template <int DP> __device__ __forceinline__ band_t<float>::frag band_cols(const
     return f;
 }
 
-// ---- staging of 64-row tiles by the whole workgroup: global memory -> registers -> LDS -----------------------------
-template <typename T, int DP> struct BandStage {
+// ---- staging of 64-row tiles by the whole workgroup (256 threads) ------------------------------------------------
+// One slice (a head of one sequence, rows `ld` apart) and its LDS images.  Rows from `limit` (>= 1) on are read as copies of
+// row limit - 1: what they hold is masked, and nothing past the sequence is touched.  Mode 0 (bf16): fetch() starts the
+// copy straight into the image, band_landed() waits for it.  Modes 1, 2: fetch() loads registers, put() writes the image,
+// whose columns past D clear() has to have zeroed once.  (Mode 0 repeats the row's last piece there: the queries
+// are zero in those columns of K, and those columns of V add to columns of the result that are not stored.)
+__device__ __forceinline__ void band_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t band_lds_address(const void *p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
+}
+template <typename T, int DP, int MODE> struct BandStage {
     static constexpr int N = DP / 32, SLOTS = DP / 8, STEP = 256 / SLOTS;  // pieces per thread, per row; rows between a thread's pieces
-    typename band_t<T>::frag f[N];
-    // rows row0 .. row0+63 of the slice at `base` (row stride ld); rows from `limit` on read as zero
-    __device__ __forceinline__ void load(const T *base, long long ld, int row0, int limit, int D, int mode) {
-        const int r = threadIdx.x / SLOTS, col = 8 * (threadIdx.x % SLOTS);
-        const T *p = base + (long long)(row0 + r) * ld;
+    static constexpr bool DIRECT = MODE == 0 && sizeof(T) == 2;
+    const char *base;
+    long long ld;  // bytes
+    typename band_t<T>::frag f[DIRECT ? 1 : N];
+    uint32_t ld32;
+
+    __device__ __forceinline__ void init(const T *slice, long long row) {
+        base = reinterpret_cast<const char *>(slice);
+        ld = row * (long long)sizeof(T);
+        ld32 = (uint32_t)ld;
+    }
+    // rows row0 .. row0 + 63
+    __device__ __forceinline__ void fetch(int row0, int limit, int D, T *image) {
+        const char *tile = base + (long long)row0 * ld;
+        const int last = limit - 1 - row0;  // last row of the tile that exists
+        if constexpr (DIRECT) {
+            const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (row0 + r + i * STEP < limit) f[i] = band_load8(p + (long long)(i * STEP) * ld, col, D, mode);
-            else band_clear(f[i]);
+            for (int i = 0; i < N; ++i) {
+                // one instruction fills 1 KiB of the image: lane's 16 bytes belong to row r, and hold the logical piece that
+                // the image's pattern puts there
+                const int r = (wave * N + i) * (64 / SLOTS) + lane / SLOTS;
+                const int slot = min((lane % SLOTS) ^ band_flip<DP>(r), D / 8 - 1);
+                const uint32_t off = (uint32_t)min(r, last) * ld32 + 16 * slot;
+                const uint32_t to = __builtin_amdgcn_readfirstlane(band_lds_address(image) + (wave * N + i) * 1024);
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(tile) : "memory", "m0");
+            }
+        } else {
+            const int r0 = threadIdx.x / SLOTS, col = 8 * (threadIdx.x % SLOTS);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int r = min(r0 + i * STEP, last);
+                if constexpr (MODE == 2) {
+                    f[i] = band_load8<2>(reinterpret_cast<const T *>(tile + (long long)r * ld), col, D);
+                } else {
+                    const T *p = reinterpret_cast<const T *>(tile + (uint32_t)r * ld32);
+                    if constexpr (MODE == 1) f[i] = band_piece(p + min(col, D - 8));
+                    else f[i] = band_load8<0>(p, col, D);
+                }
+            }
         }
     }
-    __device__ __forceinline__ void put(T *m) const {
-        const int r = threadIdx.x / SLOTS, slot = threadIdx.x % SLOTS;
+    __device__ __forceinline__ void put(T *image, int D) const {
+        if constexpr (!DIRECT) {
+            const int r0 = threadIdx.x / SLOTS, slot = threadIdx.x % SLOTS;
+            if (MODE != 1 || 8 * slot + 8 <= D) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) band_put<DP>(m, r + i * STEP, slot, f[i]);
+                for (int i = 0; i < N; ++i) band_put<DP>(image, r0 + i * STEP, slot, f[i]);
+            } else if (8 * slot < D) {
+                // the piece that ends with the row lies across two of the image's: one element at a time (those of the
+                // piece before it come a second time, with the values it wrote)
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    T e[8];
+                    *reinterpret_cast<typename band_t<T>::frag *>(e) = f[i];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) image[band_at<T, DP>(r0 + i * STEP, D - 8 + k)] = e[k];
+                }
+            }
+        }
+    }
+    // zeros in the columns past D of `rows` rows of images, by the whole workgroup; a barrier is the caller's
+    static __device__ __forceinline__ void clear(T *image, int rows, int D) {
+        if constexpr (MODE == 1)
+            for (int e = threadIdx.x; e < rows * (DP - D); e += 256) image[band_at<T, DP>(e / (DP - D), D + e % (DP - D))] = (T)0;
     }
 };
 
@@ -328,9 +421,29 @@ __device__ __forceinline__ void band_careful(const BandArgs &a, const T *qrow, c
 }
 
 int band_make_args(const char *who, const dsw_band_desc *d, BandArgs &a);
-int band_tensor(const char *who, const char *name, const void *p, const dsw_strides *s, int dtype, int D, bool null_ok, BandTensor &t);
+// fills t and raises `mode` to what the tensor needs
+int band_tensor(const char *who, const char *name, const void *p, const dsw_strides *s, int dtype, int D, bool null_ok, BandTensor &t, int &mode);
+// (T, DP, MODE) for a call: mode 2 serves narrow heads, or anything, through its widest image
+#define DSW_BAND_DISPATCH(dtype, D, mode, T, DP, MODE, ...)                                                           \
+    DSW_DISPATCH_DTYPE(dtype, T, {                                                                                      \
+        if ((mode) == 2) {                                                                                              \
+            constexpr int MODE = 2;                                                                                     \
+            if ((D) <= 32) { constexpr int DP = 32; __VA_ARGS__; }                                                      \
+            else { constexpr int DP = 128; __VA_ARGS__; }                                                               \
+        } else if ((mode) == 1) {                                                                                       \
+            constexpr int MODE = 1;                                                                                     \
+            if ((D) <= 32) { constexpr int DP = 32; __VA_ARGS__; }                                                      \
+            else if ((D) <= 64) { constexpr int DP = 64; __VA_ARGS__; }                                                 \
+            else { constexpr int DP = 128; __VA_ARGS__; }                                                               \
+        } else {                                                                                                        \
+            constexpr int MODE = 0;                                                                                     \
+            if ((D) <= 32) { constexpr int DP = 32; __VA_ARGS__; }                                                      \
+            else if ((D) <= 64) { constexpr int DP = 64; __VA_ARGS__; }                                                 \
+            else { constexpr int DP = 128; __VA_ARGS__; }                                                               \
+        }                                                                                                               \
+    })
 // launches the kernel for few query rows (band_attn_step.hip) and the one that joins its splits
-int band_launch_step(BandArgs &a, int dtype, hipStream_t st);
+int band_launch_step(BandArgs &a, int dtype, int mode, hipStream_t st);
 // whether a call goes there, and how many row blocks and splits it has
 bool band_step_plan(const dsw_band_desc &d, int &nrb, int &nsplit);
 

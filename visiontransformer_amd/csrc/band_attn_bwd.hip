@@ -12,7 +12,7 @@
 namespace dsw {
 
 // ---- delta: 16 lanes a row ---------------------------------------------------------------------------------------
-template <typename T> __global__ __launch_bounds__(256) void band_attn_delta_kernel(const BandArgs a) {
+template <typename T, int MODE> __global__ __launch_bounds__(256) void band_attn_delta_kernel(const BandArgs a) {
     const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
     const int lane = threadIdx.x & 15;
     const long long rows = (long long)a.B * a.Lq * a.Hq;
@@ -25,7 +25,7 @@ template <typename T> __global__ __launch_bounds__(256) void band_attn_delta_ker
         if (i < band_seq(a, b).qn) {
             const T *g = band_row<T>(a.dout, b, i, h), *o = band_row<T>(a.out, b, i, h);
             const float *o32 = a.out32 ? a.out32 + (size_t)row * a.D : nullptr;
-            if (a.dout.mode == 0 && a.out.mode == 0 && a.D % 8 == 0 && o32 == nullptr) {
+            if (MODE == 0 && a.D % 8 == 0 && o32 == nullptr) {
                 for (int d = 8 * lane; d < a.D; d += 128) {
                     const float4 g0 = io<T>::ld4(g + d), g1 = io<T>::ld4(g + d + 4), o0 = io<T>::ld4(o + d), o1 = io<T>::ld4(o + d + 4);
                     s += ((g0.x * o0.x + g0.y * o0.y) + (g0.z * o0.z + g0.w * o0.w)) + ((g1.x * o1.x + g1.y * o1.y) + (g1.z * o1.z + g1.w * o1.w));
@@ -41,7 +41,7 @@ template <typename T> __global__ __launch_bounds__(256) void band_attn_delta_ker
 }
 
 // ---- dk, dv: 128 keys of a workgroup, 32 per wave -----------------------------------------------------------------
-template <typename T, int DP, bool BIAS>
+template <typename T, int DP, int MODE, bool BIAS>
 __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void band_attn_dkv_kernel(const BandArgs a) {
     constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE);
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -69,8 +69,8 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
         if (key_on) {
-            kf[c] = band_load8(krow, 16 * c + 8 * hh, a.D, a.k.mode);
-            vf[c] = band_load8(vrow, 16 * c + 8 * hh, a.D, a.v.mode);
+            kf[c] = band_load8<MODE>(krow, 16 * c + 8 * hh, a.D);
+            vf[c] = band_load8<MODE>(vrow, 16 * c + 8 * hh, a.D);
         } else {
             band_clear(kf[c]);
             band_clear(vf[c]);
@@ -81,19 +81,27 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
     for (int db = 0; db < DP / 32; ++db) dk[db] = dv[db] = band_zero();
 
     const int steps = n_tiles * a.G;  // tiles of the first head, of the second, ...
-    BandStage<T, DP> qs, gs;
+    using Stage = BandStage<T, DP, MODE>;
+    Stage qs, gs;
     float st = 0.f;
-    auto load = [&](int step) {
+    if (MODE == 1 && a.D < DP) {
+        Stage::clear(lds, NB * 2 * BAND_TILE, a.D);
+        __syncthreads();
+    }
+    auto fetch = [&](int step) {
         const int g = step / n_tiles, i0 = (first + step - g * n_tiles) * BAND_TILE, h = hk * a.G + g;
-        qs.load(band_row<T>(a.q, b, 0, h), a.q.s.l, i0, sq.qn, a.D, a.q.mode);
-        gs.load(band_row<T>(a.dout, b, 0, h), a.dout.s.l, i0, sq.qn, a.D, a.dout.mode);
+        T *const Q = lds + (NB == 2 ? (step & 1) : 0) * 2 * ELEMS;
         if (threadIdx.x < 2 * BAND_TILE) {
             const int i = i0 + (threadIdx.x & (BAND_TILE - 1));
             const float *src = (threadIdx.x < BAND_TILE ? a.lse : a.delta) + ((size_t)b * a.Hq + h) * a.Lq;
             st = i < sq.qn ? src[i] : threadIdx.x < BAND_TILE ? INFINITY : 0.f;
         }
+        qs.init(band_row<T>(a.q, b, 0, h), a.q.s.l);
+        gs.init(band_row<T>(a.dout, b, 0, h), a.dout.s.l);
+        qs.fetch(i0, sq.qn, a.D, Q);
+        gs.fetch(i0, sq.qn, a.D, Q + ELEMS);
     };
-    if (steps) load(0);
+    if (steps) fetch(0);
     for (int step = 0; step < steps; ++step) {
         T *const Q = lds + (NB == 2 ? (step & 1) : 0) * 2 * ELEMS, *const G = Q + ELEMS;
         float *const S = stats + (NB == 2 ? (step & 1) : 0) * 2 * BAND_TILE;
@@ -105,11 +113,16 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
                 band_stage_bias(a, hk * a.G + g, -1, bias, 256);
             }
         }
-        qs.put(Q);
-        gs.put(G);
+        if constexpr (Stage::DIRECT) {
+            band_landed();
+        } else {
+            qs.put(Q, a.D);
+            gs.put(G, a.D);
+        }
         if (threadIdx.x < 2 * BAND_TILE) S[threadIdx.x] = st;
-        if (step + 1 < steps) load(step + 1);
-        lds_barrier();
+        if constexpr (Stage::DIRECT) lds_barrier();
+        if (step + 1 < steps) fetch(step + 1);
+        if constexpr (!Stage::DIRECT) lds_barrier();
 #pragma unroll 1
         for (int u = 0; u < 2; ++u) {
             const int r0 = i0 + 32 * u, p_lo = sq.off + r0, p_hi = sq.off + min(r0 + 31, sq.qn - 1);
@@ -162,12 +175,12 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
     }
     // (keys behind the sequence: their P and dS are zero, and so are these rows)
     const bool store = j < a.Lk;
-    band_store_row<T, DP>(const_cast<T *>(band_row<T>(a.dk, b, j, hk)), dk, a.scale, a.D, a.dk.mode, hh, store);
-    band_store_row<T, DP>(const_cast<T *>(band_row<T>(a.dv, b, j, hk)), dv, 1.f, a.D, a.dv.mode, hh, store);
+    band_store_row<T, DP, MODE>(const_cast<T *>(band_row<T>(a.dk, b, j, hk)), dk, a.scale, a.D, hh, store);
+    band_store_row<T, DP, MODE>(const_cast<T *>(band_row<T>(a.dv, b, j, hk)), dv, 1.f, a.D, hh, store);
 }
 
 // ---- dq: 128 rows of a workgroup, 32 per wave; bias gradient by distance ---------------------------------------------
-template <typename T, int DP, bool BIAS, bool DTABLE>
+template <typename T, int DP, int MODE, bool BIAS, bool DTABLE>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void band_attn_dq_kernel(const BandArgs a) {
     constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE);
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -199,8 +212,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
         if (row_on) {
-            qf[c] = band_load8(qrow, 16 * c + 8 * hh, a.D, a.q.mode);
-            gf[c] = band_load8(grow, 16 * c + 8 * hh, a.D, a.dout.mode);
+            qf[c] = band_load8<MODE>(qrow, 16 * c + 8 * hh, a.D);
+            gf[c] = band_load8<MODE>(grow, 16 * c + 8 * hh, a.D);
         } else {
             band_clear(qf[c]);
             band_clear(gf[c]);
@@ -213,23 +226,34 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     for (int db = 0; db < DP / 32; ++db) dq[db] = band_zero();
     float far_lo = 0.f, far_hi = 0.f;
 
-    BandStage<T, DP> ks, vs;
+    using Stage = BandStage<T, DP, MODE>;
+    Stage ks, vs;
+    ks.init(kbase, a.k.s.l);
+    vs.init(vbase, a.v.s.l);
+    if (MODE == 1 && a.D < DP) {
+        Stage::clear(lds, NB * 2 * BAND_TILE, a.D);
+        __syncthreads();
+    }
     if (tiles.count) {
-        const int j0 = tiles.at(0) * BAND_TILE;
-        ks.load(kbase, a.k.s.l, j0, sq.kn, a.D, a.k.mode);
-        vs.load(vbase, a.v.s.l, j0, sq.kn, a.D, a.v.mode);
+        ks.fetch(tiles.at(0) * BAND_TILE, sq.kn, a.D, lds);
+        vs.fetch(tiles.at(0) * BAND_TILE, sq.kn, a.D, lds + ELEMS);
     }
     for (int it = 0; it < tiles.count; ++it) {
         T *const K = lds + (NB == 2 ? (it & 1) : 0) * 2 * ELEMS, *const V = K + ELEMS;
-        if constexpr (NB == 1) lds_barrier();
-        ks.put(K);
-        vs.put(V);
-        if (it + 1 < tiles.count) {
-            const int j1 = tiles.at(it + 1) * BAND_TILE;
-            ks.load(kbase, a.k.s.l, j1, sq.kn, a.D, a.k.mode);
-            vs.load(vbase, a.v.s.l, j1, sq.kn, a.D, a.v.mode);
+        if constexpr (Stage::DIRECT) {
+            band_landed();
+            lds_barrier();
+        } else {
+            if constexpr (NB == 1) lds_barrier();
+            ks.put(K, a.D);
+            vs.put(V, a.D);
         }
-        lds_barrier();
+        if (it + 1 < tiles.count) {
+            T *const K1 = lds + (NB == 2 ? ((it + 1) & 1) : 0) * 2 * ELEMS;
+            ks.fetch(tiles.at(it + 1) * BAND_TILE, sq.kn, a.D, K1);
+            vs.fetch(tiles.at(it + 1) * BAND_TILE, sq.kn, a.D, K1 + ELEMS);
+        }
+        if constexpr (!Stage::DIRECT) lds_barrier();
 #pragma unroll 1
         for (int u = 0; u < 2; ++u) {
             const int j0 = tiles.at(it) * BAND_TILE + 32 * u, j9 = j0 + 31;
@@ -283,7 +307,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
             }
         }
     }
-    band_store_row<T, DP>(const_cast<T *>(band_row<T>(a.dq, b, i, h)), dq, a.scale, a.D, a.dq.mode, hh, i < a.Lq);
+    band_store_row<T, DP, MODE>(const_cast<T *>(band_row<T>(a.dq, b, i, h)), dq, a.scale, a.D, hh, i < a.Lq);
 
     if constexpr (DTABLE) {
         // clipped distances meet in the two end entries, then the eight tables are added
@@ -338,19 +362,19 @@ template <typename K> static int allow_lds(K kern, size_t lds) {
     return e == hipSuccess ? DSW_OK : fail(DSW_ELAUNCH, "dsw_band_attn_bwd: %zu bytes of LDS: %s", lds, hipGetErrorString(e));
 }
 
-template <typename T, int DP, bool BIAS, bool DTABLE> static int launch_bwd(const BandArgs &a, hipStream_t st) {
+template <typename T, int DP, int MODE, bool BIAS, bool DTABLE> static int launch_bwd(const BandArgs &a, hipStream_t st) {
     const size_t images = (size_t)band_t<T>::nbuf(DP) * 2 * band_t<T>::template elems<DP>(BAND_TILE) * sizeof(T);
     const size_t bl = BIAS ? (2 * (a.M + BAND_MARGIN) + 1) * sizeof(float) : 0;
     if (a.Lk) {
         const size_t lds = images + (size_t)band_t<T>::nbuf(DP) * 2 * BAND_TILE * sizeof(float) + bl;
-        auto kern = band_attn_dkv_kernel<T, DP, BIAS>;
+        auto kern = band_attn_dkv_kernel<T, DP, MODE, BIAS>;
         if (int rc = allow_lds(kern, lds)) return rc;
         kern<<<dim3((unsigned)((long long)a.B * a.Hkv * ((a.Lk + BAND_ROWS - 1) / BAND_ROWS))), 256, lds, st>>>(a);
         if (int rc = check_launch("dsw_band_attn_bwd (dk, dv)")) return rc;
     }
     if (a.Lq) {
         const size_t lds = images + bl + (DTABLE ? 8 * bl : 0);
-        auto kern = band_attn_dq_kernel<T, DP, BIAS, DTABLE>;
+        auto kern = band_attn_dq_kernel<T, DP, MODE, BIAS, DTABLE>;
         if (int rc = allow_lds(kern, lds)) return rc;
         kern<<<dim3((unsigned)((long long)a.B * a.Hq * ((a.Lq + BAND_ROWS - 1) / BAND_ROWS))), 256, lds, st>>>(a);
         if (int rc = check_launch("dsw_band_attn_bwd (dq)")) return rc;
@@ -363,13 +387,6 @@ static size_t round16(size_t n) { return (n + 3) & ~(size_t)3; }
 }  // namespace dsw
 
 using namespace dsw;
-
-#define DSW_BAND_DISPATCH(dtype, D, T, DP, ...)                                   \
-    DSW_DISPATCH_DTYPE(dtype, T, {                                                \
-        if ((D) <= 32) { constexpr int DP = 32; __VA_ARGS__; }                    \
-        else if ((D) <= 64) { constexpr int DP = 64; __VA_ARGS__; }               \
-        else { constexpr int DP = 128; __VA_ARGS__; }                             \
-    })
 
 extern "C" size_t dsw_band_attn_bwd_workspace(const dsw_band_desc *d) {
     BandArgs a;
@@ -390,10 +407,11 @@ extern "C" int dsw_band_attn_bwd(const dsw_band_desc *d, const void *q, const ds
     if (rc) return rc;
     if (a.B == 0 || a.Hq == 0) return DSW_OK;
     const bool no_rows = a.Lq == 0, no_keys = a.Lk == 0;
-    if ((rc = band_tensor(who, "q", q, sq, d->dtype, a.D, no_rows, a.q)) || (rc = band_tensor(who, "k", k, sk, d->dtype, a.D, no_keys, a.k)) ||
-        (rc = band_tensor(who, "v", v, sv, d->dtype, a.D, no_keys, a.v)) || (rc = band_tensor(who, "out", out, so, d->dtype, a.D, no_rows, a.out)) ||
-        (rc = band_tensor(who, "dout", dout, sdo, d->dtype, a.D, no_rows, a.dout)) || (rc = band_tensor(who, "dq", dq, sdq, d->dtype, a.D, no_rows, a.dq)) ||
-        (rc = band_tensor(who, "dk", dk, sdk, d->dtype, a.D, no_keys, a.dk)) || (rc = band_tensor(who, "dv", dv, sdv, d->dtype, a.D, no_keys, a.dv)))
+    int mode = 0;
+    if ((rc = band_tensor(who, "q", q, sq, d->dtype, a.D, no_rows, a.q, mode)) || (rc = band_tensor(who, "k", k, sk, d->dtype, a.D, no_keys, a.k, mode)) ||
+        (rc = band_tensor(who, "v", v, sv, d->dtype, a.D, no_keys, a.v, mode)) || (rc = band_tensor(who, "out", out, so, d->dtype, a.D, no_rows, a.out, mode)) ||
+        (rc = band_tensor(who, "dout", dout, sdo, d->dtype, a.D, no_rows, a.dout, mode)) || (rc = band_tensor(who, "dq", dq, sdq, d->dtype, a.D, no_rows, a.dq, mode)) ||
+        (rc = band_tensor(who, "dk", dk, sdk, d->dtype, a.D, no_keys, a.dk, mode)) || (rc = band_tensor(who, "dv", dv, sdv, d->dtype, a.D, no_keys, a.dv, mode)))
         return rc;
     DSW_REQUIRE(no_rows || lse, "%s: null lse", who);
     DSW_REQUIRE(d_table == nullptr || a.table, "%s: a gradient for a table that is not there", who);
@@ -407,11 +425,15 @@ extern "C" int dsw_band_attn_bwd(const dsw_band_desc *d, const void *q, const ds
     if (!no_rows) {
         const long long rows = (long long)a.B * a.Lq * a.Hq;
         const dim3 grid((unsigned)((rows + 15) / 16));
-        DSW_DISPATCH_DTYPE(d->dtype, T, (band_attn_delta_kernel<T><<<grid, 256, 0, st>>>(a)));
+        DSW_DISPATCH_DTYPE(d->dtype, T, {
+            if (mode == 0) band_attn_delta_kernel<T, 0><<<grid, 256, 0, st>>>(a);
+            else band_attn_delta_kernel<T, 2><<<grid, 256, 0, st>>>(a);
+        });
         if ((rc = check_launch("dsw_band_attn_bwd (delta)"))) return rc;
     }
-    DSW_BAND_DISPATCH(d->dtype, a.D, T, DP, {
-        rc = d_table ? launch_bwd<T, DP, true, true>(a, st) : a.table ? launch_bwd<T, DP, true, false>(a, st) : launch_bwd<T, DP, false, false>(a, st);
+    DSW_BAND_DISPATCH(d->dtype, a.D, mode, T, DP, MODE, {
+        rc = d_table ? launch_bwd<T, DP, MODE, true, true>(a, st)
+             : a.table ? launch_bwd<T, DP, MODE, true, false>(a, st) : launch_bwd<T, DP, MODE, false, false>(a, st);
     });
     if (rc || d_table == nullptr) return rc;
     const int n = 2 * a.M + 1, rows = a.B * ((a.Lq + BAND_ROWS - 1) / BAND_ROWS);

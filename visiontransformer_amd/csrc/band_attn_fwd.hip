@@ -10,7 +10,7 @@
 
 namespace dsw {
 
-template <typename T, int DP, bool BIAS, bool EXACT>
+template <typename T, int DP, int MODE, bool BIAS, bool EXACT>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void band_attn_fwd_kernel(const BandArgs a) {
     constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE);
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -38,112 +38,137 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     typename band_t<T>::frag qf[DP / 16];
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
-        if (row_on) qf[c] = band_load8(qrow, 16 * c + 8 * hh, a.D, a.q.mode);
+        if (row_on) qf[c] = band_load8<MODE>(qrow, 16 * c + 8 * hh, a.D);
         else band_clear(qf[c]);
     }
     f32x16 o[DP / 32];
-#pragma unroll
-    for (int db = 0; db < DP / 32; ++db) o[db] = band_zero();
-    float m = -INFINITY, l = 0.f;
+    float m, l;
 
-    BandStage<T, DP> ks, vs;
-    if (tiles.count) {
-        const int j0 = tiles.at(0) * BAND_TILE;
-        ks.load(kbase, a.k.s.l, j0, sq.kn, a.D, a.k.mode);
-        vs.load(vbase, a.v.s.l, j0, sq.kn, a.D, a.v.mode);
+    BandStage<T, DP, MODE> ks, vs;
+    ks.init(kbase, a.k.s.l);
+    vs.init(vbase, a.v.s.l);
+    if (MODE == 1 && a.D < DP) {
+        BandStage<T, DP, MODE>::clear(lds, NB * 2 * BAND_TILE, a.D);
+        __syncthreads();
     }
-    for (int it = 0; it < tiles.count; ++it) {
-        T *const K = lds + (NB == 2 ? (it & 1) : 0) * 2 * ELEMS, *const V = K + ELEMS;
-        if constexpr (NB == 1) lds_barrier();
-        ks.put(K);
-        vs.put(V);
-        if (it + 1 < tiles.count) {
-            const int j1 = tiles.at(it + 1) * BAND_TILE;
-            ks.load(kbase, a.k.s.l, j1, sq.kn, a.D, a.k.mode);
-            vs.load(vbase, a.v.s.l, j1, sq.kn, a.D, a.v.mode);
-        }
-        lds_barrier();
-        const int j0 = tiles.at(it) * BAND_TILE, j9 = j0 + BAND_TILE - 1;
-        if (!wave_on || j0 > w_hi + a.right || (j9 < w_lo - a.left && j0 >= a.sinks)) continue;
-        const bool full = j9 < sq.kn && j9 <= w_lo + a.right && (j0 >= w_hi - a.left || j9 < a.sinks);
-
-        f32x16 s[2];
+    bool safe = false;
+    for (;;) {
+        m = -INFINITY;
+        l = 0.f;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            s[u] = band_zero();
-#pragma unroll
-            for (int c = 0; c < DP / 16; ++c) s[u] = band_mma(band_rows<DP>(K, 32 * u + l31, c, hh), qf[c], s[u]);
+        for (int db = 0; db < DP / 32; ++db) o[db] = band_zero();
+        bool fresh = true;  // some row has no reference yet
+        if (tiles.count) {
+            ks.fetch(tiles.at(0) * BAND_TILE, sq.kn, a.D, lds);
+            vs.fetch(tiles.at(0) * BAND_TILE, sq.kn, a.D, lds + ELEMS);
         }
-        float bu = 0.f;  // bias of a tile whose distances are all clipped
-        bool near = false;
-        if constexpr (BIAS) {
-            near = j9 - w_lo > -a.M && j0 - w_hi < a.M;
-            if (near) {
-                const float *br = bias + (j0 + 4 * hh - p + a.M + BAND_MARGIN);
+        for (int it = 0; it < tiles.count; ++it) {
+            T *const K = lds + (NB == 2 ? (it & 1) : 0) * 2 * ELEMS, *const V = K + ELEMS;
+            if constexpr (!BandStage<T, DP, MODE>::DIRECT) {
+                if constexpr (NB == 1) lds_barrier();
+                ks.put(K, a.D);
+                vs.put(V, a.D);
+            } else {
+                band_landed();
+                lds_barrier();
+            }
+            if (it + 1 < tiles.count) {
+                T *const K1 = lds + (NB == 2 ? ((it + 1) & 1) : 0) * 2 * ELEMS;
+                ks.fetch(tiles.at(it + 1) * BAND_TILE, sq.kn, a.D, K1);
+                vs.fetch(tiles.at(it + 1) * BAND_TILE, sq.kn, a.D, K1 + ELEMS);
+            }
+            if constexpr (!BandStage<T, DP, MODE>::DIRECT) lds_barrier();
+            const int j0 = tiles.at(it) * BAND_TILE, j9 = j0 + BAND_TILE - 1;
+            if (!wave_on || j0 > w_hi + a.right || (j9 < w_lo - a.left && j0 >= a.sinks)) continue;
+            const bool full = j9 < sq.kn && j9 <= w_lo + a.right && (j0 >= w_hi - a.left || j9 < a.sinks);
+            f32x16 s[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                s[u] = band_zero();
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) s[u] = band_mma(band_rows<DP>(K, 32 * u + l31, c, hh), qf[c], s[u]);
+            }
+            float cs = a.c, bu = 0.f;  // the logits are cs * s + bu
+            if constexpr (BIAS) {
+                if (j9 - w_lo > -a.M && j0 - w_hi < a.M) {
+                    const float *br = bias + (j0 + 4 * hh - p + a.M + BAND_MARGIN);
+                    cs = 1.f;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[u][r] = __builtin_fmaf(s[u][r], a.c, br[32 * u + rho(r)]);
+                } else {
+                    bu = bias[j0 > w_hi ? 2 * (a.M + BAND_MARGIN) : 0];  // (all distances clipped: one bias)
+                }
+            }
+            if (!full) {
+                const BandMask mask = band_row_mask(a, p, sq.kn, j0 + 4 * hh);
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[u][r] = __builtin_fmaf(s[u][r], a.c, br[32 * u + rho(r)]);
-            } else {
-                bu = bias[j0 > w_hi ? 2 * (a.M + BAND_MARGIN) : 0];
+                    for (int r = 0; r < 16; ++r) s[u][r] = mask.sees(32 * u + rho(r)) ? s[u][r] : -INFINITY;
             }
-        }
-        if (!full) {
-            const BandMask mask = band_row_mask(a, p, sq.kn, j0 + 4 * hh);
+            if (fresh || safe) {
+                float x = s[0][0];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+                for (int r = 1; r < 32; ++r) x = fmaxf(x, s[r >> 4][r & 15]);
+                x = max_across_halves(__builtin_fmaf(x, cs, bu));
+                const float mn = m == -INFINITY || safe ? fmaxf(m, x) : m;
+                const float alpha = mn == m || m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= alpha;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[u][r] = mask.sees(32 * u + rho(r)) ? s[u][r] : -INFINITY;
-        }
-        float x = -INFINITY;
+                for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) x = fmaxf(x, s[u][r]);
-        const float c = BIAS && near ? 1.f : a.c;
-        x = max_across_halves(__builtin_fmaf(x, c, bu));
-        if (__any(x > m + 8.f)) {
-            const float mn = fmaxf(m, x), alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= alpha;
-#pragma unroll
-            for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-        }
-        const float shift = bu - (m == -INFINITY ? 0.f : m);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], c, shift));
-                l += s[u][r];
+                    for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+                fresh = __any((int)row_on & (int)(m == -INFINITY));
             }
+            const float shift = bu - (m == -INFINITY ? 0.f : m);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                typename band_t<T>::frag pf;
-                band_pack(s[u], k, pf);
+            for (int u = 0; u < 2; ++u) {
 #pragma unroll
-                for (int db = 0; db < DP / 32; ++db) {
-                    const auto vf = band_cols<DP>(V, 32 * u + 16 * k, db, lane);
-                    o[db] = band_mma(vf, pf, o[db]);
-                    if constexpr (EXACT && sizeof(T) == 2) {
-                        uint4 rf;
+                for (int r = 0; r < 16; ++r) s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], cs, shift));
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    typename band_t<T>::frag pf, rf;
+                    band_pack(s[u], k, pf);
+                    l = band_sum(pf, l);
+                    if constexpr (EXACT) {
                         band_pack_rest(s[u], k, pf, rf);
-                        o[db] = band_mma(vf, rf, o[db]);
+                        l = band_sum(rf, l);
+                    }
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) {
+                        const auto vf = band_cols<DP>(V, 32 * u + 16 * k, db, lane);
+                        o[db] = band_mma(vf, pf, o[db]);
+                        if constexpr (EXACT) o[db] = band_mma(vf, rf, o[db]);
                     }
                 }
             }
+            if (__any(l > 0x1p60f)) {  // far above the reference: move it up
+                const float up = l > 0x1p60f ? 0x1p-60f : 1.f, both = fminf(up, __shfl_xor(up, 32, 64));
+                m += both < 1.f ? 60.f : 0.f;
+                l *= both;
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[db][r] *= both;
+            }
         }
+        float bad = l * 0.f;
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) bad = __builtin_fmaf(o[db][r], 0.f, bad);
+        const bool again = __syncthreads_or(row_on && bad != 0.f);
+        if (!again) break;
+        if (safe) {
+            if (__any(row_on && bad != 0.f))
+                band_careful<T, DP, BIAS, BAND_TILE>(a, qrow, kbase, vbase, h, p, row_on, sq.kn, tiles, 0, tiles.count, 1, hh, m, l, o);
+            break;
+        }
+        safe = true;
     }
-
-    float bad = 0.f;
-#pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) bad = __builtin_fmaf(o[db][r], 0.f, bad);
-    if (__any(bad != 0.f))
-        band_careful<T, DP, BIAS, BAND_TILE>(a, qrow, kbase, vbase, h, p, row_on, sq.kn, tiles, 0, tiles.count, 1, hh, m, l, o);
 
     l += __shfl_xor(l, 32, 64);
     const float inv = !row_on || l == 0.f ? 0.f : 1.f / l;
@@ -152,17 +177,17 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[db][r] = row_on ? o[db][r] : 0.f;
     const bool store = i < a.Lq;
-    band_store_row<T, DP>(const_cast<T *>(band_row<T>(a.out, b, i, h)), o, inv, a.D, a.out.mode, hh, store);
-    if constexpr (EXACT)
-        band_store_row<float, DP>(a.out32 + (((size_t)b * a.Lq + i) * a.Hq + h) * a.D, o, inv, a.D, a.D % 4 ? 2 : 0, hh, store);
+    band_store_row<T, DP, MODE>(const_cast<T *>(band_row<T>(a.out, b, i, h)), o, inv, a.D, hh, store);
+    if constexpr (EXACT)  // (in mode 0 D is a multiple of 8)
+        band_store_row<float, DP, MODE>(a.out32 + (((size_t)b * a.Lq + i) * a.Hq + h) * a.D, o, inv, a.D, hh, store);
     if (a.lse && store && hh == 0)
         a.lse[((size_t)b * a.Hq + h) * a.Lq + i] = !row_on || l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
-template <typename T, int DP, bool BIAS, bool EXACT> static int launch_fwd(const BandArgs &a, hipStream_t st) {
+template <typename T, int DP, int MODE, bool BIAS, bool EXACT> static int launch_fwd(const BandArgs &a, hipStream_t st) {
     const size_t lds = (size_t)band_t<T>::nbuf(DP) * 2 * band_t<T>::template elems<DP>(BAND_TILE) * sizeof(T) +
                        (BIAS ? (2 * (a.M + BAND_MARGIN) + 1) * sizeof(float) : 0);
-    auto kern = band_attn_fwd_kernel<T, DP, BIAS, EXACT>;
+    auto kern = band_attn_fwd_kernel<T, DP, MODE, BIAS, EXACT>;
     if (lds > 65536) {
         hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return fail(DSW_ELAUNCH, "dsw_band_attn_fwd: %zu bytes of LDS: %s", lds, hipGetErrorString(e));
@@ -172,14 +197,15 @@ template <typename T, int DP, bool BIAS, bool EXACT> static int launch_fwd(const
     return check_launch("dsw_band_attn_fwd");
 }
 
-int band_tensor(const char *who, const char *name, const void *p, const dsw_strides *s, int dtype, int D, bool null_ok, BandTensor &t) {
+int band_tensor(const char *who, const char *name, const void *p, const dsw_strides *s, int dtype, int D, bool null_ok, BandTensor &t, int &mode) {
     DSW_REQUIRE((p && s) || null_ok, "%s: null %s", who, name);
     t.p = p;
     t.s = s ? *s : dsw_strides{0, 0, 0};
+    DSW_REQUIRE(t.s.b >= 0 && t.s.l >= 0 && t.s.h >= 0, "%s: negative stride of %s", who, name);
     const int size = dtype == DSW_F32 ? 4 : 2, wide = 16 / size;
-    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-    auto fits = [&](int n) { return D % n == 0 && at % (n * size) == 0 && t.s.b % n == 0 && t.s.l % n == 0 && t.s.h % n == 0; };
-    t.mode = fits(wide) ? 0 : fits(4 / size) ? 1 : 2;
+    const bool whole = D % wide == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && t.s.b % wide == 0 && t.s.l % wide == 0 && t.s.h % wide == 0;
+    const int m = D < 8 || t.s.l * size * BAND_TILE >= (1LL << 31) ? 2 : whole ? 0 : 1;
+    mode = m > mode ? m : mode;
     return DSW_OK;
 }
 
@@ -216,13 +242,6 @@ int band_make_args(const char *who, const dsw_band_desc *d, BandArgs &a) {
 
 using namespace dsw;
 
-#define DSW_BAND_DISPATCH(dtype, D, T, DP, ...)                                   \
-    DSW_DISPATCH_DTYPE(dtype, T, {                                                \
-        if ((D) <= 32) { constexpr int DP = 32; __VA_ARGS__; }                    \
-        else if ((D) <= 64) { constexpr int DP = 64; __VA_ARGS__; }               \
-        else { constexpr int DP = 128; __VA_ARGS__; }                             \
-    })
-
 extern "C" size_t dsw_band_attn_fwd_workspace(const dsw_band_desc *d) {
     int nrb = 0, nsplit = 0;
     BandArgs a;
@@ -240,8 +259,9 @@ extern "C" int dsw_band_attn_fwd(const dsw_band_desc *d, const void *q, const ds
     if (rc) return rc;
     if (a.B == 0 || a.Lq == 0 || a.Hq == 0) return DSW_OK;
     const bool no_keys = a.Lk == 0;
-    if ((rc = band_tensor(who, "q", q, sq, d->dtype, a.D, false, a.q)) || (rc = band_tensor(who, "k", k, sk, d->dtype, a.D, no_keys, a.k)) ||
-        (rc = band_tensor(who, "v", v, sv, d->dtype, a.D, no_keys, a.v)) || (rc = band_tensor(who, "out", out, so, d->dtype, a.D, false, a.out)))
+    int mode = 0;
+    if ((rc = band_tensor(who, "q", q, sq, d->dtype, a.D, false, a.q, mode)) || (rc = band_tensor(who, "k", k, sk, d->dtype, a.D, no_keys, a.k, mode)) ||
+        (rc = band_tensor(who, "v", v, sv, d->dtype, a.D, no_keys, a.v, mode)) || (rc = band_tensor(who, "out", out, so, d->dtype, a.D, false, a.out, mode)))
         return rc;
     DSW_REQUIRE(out32 == nullptr || (a.table && d->dtype == DSW_BF16), "%s: out32 goes with a bias table and bf16 tensors", who);
     a.lse = lse;
@@ -251,13 +271,13 @@ extern "C" int dsw_band_attn_fwd(const dsw_band_desc *d, const void *q, const ds
         const size_t need = dsw_band_attn_fwd_workspace(d);
         DSW_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "%s: workspace of %zu bytes, %zu are needed", who, workspace_bytes, need);
         a.partial = static_cast<float *>(workspace);
-        return band_launch_step(a, d->dtype, st);
+        return band_launch_step(a, d->dtype, mode, st);
     }
-    DSW_BAND_DISPATCH(d->dtype, a.D, T, DP, {
+    DSW_BAND_DISPATCH(d->dtype, a.D, mode, T, DP, MODE, {
         if constexpr (sizeof(T) == 2) {
-            if (out32) return launch_fwd<T, DP, true, true>(a, st);
+            if (out32) return launch_fwd<T, DP, MODE, true, true>(a, st);
         }
-        return a.table ? launch_fwd<T, DP, true, false>(a, st) : launch_fwd<T, DP, false, false>(a, st);
+        return a.table ? launch_fwd<T, DP, MODE, true, false>(a, st) : launch_fwd<T, DP, MODE, false, false>(a, st);
     });
     return DSW_OK;
 }

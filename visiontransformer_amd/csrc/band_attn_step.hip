@@ -12,7 +12,7 @@ namespace dsw {
 
 constexpr int STEP_KEYS = 32;
 
-template <typename T, int DP, bool BIAS>
+template <typename T, int DP, int MODE, bool BIAS>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void band_attn_step_kernel(const BandArgs a) {
     constexpr int ELEMS = band_t<T>::template elems<DP>(STEP_KEYS);
     constexpr int SLOTS = DP / 8, NV = STEP_KEYS * SLOTS / 64, STEP = 64 / SLOTS;
@@ -40,8 +40,18 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     typename band_t<T>::frag qf[DP / 16];
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
-        if (row_on) qf[c] = band_load8(qrow, 16 * c + 8 * hh, a.D, a.q.mode);
-        else band_clear(qf[c]);
+        band_clear(qf[c]);
+        if (row_on) qf[c] = band_load8<MODE>(qrow, 16 * c + 8 * hh, a.D);
+        if constexpr (MODE == 1) {
+            // K's piece there is the one that ends with the row (see load below): the query's columns go where it has them
+            const int col = 16 * c + 8 * hh, back = col + 8 - a.D;
+            if (row_on && back > 0) {
+                T e[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) e[k] = k >= back ? qrow[a.D - 8 + k] : (T)0;
+                __builtin_memcpy(&qf[c], e, sizeof(e));
+            }
+        }
     }
     f32x16 o[DP / 32];
 #pragma unroll
@@ -49,30 +59,47 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     float m = -INFINITY, l = 0.f;
 
     typename band_t<T>::frag kf[DP / 16], vf[NV];
+    // Keys that no row of the block sees are not read (they may be uninitialised parts of a cache): a visible one stands in
+    // for them, and the mask drops it.
+    const int j_lo = max(0, p_lo - a.left), j_hi = min(sq.kn - 1, p_hi + a.right);
     auto load = [&](int j0) {
-        // (rows that no query of the block sees are not read: they may be uninitialised parts of a cache)
-        auto wanted = [&](int j) { return j < sq.kn && j <= p_hi + a.right && (j >= p_lo - a.left || j < a.sinks); };
-        const int j = j0 + l31;
-        const T *kr = kbase + (long long)j * a.k.s.l;
-        const bool on = wanted(j);
+        auto stand_in = [&](int j) { return min(j >= j_lo || j < a.sinks ? j : j_lo, j_hi); };
+        const T *kr = kbase + (long long)stand_in(j0 + l31) * a.k.s.l;
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) {
-            if (on) kf[c] = band_load8(kr, 16 * c + 8 * hh, a.D, a.k.mode);
-            else band_clear(kf[c]);
+            const int col = 16 * c + 8 * hh;
+            if constexpr (MODE == 1) kf[c] = band_piece(kr + min(col, a.D - 8));
+            else kf[c] = band_load8<MODE>(kr, col, a.D);
         }
         const int r = lane / SLOTS, col = 8 * (lane % SLOTS);
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-            const int jv = j0 + r + n * STEP;
-            if (wanted(jv)) vf[n] = band_load8(vbase + (long long)jv * a.v.s.l, col, a.D, a.v.mode);
-            else band_clear(vf[n]);
+            const T *vr = vbase + (long long)stand_in(j0 + r + n * STEP) * a.v.s.l;
+            if constexpr (MODE == 1) vf[n] = band_piece(vr + min(col, a.D - 8));
+            else vf[n] = band_load8<MODE>(vr, col, a.D);
         }
     };
+    auto put = [&]() {
+        const int r = lane / SLOTS, slot = lane % SLOTS;
+        if (MODE != 1 || 8 * slot + 8 <= a.D) {
+#pragma unroll
+            for (int n = 0; n < NV; ++n) band_put<DP>(V, r + n * STEP, slot, vf[n]);
+        } else if (8 * slot < a.D) {
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                T e[8];
+                __builtin_memcpy(e, &vf[n], sizeof(e));
+#pragma unroll
+                for (int k = 0; k < 8; ++k) V[band_at<T, DP>(r + n * STEP, a.D - 8 + k)] = e[k];
+            }
+        }
+    };
+    if (MODE == 1 && a.D < DP)  // the columns past D, which put() leaves alone
+        for (int e = lane; e < STEP_KEYS * (DP - a.D); e += 64) V[band_at<T, DP>(e / (DP - a.D), a.D + e % (DP - a.D))] = (T)0;
     if (t_begin < t_end) load(tiles.at(t_begin) * STEP_KEYS);
     for (int t = t_begin; t < t_end; t += 4) {
         const int j0 = tiles.at(t) * STEP_KEYS;
-#pragma unroll
-        for (int n = 0; n < NV; ++n) band_put<DP>(V, lane / SLOTS + n * STEP, lane % SLOTS, vf[n]);
+        put();
         f32x16 s = band_zero();
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) s = band_mma(kf[c], qf[c], s);
@@ -210,11 +237,11 @@ bool band_step_plan(const dsw_band_desc &d, int &nrb, int &nsplit) {
     return true;
 }
 
-template <typename T, int DP, bool BIAS> static int launch_step(const BandArgs &a, hipStream_t st) {
+template <typename T, int DP, int MODE, bool BIAS> static int launch_step(const BandArgs &a, hipStream_t st) {
     const int R = a.Lq * a.G, nrow = R < 32 ? R : 32;
     const size_t tile = (size_t)4 * band_t<T>::template elems<DP>(STEP_KEYS) * sizeof(T);
     const size_t meet = (size_t)(4 * 32 * 2 + 4 * nrow * a.D) * sizeof(float), lds = tile > meet ? tile : meet;
-    auto kern = band_attn_step_kernel<T, DP, BIAS>;
+    auto kern = band_attn_step_kernel<T, DP, MODE, BIAS>;
     if (lds > 65536) {
         hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return fail(DSW_ELAUNCH, "dsw_band_attn_fwd: %zu bytes of LDS: %s", lds, hipGetErrorString(e));
@@ -229,12 +256,8 @@ template <typename T, int DP, bool BIAS> static int launch_step(const BandArgs &
     return check_launch("dsw_band_attn_fwd (join)");
 }
 
-int band_launch_step(BandArgs &a, int dtype, hipStream_t st) {
-    DSW_DISPATCH_DTYPE(dtype, T, {
-        if (a.D <= 32) return a.table ? launch_step<T, 32, true>(a, st) : launch_step<T, 32, false>(a, st);
-        if (a.D <= 64) return a.table ? launch_step<T, 64, true>(a, st) : launch_step<T, 64, false>(a, st);
-        return a.table ? launch_step<T, 128, true>(a, st) : launch_step<T, 128, false>(a, st);
-    });
+int band_launch_step(BandArgs &a, int dtype, int mode, hipStream_t st) {
+    DSW_BAND_DISPATCH(dtype, a.D, mode, T, DP, MODE, return a.table ? launch_step<T, DP, MODE, true>(a, st) : launch_step<T, DP, MODE, false>(a, st));
     return DSW_OK;
 }
 
