@@ -22,8 +22,8 @@ struct BandTensor {
 };
 // How a call's tensors are accessed, a template argument of the kernels (a branch per access cost more than the access):
 // 0  16-byte pieces: D and all strides multiples of 16 bytes, rows 16-byte aligned; bf16 tiles go to LDS without registers
-// 1  pieces at any element offset; the last piece of a row is the one that ends with it (8 <= D)
-// 2  single elements (D < 8, or rows so far apart that a tile spans 2 GiB)
+// 1  4-byte pieces: everything a multiple of 4 bytes, and 8 <= D (heads of 30); bf16 tiles go to LDS without registers
+// 2  single elements (D < 8, odd sizes in bf16, or rows so far apart that a tile spans 2 GiB)
 
 struct BandArgs {
     BandTensor q, k, v, out, dout, dq, dk, dv;
@@ -39,6 +39,8 @@ struct BandArgs {
     float *delta;        // [B][Hq][Lq]
     float *partial;      // step kernel: see there; dQ kernel: bias gradients by distance
     int nsplit, nrb;
+    float *shares;       // dK, dV kernel: sums of the blocks that several workgroups share
+    int sink_blocks, sink_chunks, chunks;
 };
 
 // ---- element types ------------------------------------------------------------------------------------------
@@ -250,43 +252,73 @@ template <int DP> __device__ __forceinline__ band_t<float>::frag band_cols(const
 }
 
 // ---- staging of 64-row tiles by the whole workgroup (256 threads) ------------------------------------------------
-// One slice (a head of one sequence, rows `ld` apart) and its LDS images.  Rows from `limit` (>= 1) on are read as copies of
-// row limit - 1: what they hold is masked, and nothing past the sequence is touched.  Mode 0 (bf16): fetch() starts the
-// copy straight into the image, band_landed() waits for it.  Modes 1, 2: fetch() loads registers, put() writes the image,
-// whose columns past D clear() has to have zeroed once.  (Mode 0 repeats the row's last piece there: the queries
-// are zero in those columns of K, and those columns of V add to columns of the result that are not stored.)
+// Tiles of one slice (a head of one sequence, rows `ld` apart) and their LDS images.  Rows behind the last one read as copies of
+// it: what they hold is masked, and nothing past the sequence is touched.  DIRECT (bf16, modes 0 and 1): fetch()
+// starts the copy straight into the image, band_landed() waits for it; the columns past D repeat the row's last piece
+// (the queries are zero in those columns of K, and those columns of V add to columns of the result that are not stored).
+// The copies are written in assembly because the compiler, which cannot tell the images apart, would wait for them in front
+// of the first LDS read of any image; m0, which carries their destination, is used by nothing else in these kernels.
+// Otherwise fetch() loads registers and put() writes the image; in mode 1 the last piece of a row is the one that ends
+// with it, and clear() has to have zeroed the columns past D once.
 __device__ __forceinline__ void band_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ uint32_t band_lds_address(const void *p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
 }
 template <typename T, int DP, int MODE> struct BandStage {
     static constexpr int N = DP / 32, SLOTS = DP / 8, STEP = 256 / SLOTS;  // pieces per thread, per row; rows between a thread's pieces
-    static constexpr bool DIRECT = MODE == 0 && sizeof(T) == 2;
-    const char *base;
+    static constexpr bool DIRECT = MODE <= 1 && sizeof(T) == 2, DWORDS = DIRECT && MODE == 1;
+    static constexpr int COPIES = DWORDS ? 4 * N : N, BYTES = DWORDS ? 256 : 1024;  // copy instructions per wave and tile, bytes of each
     long long ld;  // bytes
-    typename band_t<T>::frag f[DIRECT ? 1 : N];
     uint32_t ld32;
+    typename band_t<T>::frag f[DIRECT ? 1 : N];
+    static constexpr bool KEPT = DIRECT && COPIES <= 4;  // (more would cost more registers than their computation takes time)
+    uint32_t off[KEPT ? COPIES : 1];  // this lane's bytes of each copy, from the tile's first row
 
-    __device__ __forceinline__ void init(const T *slice, long long row) {
-        base = reinterpret_cast<const char *>(slice);
+    // row and byte within the row of what copy i of this lane fetches: the place in the image follows from the lane, the
+    // logical piece there from the image's pattern
+    static __device__ __forceinline__ void source(int i, int D, int &r, int &byte) {
+        const int lane = threadIdx.x & 63, n = (threadIdx.x >> 6) * COPIES + i;
+        if constexpr (DWORDS) {
+            const int at = n * 64 + lane, w = at % (DP / 2);
+            r = at / (DP / 2);
+            byte = 2 * min((((w >> 2) ^ band_flip<DP>(r)) << 3) + 2 * (w & 3), D - 2);
+        } else {
+            r = n * (64 / SLOTS) + lane / SLOTS;
+            byte = 16 * min((lane % SLOTS) ^ band_flip<DP>(r), D / 8 - 1);
+        }
+    }
+    __device__ __forceinline__ void init(long long row, int D) {
         ld = row * (long long)sizeof(T);
         ld32 = (uint32_t)ld;
-    }
-    // rows row0 .. row0 + 63
-    __device__ __forceinline__ void fetch(int row0, int limit, int D, T *image) {
-        const char *tile = base + (long long)row0 * ld;
-        const int last = limit - 1 - row0;  // last row of the tile that exists
-        if constexpr (DIRECT) {
-            const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if constexpr (KEPT) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                // one instruction fills 1 KiB of the image: lane's 16 bytes belong to row r, and hold the logical piece that
-                // the image's pattern puts there
-                const int r = (wave * N + i) * (64 / SLOTS) + lane / SLOTS;
-                const int slot = min((lane % SLOTS) ^ band_flip<DP>(r), D / 8 - 1);
-                const uint32_t off = (uint32_t)min(r, last) * ld32 + 16 * slot;
-                const uint32_t to = __builtin_amdgcn_readfirstlane(band_lds_address(image) + (wave * N + i) * 1024);
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(tile) : "memory", "m0");
+            for (int i = 0; i < COPIES; ++i) {
+                int r, byte;
+                source(i, D, r, byte);
+                off[i] = (uint32_t)r * ld32 + byte;
+            }
+        }
+    }
+    // the 64 rows at `tile`, of which rows 0 .. last exist
+    __device__ __forceinline__ void fetch(const char *tile, int last, int D, T *image) {
+        if constexpr (DIRECT) {
+            const uint32_t to = __builtin_amdgcn_readfirstlane(band_lds_address(image) + (threadIdx.x >> 6) * (COPIES * BYTES));
+            const uint64_t at = reinterpret_cast<uint64_t>(tile);  // (the same in all lanes, which the compiler does not always see)
+            // (readfirstlane returns an int: without the casts a low half with its top bit set would fill the high half)
+            const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32));
+            const uint64_t rows = ((uint64_t)hi << 32) | lo;
+#pragma unroll
+            for (int i = 0; i < COPIES; ++i) {
+                uint32_t from = off[KEPT ? i : 0];
+                if (!KEPT || last < BAND_TILE - 1) {
+                    int r, byte;
+                    source(i, D, r, byte);
+                    from = (uint32_t)min(r, last) * ld32 + byte;
+                }
+                if constexpr (DWORDS)
+                    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to + i * BYTES), "v"(from), "s"(rows) : "memory");
+                else
+                    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to + i * BYTES), "v"(from), "s"(rows) : "memory");
             }
         } else {
             const int r0 = threadIdx.x / SLOTS, col = 8 * (threadIdx.x % SLOTS);
@@ -324,7 +356,7 @@ template <typename T, int DP, int MODE> struct BandStage {
     }
     // zeros in the columns past D of `rows` rows of images, by the whole workgroup; a barrier is the caller's
     static __device__ __forceinline__ void clear(T *image, int rows, int D) {
-        if constexpr (MODE == 1)
+        if constexpr (MODE == 1 && !DIRECT)
             for (int e = threadIdx.x; e < rows * (DP - D); e += 256) image[band_at<T, DP>(e / (DP - D), D + e % (DP - D))] = (T)0;
     }
 };
@@ -358,6 +390,19 @@ template <int SIZE> __device__ __forceinline__ BandTiles band_tiles(const BandAr
     return t;
 }
 
+// the walk over them: first key and its rows' address in a slice, without a multiplication per tile
+struct BandWalk {
+    const char *base, *p;
+    long long step, jump;
+    __device__ __forceinline__ void init(const void *slice, long long ld_bytes, int size, const BandTiles &t) {
+        base = static_cast<const char *>(slice);
+        step = ld_bytes * size;
+        jump = step * t.first;
+        p = t.n_sink ? base : base + jump;
+    }
+    __device__ __forceinline__ void next(int i, const BandTiles &t) { p = i == t.n_sink ? base + jump : p + step; }  // to tile i
+};
+
 // the bias of one head by distance, times log2(e), in LDS: entry e is distance sign * (e - M - BAND_MARGIN), clipped
 __device__ __forceinline__ float band_bias_at(const BandArgs &a, int head, int rel) {
     const int m = min(max(rel, -a.M), a.M) + a.M;
@@ -379,6 +424,41 @@ struct BandMask {
 __device__ __forceinline__ BandMask band_row_mask(const BandArgs &a, int p, int kn, int base) {
     return {min(kn - 1, p + a.right) - base, p - a.left - base, a.sinks - base};
 }
+
+// A 64-key or 32-key tile against the 32 rows of a wave, decided by a handful of scalars made once per wave
+template <int SIZE> struct BandEdges {
+    int none_hi, none_lo, hi_ok, lo_ok, sinks;
+    __device__ __forceinline__ void init(const BandArgs &a, int kn, int w_lo, int w_hi, bool on) {
+        none_hi = on ? min(kn - 1, w_hi + a.right) : -1;   // j0 beyond: no key of the tile is seen
+        none_lo = w_lo - a.left - (SIZE - 1);              // j0 before, and no sink: likewise
+        hi_ok = min(kn - SIZE, w_lo + a.right - (SIZE - 1));  // j0 up to here: no row's right end cuts the tile
+        lo_ok = w_hi - a.left;                             // j0 from here: no row's left end does
+        sinks = a.sinks;
+    }
+    __device__ __forceinline__ bool none(int j0) const { return j0 > none_hi || (j0 < none_lo && j0 >= sinks); }
+    __device__ __forceinline__ bool cut_hi(int j0) const { return j0 > hi_ok; }
+    __device__ __forceinline__ bool cut_lo(int j0) const { return j0 < lo_ok && j0 + SIZE > sinks; }
+};
+
+// The 128 query rows of a workgroup (forward, dQ).  Made twice, before the loop and after it, from the arguments: what only
+// the end needs does not have to be kept in scalar registers through the loop, which were spilled for it.
+struct BandPlace {
+    int b, h, hk, i_lo, i0, i;
+    BandSeq sq;
+    BandTiles tiles;
+    __device__ __forceinline__ BandPlace(const BandArgs &a, int block, int blocks) {
+        const int nqb = (a.Lq + BAND_ROWS - 1) / BAND_ROWS;
+        const int idx = xcd_remap(block, blocks);
+        const int g = idx % a.G, rest = idx / a.G;
+        const int qb = nqb - 1 - rest % nqb, bh = rest / nqb;  // (the last rows of a causal call have the most to do: first)
+        hk = bh % a.Hkv, b = bh / a.Hkv, h = hk * a.G + g;
+        i_lo = qb * BAND_ROWS;
+        i0 = i_lo + 32 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        i = i0 + (threadIdx.x & 31);
+        sq = band_seq(a, b);
+        tiles = band_tiles<BAND_TILE>(a, sq.kn, sq.off + i_lo, sq.off + min(i_lo + BAND_ROWS, sq.qn) - 1);
+    }
+};
 
 // Non-finite values in keys or values that a row does not see must not reach it: a probability of zero times an
 // infinity is not zero.  The tiles' products cannot tell, so a wave that ends with a non-finite result (seen nowhere
@@ -423,25 +503,22 @@ __device__ __forceinline__ void band_careful(const BandArgs &a, const T *qrow, c
 int band_make_args(const char *who, const dsw_band_desc *d, BandArgs &a);
 // fills t and raises `mode` to what the tensor needs
 int band_tensor(const char *who, const char *name, const void *p, const dsw_strides *s, int dtype, int D, bool null_ok, BandTensor &t, int &mode);
-// (T, DP, MODE) for a call: mode 2 serves narrow heads, or anything, through its widest image
+// (T, DP, MODE) for a call
 #define DSW_BAND_DISPATCH(dtype, D, mode, T, DP, MODE, ...)                                                           \
     DSW_DISPATCH_DTYPE(dtype, T, {                                                                                      \
-        if ((mode) == 2) {                                                                                              \
-            constexpr int MODE = 2;                                                                                     \
-            if ((D) <= 32) { constexpr int DP = 32; __VA_ARGS__; }                                                      \
-            else { constexpr int DP = 128; __VA_ARGS__; }                                                               \
-        } else if ((mode) == 1) {                                                                                       \
-            constexpr int MODE = 1;                                                                                     \
-            if ((D) <= 32) { constexpr int DP = 32; __VA_ARGS__; }                                                      \
-            else if ((D) <= 64) { constexpr int DP = 64; __VA_ARGS__; }                                                 \
-            else { constexpr int DP = 128; __VA_ARGS__; }                                                               \
-        } else {                                                                                                        \
-            constexpr int MODE = 0;                                                                                     \
-            if ((D) <= 32) { constexpr int DP = 32; __VA_ARGS__; }                                                      \
-            else if ((D) <= 64) { constexpr int DP = 64; __VA_ARGS__; }                                                 \
-            else { constexpr int DP = 128; __VA_ARGS__; }                                                               \
-        }                                                                                                               \
+        if ((mode) == 2) { constexpr int MODE = 2; DSW_BAND_WIDTHS(D, DP, __VA_ARGS__) }                                \
+        else if ((mode) == 1) { constexpr int MODE = 1; DSW_BAND_WIDTHS(D, DP, __VA_ARGS__) }                           \
+        else { constexpr int MODE = 0; DSW_BAND_WIDTHS(D, DP, __VA_ARGS__) }                                            \
     })
+#define DSW_BAND_WIDTHS(D, DP, ...)                               \
+    if ((D) <= 32) { constexpr int DP = 32; __VA_ARGS__; }        \
+    else if ((D) <= 64) { constexpr int DP = 64; __VA_ARGS__; }   \
+    else { constexpr int DP = 128; __VA_ARGS__; }
+// how the dK, dV kernel shares its key blocks out (band_attn_bwd.hip)
+struct BandChunks {
+    int sink_blocks, sink_chunks, chunks;
+    long long shares;  // workgroups that write a share
+};
 // launches the kernel for few query rows (band_attn_step.hip) and the one that joins its splits
 int band_launch_step(BandArgs &a, int dtype, int mode, hipStream_t st);
 // whether a call goes there, and how many row blocks and splits it has

@@ -41,17 +41,26 @@ template <typename T, int MODE> __global__ __launch_bounds__(256) void band_attn
 }
 
 // ---- dk, dv: 128 keys of a workgroup, 32 per wave -----------------------------------------------------------------
+// A key block's work is its row tiles times the query heads that share the keys.  Blocks of sinks are seen by every row
+// behind them, the others by a window's; and where there are few blocks, one workgroup each does not fill the chip.  So a
+// block is cut into `chunks` (`sink_chunks`) runs of that work; more than one leave fp32 sums in `shares`, which
+// band_attn_join_dkv_kernel adds in their order.
 template <typename T, int DP, int MODE, bool BIAS>
 __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void band_attn_dkv_kernel(const BandArgs a) {
-    constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE);
+    constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE), C = DP / 16;
+    constexpr bool AHEAD = DP < 128 && sizeof(T) == 2;  // registers for LDS reads well ahead of the products that need them
+    using Stage = BandStage<T, DP, MODE>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     T *const lds = reinterpret_cast<T *>(smem);                        // [NB][Q | dO]
-    float *const stats = reinterpret_cast<float *>(lds + NB * 2 * ELEMS);  // [NB][lse | delta][64]
+    float *const stats = reinterpret_cast<float *>(lds + NB * 2 * ELEMS);  // [NB][-lse | delta][64]
     float *const bias = stats + NB * 2 * BAND_TILE;
 
-    const int nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS;
+    const int nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS, units = a.sink_blocks * a.sink_chunks + (nkb - a.sink_blocks) * a.chunks;
     const int idx = xcd_remap(blockIdx.x, gridDim.x);
-    const int kb = idx % nkb, bh = idx / nkb, hk = bh % a.Hkv, b = bh / a.Hkv;
+    const int bh = idx / units, unit = idx - bh * units, hk = bh % a.Hkv, b = bh / a.Hkv;
+    const bool of_sinks = unit < a.sink_blocks * a.sink_chunks;
+    const int nc = of_sinks ? a.sink_chunks : a.chunks, left_over = unit - (of_sinks ? 0 : a.sink_blocks * a.sink_chunks);
+    const int kb = (of_sinks ? 0 : a.sink_blocks) + left_over / nc, chunk = left_over % nc;
     const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const BandSeq sq = band_seq(a, b);
@@ -63,11 +72,13 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
     const int first = max(0, k_lo - a.right - sq.off) / BAND_TILE;
     const int last_row = k_lo < a.sinks ? sq.qn - 1 : min(sq.qn - 1, k_hi + a.left - sq.off);
     const int n_tiles = k_lo < sq.kn && last_row >= 0 ? max(0, last_row / BAND_TILE - first + 1) : 0;
+    // this chunk's steps: the tiles of the first head, of the second, ...
+    const int share = (n_tiles * a.G + nc - 1) / nc, begin = min(chunk * share, n_tiles * a.G), end = min(begin + share, n_tiles * a.G);
 
-    typename band_t<T>::frag kf[DP / 16], vf[DP / 16];
+    typename band_t<T>::frag kf[C], vf[C];
     const T *const krow = band_row<T>(a.k, b, j, hk), *const vrow = band_row<T>(a.v, b, j, hk);
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
+    for (int c = 0; c < C; ++c) {
         if (key_on) {
             kf[c] = band_load8<MODE>(krow, 16 * c + 8 * hh, a.D);
             vf[c] = band_load8<MODE>(vrow, 16 * c + 8 * hh, a.D);
@@ -80,36 +91,36 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) dk[db] = dv[db] = band_zero();
 
-    const int steps = n_tiles * a.G;  // tiles of the first head, of the second, ...
-    using Stage = BandStage<T, DP, MODE>;
     Stage qs, gs;
     float st = 0.f;
-    if (MODE == 1 && a.D < DP) {
+    if (MODE == 1 && !Stage::DIRECT && a.D < DP) {
         Stage::clear(lds, NB * 2 * BAND_TILE, a.D);
         __syncthreads();
     }
-    auto fetch = [&](int step) {
-        const int g = step / n_tiles, i0 = (first + step - g * n_tiles) * BAND_TILE, h = hk * a.G + g;
-        T *const Q = lds + (NB == 2 ? (step & 1) : 0) * 2 * ELEMS;
+    qs.init(a.q.s.l, a.D);
+    gs.init(a.dout.s.l, a.D);
+    auto fetch = [&](int tile, int h, T *image) {
+        const int i0 = tile * BAND_TILE;
         if (threadIdx.x < 2 * BAND_TILE) {
             const int i = i0 + (threadIdx.x & (BAND_TILE - 1));
-            const float *src = (threadIdx.x < BAND_TILE ? a.lse : a.delta) + ((size_t)b * a.Hq + h) * a.Lq;
-            st = i < sq.qn ? src[i] : threadIdx.x < BAND_TILE ? INFINITY : 0.f;
+            const bool of_lse = threadIdx.x < BAND_TILE;
+            const float *src = (of_lse ? a.lse : a.delta) + ((size_t)b * a.Hq + h) * a.Lq;
+            const float v = src[min(i, sq.qn - 1)];
+            st = of_lse ? (i < sq.qn ? -v : -INFINITY) : v;
         }
-        qs.init(band_row<T>(a.q, b, 0, h), a.q.s.l);
-        gs.init(band_row<T>(a.dout, b, 0, h), a.dout.s.l);
-        qs.fetch(i0, sq.qn, a.D, Q);
-        gs.fetch(i0, sq.qn, a.D, Q + ELEMS);
+        qs.fetch(reinterpret_cast<const char *>(band_row<T>(a.q, b, i0, h)), sq.qn - 1 - i0, a.D, image);
+        gs.fetch(reinterpret_cast<const char *>(band_row<T>(a.dout, b, i0, h)), sq.qn - 1 - i0, a.D, image + ELEMS);
     };
-    if (steps) fetch(0);
-    for (int step = 0; step < steps; ++step) {
-        T *const Q = lds + (NB == 2 ? (step & 1) : 0) * 2 * ELEMS, *const G = Q + ELEMS;
-        float *const S = stats + (NB == 2 ? (step & 1) : 0) * 2 * BAND_TILE;
-        const int g = step / n_tiles, i0 = (first + step - g * n_tiles) * BAND_TILE;
+    int g = n_tiles ? begin / n_tiles : 0, tile = first + begin - g * n_tiles;
+    if (begin < end) fetch(tile, hk * a.G + g, lds);
+    bool new_head = true;
+    for (int step = begin; step < end; ++step) {
+        T *const Q = lds + (NB == 2 ? ((step - begin) & 1) : 0) * 2 * ELEMS, *const G = Q + ELEMS;
+        float *const S = stats + (NB == 2 ? ((step - begin) & 1) : 0) * 2 * BAND_TILE;
         if constexpr (NB == 1) lds_barrier();
         if constexpr (BIAS) {
-            if (step == g * n_tiles) {  // another head's bias
-                lds_barrier();          // the last head's readers are done
+            if (new_head) {
+                lds_barrier();  // the last head's readers are done
                 band_stage_bias(a, hk * a.G + g, -1, bias, 256);
             }
         }
@@ -121,7 +132,11 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
         }
         if (threadIdx.x < 2 * BAND_TILE) S[threadIdx.x] = st;
         if constexpr (Stage::DIRECT) lds_barrier();
-        if (step + 1 < steps) fetch(step + 1);
+        const int i0 = tile * BAND_TILE;
+        new_head = tile + 1 == first + n_tiles;
+        tile = new_head ? first : tile + 1;
+        g += new_head;
+        if (step + 1 < end) fetch(tile, hk * a.G + g, lds + (NB == 2 ? ((step + 1 - begin) & 1) : 0) * 2 * ELEMS);
         if constexpr (!Stage::DIRECT) lds_barrier();
 #pragma unroll 1
         for (int u = 0; u < 2; ++u) {
@@ -129,37 +144,57 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
             if (r0 >= sq.qn || j_lo >= sq.kn || j_lo > p_hi + a.right || (j_hi < p_lo - a.left && j_lo >= a.sinks)) continue;
             const bool full = j_hi < sq.kn && j_hi <= p_lo + a.right && (j_lo >= p_hi - a.left || j_hi < a.sinks);
             f32x16 s = band_zero(), dp = band_zero();
+            float nl[16], del[16];
+            {
+                typename band_t<T>::frag qf[C], gf[C];
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) s = band_mma(band_rows<DP>(Q, 32 * u + l31, c, hh), kf[c], s);
+                for (int c = 0; c < C; ++c) {
+                    qf[c] = band_rows<DP>(Q, 32 * u + l31, c, hh);
+                    gf[c] = band_rows<DP>(G, 32 * u + l31, c, hh);
+                }
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) dp = band_mma(band_rows<DP>(G, 32 * u + l31, c, hh), vf[c], dp);
-            float bu = 0.f;
-            bool near = false;
-            if constexpr (BIAS) {
-                near = j_lo - p_hi < a.M && j_hi - p_lo > -a.M;
-                if (!near) bu = bias[j_lo > p_hi ? 0 : 2 * (a.M + BAND_MARGIN)];
-            }
-            const float *br = bias + (p_lo + 4 * hh - j + a.M + BAND_MARGIN);
-            // the mask from the key's side: position p sees key j when p >= j - right and (p <= j + left or j < sinks)
-            const int p_min = key_on ? j - a.right - p_lo - 4 * hh : BAND_FAR, p_max = j < a.sinks ? BAND_FAR : j + a.left - p_lo - 4 * hh;
+                for (int k = 0; k < 4; ++k) {
+                    *reinterpret_cast<float4 *>(nl + 4 * k) = *reinterpret_cast<const float4 *>(S + 32 * u + 8 * k + 4 * hh);
+                    *reinterpret_cast<float4 *>(del + 4 * k) = *reinterpret_cast<const float4 *>(S + BAND_TILE + 32 * u + 8 * k + 4 * hh);
+                }
+                if (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float4 ls = *reinterpret_cast<const float4 *>(S + 32 * u + 8 * k + 4 * hh);
-                const float4 de = *reinterpret_cast<const float4 *>(S + BAND_TILE + 32 * u + 8 * k + 4 * hh);
-                const float lse[4] = {ls.x, ls.y, ls.z, ls.w}, del[4] = {de.x, de.y, de.z, de.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 4 * k + e;
-                    float add = bu;
-                    if constexpr (BIAS) {
-                        if (near) add = br[rho(r)];
-                    }
-                    float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, add - lse[e]));
-                    if (!full) pr = (int)(rho(r) >= p_min) & (int)(rho(r) <= p_max) ? pr : 0.f;
-                    s[r] = pr;
-                    dp[r] = pr == 0.f ? 0.f : pr * (dp[r] - del[e]);
+                for (int c = 0; c < C; ++c) {
+                    s = band_mma(qf[c], kf[c], s);
+                    dp = band_mma(gf[c], vf[c], dp);
                 }
             }
+            typename band_t<T>::frag gc[2][DP / 32], qc[2][DP / 32];
+            if (AHEAD) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) {
+                        gc[k][db] = band_cols<DP>(G, 32 * u + 16 * k, db, lane);
+                        qc[k][db] = band_cols<DP>(Q, 32 * u + 16 * k, db, lane);
+                    }
+            }
+            if constexpr (BIAS) {
+                if (j_lo - p_hi < a.M && j_hi - p_lo > -a.M) {
+                    const float *br = bias + (p_lo + 4 * hh - j + a.M + BAND_MARGIN);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) nl[r] += br[rho(r)];
+                } else {
+                    const float bu = bias[j_lo > p_hi ? 0 : 2 * (a.M + BAND_MARGIN)];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) nl[r] += bu;
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, nl[r]));
+            if (!full) {
+                // the mask from the key's side: position p sees key j when p >= j - right and (p <= j + left or j < sinks)
+                const int p_min = key_on ? j - a.right - p_lo - 4 * hh : BAND_FAR, p_max = j < a.sinks ? BAND_FAR : j + a.left - p_lo - 4 * hh;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = (int)(rho(r) >= p_min) & (int)(rho(r) <= p_max) ? s[r] : 0.f;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] = s[r] * (dp[r] - del[r]);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 typename band_t<T>::frag pf, sf;
@@ -167,60 +202,111 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
                 band_pack(dp, k, sf);
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db) {
-                    dv[db] = band_mma(band_cols<DP>(G, 32 * u + 16 * k, db, lane), pf, dv[db]);
-                    dk[db] = band_mma(band_cols<DP>(Q, 32 * u + 16 * k, db, lane), sf, dk[db]);
+                    if (!AHEAD) {
+                        gc[k][db] = band_cols<DP>(G, 32 * u + 16 * k, db, lane);
+                        qc[k][db] = band_cols<DP>(Q, 32 * u + 16 * k, db, lane);
+                    }
+                    dv[db] = band_mma(gc[k][db], pf, dv[db]);
+                    dk[db] = band_mma(qc[k][db], sf, dk[db]);
                 }
             }
         }
     }
     // (keys behind the sequence: their P and dS are zero, and so are these rows)
-    const bool store = j < a.Lk;
-    band_store_row<T, DP, MODE>(const_cast<T *>(band_row<T>(a.dk, b, j, hk)), dk, a.scale, a.D, hh, store);
-    band_store_row<T, DP, MODE>(const_cast<T *>(band_row<T>(a.dv, b, j, hk)), dv, 1.f, a.D, hh, store);
+    if (nc == 1) {
+        const bool store = j < a.Lk;
+        band_store_row<T, DP, MODE>(const_cast<T *>(band_row<T>(a.dk, b, j, hk)), dk, a.scale, a.D, hh, store);
+        band_store_row<T, DP, MODE>(const_cast<T *>(band_row<T>(a.dv, b, j, hk)), dv, 1.f, a.D, hh, store);
+    } else {
+        const int per = a.chunks > 1 ? units : a.sink_blocks * a.sink_chunks;  // shares of one (sequence, key head)
+        float *const at = a.shares + (((size_t)bh * per + unit) * 2 * BAND_ROWS + 32 * wave + l31) * a.D;
+        // (fp32 rows of D: 16-byte pieces fit where D is a multiple of 4, as in mode 0)
+        band_store_row<float, DP, MODE>(at, dk, 1.f, a.D, hh, true);
+        band_store_row<float, DP, MODE>(at + (size_t)BAND_ROWS * a.D, dv, 1.f, a.D, hh, true);
+    }
+}
+
+// one element of dk or dv per thread: the sum of its block's shares, in their order
+template <typename T> __global__ __launch_bounds__(256) void band_attn_join_dkv_kernel(const BandArgs a) {
+    const int nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS, n_sink = a.sink_blocks * a.sink_chunks;
+    const int blocks = a.chunks > 1 ? nkb : a.sink_blocks, per = a.chunks > 1 ? n_sink + (nkb - a.sink_blocks) * a.chunks : n_sink;
+    const int block = blockIdx.x / a.D, bh = block / blocks, kb = block - bh * blocks, hk = bh % a.Hkv, b = bh / a.Hkv;
+    const int nc = kb < a.sink_blocks ? a.sink_chunks : a.chunks;
+    const int unit = kb < a.sink_blocks ? kb * a.sink_chunks : n_sink + (kb - a.sink_blocks) * a.chunks;
+    const int size = BAND_ROWS * a.D, e = (blockIdx.x - block * a.D) * 256 + threadIdx.x;  // D workgroups per block
+    const int which = e >= size, row = (e - which * size) / a.D, d = e - which * size - row * a.D, j = kb * BAND_ROWS + row;
+    if (j >= a.Lk) return;
+    const float *src = a.shares + ((size_t)bh * per + unit) * 2 * size + e;
+    float v = 0.f;
+    for (int c = 0; c < nc; ++c) v += src[(size_t)c * 2 * size];
+    const BandTensor &t = which ? a.dv : a.dk;
+    io<T>::st(const_cast<T *>(band_row<T>(t, b, j, hk)) + d, which ? v : v * a.scale);
+}
+
+// Two workgroups a CU are wanted (one for wide heads and fp32, whose registers allow no more), of at least 8 steps; blocks of
+// sinks are cut into chunks as long as the others' ones.
+static BandChunks band_chunks(const BandArgs &a, int dtype) {
+    BandChunks c = {0, 1, 1, 0};
+    const long long nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS, heads = (long long)a.B * a.Hkv, tiles = (a.Lq + BAND_TILE - 1) / BAND_TILE;
+    if (nkb == 0 || heads == 0 || tiles == 0) return c;
+    const long long window = (long long)a.left + a.right + BAND_ROWS, reach = window >= a.Lq ? tiles : window / BAND_TILE + 2;
+    const long long normal = (reach < tiles ? reach : tiles) * a.G;  // steps of a block in the middle
+    const long long want = a.D > 64 || dtype == DSW_F32 ? 256 : 512, n = (want + heads * nkb - 1) / (heads * nkb), most = normal / 8;
+    c.chunks = (int)(n < most ? n : most);
+    if (c.chunks < 1) c.chunks = 1;
+    if (c.chunks > 64) c.chunks = 64;
+    const long long sink_blocks = a.sinks > 0 && normal < tiles * a.G ? (a.sinks + BAND_ROWS - 1) / BAND_ROWS : 0;
+    c.sink_blocks = (int)(sink_blocks < nkb ? sink_blocks : nkb);
+    const long long len = (normal + c.chunks - 1) / c.chunks, k = (tiles * a.G + len - 1) / len;
+    c.sink_chunks = c.sink_blocks ? (int)(k < 1024 ? k : 1024) : 1;
+    c.shares = heads * ((c.sink_chunks > 1 ? (long long)c.sink_blocks * c.sink_chunks : 0));
+    if (c.chunks > 1) c.shares = heads * ((long long)c.sink_blocks * c.sink_chunks + (nkb - c.sink_blocks) * c.chunks);
+    return c;
 }
 
 // ---- dq: 128 rows of a workgroup, 32 per wave; bias gradient by distance ---------------------------------------------
 template <typename T, int DP, int MODE, bool BIAS, bool DTABLE>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void band_attn_dq_kernel(const BandArgs a) {
-    constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE);
+    constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE), C = DP / 16;
+    constexpr bool AHEAD = DP < 128 && sizeof(T) == 2;  // registers for LDS reads well ahead of the products that need them
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     T *const lds = reinterpret_cast<T *>(smem);  // [NB][K | V]
     float *const bias = reinterpret_cast<float *>(lds + NB * 2 * ELEMS);
     const int BL = 2 * (a.M + BAND_MARGIN) + 1;
     float *const sums = bias + BL;  // [4 waves][2 lane halves][BL]: dS by distance
 
-    const int nqb = (a.Lq + BAND_ROWS - 1) / BAND_ROWS;
-    const int idx = xcd_remap(blockIdx.x, gridDim.x);
-    const int g = idx % a.G, rest = idx / a.G;
-    const int qb = nqb - 1 - rest % nqb, bh = rest / nqb;
-    const int hk = bh % a.Hkv, b = bh / a.Hkv, h = hk * a.G + g;
     const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const BandSeq sq = band_seq(a, b);
-    const int i_lo = qb * BAND_ROWS, i0 = i_lo + 32 * wave, i = i0 + l31;
-    const bool row_on = i < sq.qn, wave_on = i0 < sq.qn;
-    const int p = sq.off + i, w_lo = sq.off + i0, w_hi = sq.off + min(i0 + 31, sq.qn - 1);
-    const BandTiles tiles = band_tiles<BAND_TILE>(a, sq.kn, sq.off + i_lo, sq.off + min(i_lo + BAND_ROWS, sq.qn) - 1);
+    const BandPlace at(a, blockIdx.x, gridDim.x);
+    const BandSeq &sq = at.sq;
+    const BandTiles &tiles = at.tiles;
+    const int b = at.b, h = at.h, i = at.i;
+    const bool row_on = i < sq.qn;
+    const int p = sq.off + i, w_lo = sq.off + at.i0, w_hi = sq.off + min(at.i0 + 31, sq.qn - 1);
+    BandEdges<32> edges;
+    edges.init(a, sq.kn, w_lo, w_hi, at.i0 < sq.qn);
+    const int key_hi = min(sq.kn - 1, p + a.right), key_lo = p - a.left;
+    const float scale = a.c;
+    const int D = a.D, M = a.M;
 
-    const T *const kbase = band_row<T>(a.k, b, 0, hk), *const vbase = band_row<T>(a.v, b, 0, hk);
     if constexpr (BIAS) band_stage_bias(a, h, 1, bias, 256);
     if constexpr (DTABLE) {
         for (int e = threadIdx.x; e < 8 * BL; e += 256) sums[e] = 0.f;
     }
-    typename band_t<T>::frag qf[DP / 16], gf[DP / 16];
+    typename band_t<T>::frag qf[C], gf[C];
     const T *const qrow = band_row<T>(a.q, b, i, h), *const grow = band_row<T>(a.dout, b, i, h);
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
+    for (int c = 0; c < C; ++c) {
         if (row_on) {
-            qf[c] = band_load8<MODE>(qrow, 16 * c + 8 * hh, a.D);
-            gf[c] = band_load8<MODE>(grow, 16 * c + 8 * hh, a.D);
+            qf[c] = band_load8<MODE>(qrow, 16 * c + 8 * hh, D);
+            gf[c] = band_load8<MODE>(grow, 16 * c + 8 * hh, D);
         } else {
             band_clear(qf[c]);
             band_clear(gf[c]);
         }
     }
-    const size_t at = ((size_t)b * a.Hq + h) * a.Lq + i;
-    const float lse = row_on ? a.lse[at] : INFINITY, del = row_on ? a.delta[at] : 0.f;
+    const size_t stat = ((size_t)b * a.Hq + h) * a.Lq + i;
+    const float nl = row_on ? -a.lse[stat] : -INFINITY, del = row_on ? a.delta[stat] : 0.f;
     f32x16 dq[DP / 32];
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) dq[db] = band_zero();
@@ -228,15 +314,19 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
 
     using Stage = BandStage<T, DP, MODE>;
     Stage ks, vs;
-    ks.init(kbase, a.k.s.l);
-    vs.init(vbase, a.v.s.l);
-    if (MODE == 1 && a.D < DP) {
-        Stage::clear(lds, NB * 2 * BAND_TILE, a.D);
+    ks.init(a.k.s.l, D);
+    vs.init(a.v.s.l, D);
+    if (MODE == 1 && !Stage::DIRECT && D < DP) {
+        Stage::clear(lds, NB * 2 * BAND_TILE, D);
         __syncthreads();
     }
+    BandWalk kw, vw;
+    kw.init(band_row<T>(a.k, b, 0, at.hk), ks.ld, BAND_TILE, tiles);
+    vw.init(band_row<T>(a.v, b, 0, at.hk), vs.ld, BAND_TILE, tiles);
+    int jt = tiles.n_sink ? 0 : tiles.first * BAND_TILE;
     if (tiles.count) {
-        ks.fetch(tiles.at(0) * BAND_TILE, sq.kn, a.D, lds);
-        vs.fetch(tiles.at(0) * BAND_TILE, sq.kn, a.D, lds + ELEMS);
+        ks.fetch(kw.p, sq.kn - 1 - jt, D, lds);
+        vs.fetch(vw.p, sq.kn - 1 - jt, D, lds + ELEMS);
     }
     for (int it = 0; it < tiles.count; ++it) {
         T *const K = lds + (NB == 2 ? (it & 1) : 0) * 2 * ELEMS, *const V = K + ELEMS;
@@ -245,43 +335,72 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
             lds_barrier();
         } else {
             if constexpr (NB == 1) lds_barrier();
-            ks.put(K, a.D);
-            vs.put(V, a.D);
+            ks.put(K, D);
+            vs.put(V, D);
         }
+        const int tile = jt;
+        jt = it + 1 == tiles.n_sink ? tiles.first * BAND_TILE : jt + BAND_TILE;
         if (it + 1 < tiles.count) {
             T *const K1 = lds + (NB == 2 ? ((it + 1) & 1) : 0) * 2 * ELEMS;
-            ks.fetch(tiles.at(it + 1) * BAND_TILE, sq.kn, a.D, K1);
-            vs.fetch(tiles.at(it + 1) * BAND_TILE, sq.kn, a.D, K1 + ELEMS);
+            kw.next(it + 1, tiles);
+            vw.next(it + 1, tiles);
+            ks.fetch(kw.p, sq.kn - 1 - jt, D, K1);
+            vs.fetch(vw.p, sq.kn - 1 - jt, D, K1 + ELEMS);
         }
         if constexpr (!Stage::DIRECT) lds_barrier();
 #pragma unroll 1
         for (int u = 0; u < 2; ++u) {
-            const int j0 = tiles.at(it) * BAND_TILE + 32 * u, j9 = j0 + 31;
-            if (!wave_on || j0 >= sq.kn || j0 > w_hi + a.right || (j9 < w_lo - a.left && j0 >= a.sinks)) continue;
-            const bool full = j9 < sq.kn && j9 <= w_lo + a.right && (j0 >= w_hi - a.left || j9 < a.sinks);
+            const int j0 = tile + 32 * u;
+            if (edges.none(j0)) continue;
             f32x16 s = band_zero(), dp = band_zero();
+            {
+                typename band_t<T>::frag kf[C], vf[C];
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) s = band_mma(band_rows<DP>(K, 32 * u + l31, c, hh), qf[c], s);
-#pragma unroll
-            for (int c = 0; c < DP / 16; ++c) dp = band_mma(band_rows<DP>(V, 32 * u + l31, c, hh), gf[c], dp);
-            float bu = 0.f;
-            bool near = false;
-            if constexpr (BIAS) {
-                near = j9 - w_lo > -a.M && j0 - w_hi < a.M;
-                if (!near) bu = bias[j0 > w_hi ? BL - 1 : 0];
-            }
-            const int e0 = j0 + 4 * hh - p + a.M + BAND_MARGIN;
-            const BandMask mask = band_row_mask(a, p, sq.kn, j0 + 4 * hh);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float add = bu;
-                if constexpr (BIAS) {
-                    if (near) add = bias[e0 + rho(r)];
+                for (int c = 0; c < C; ++c) {
+                    kf[c] = band_rows<DP>(K, 32 * u + l31, c, hh);
+                    vf[c] = band_rows<DP>(V, 32 * u + l31, c, hh);
                 }
-                float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, add - lse));
-                if (!full) pr = mask.sees(rho(r)) ? pr : 0.f;
-                s[r] = pr == 0.f ? 0.f : pr * (dp[r] - del);
+                if (AHEAD) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    s = band_mma(kf[c], qf[c], s);
+                    dp = band_mma(vf[c], gf[c], dp);
+                }
             }
+            typename band_t<T>::frag kc[2][DP / 32];
+            if (AHEAD) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) kc[k][db] = band_cols<DP>(K, 32 * u + 16 * k, db, lane);
+            }
+            float cs = scale, shift = nl;
+            bool near = false;
+            const int e0 = j0 + 4 * hh - p + M + BAND_MARGIN;
+            if constexpr (BIAS) {
+                near = j0 + 31 - w_lo > -M && j0 - w_hi < M;
+                if (near) {
+                    cs = 1.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], scale, bias[e0 + rho(r)]);
+                } else {
+                    shift += bias[j0 > w_hi ? BL - 1 : 0];
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], cs, shift));
+            if (edges.cut_hi(j0)) {
+                const int hi = key_hi - j0 - 4 * hh;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = rho(r) <= hi ? s[r] : 0.f;
+            }
+            if (edges.cut_lo(j0)) {
+                const int lo = key_lo - j0 - 4 * hh, first = edges.sinks - j0 - 4 * hh;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = (int)(rho(r) >= lo) | (int)(rho(r) < first) ? s[r] : 0.f;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] *= dp[r] - del;
             if constexpr (DTABLE) {
                 // the 32 lanes of a half hold one key each time: 32 different distances, in a table that only this wave's
                 // half adds to, one instruction after the other - the order of the sums is fixed
@@ -303,7 +422,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
                 typename band_t<T>::frag sf;
                 band_pack(s, k, sf);
 #pragma unroll
-                for (int db = 0; db < DP / 32; ++db) dq[db] = band_mma(band_cols<DP>(K, 32 * u + 16 * k, db, lane), sf, dq[db]);
+                for (int db = 0; db < DP / 32; ++db) {
+                    if (!AHEAD) kc[k][db] = band_cols<DP>(K, 32 * u + 16 * k, db, lane);
+                    dq[db] = band_mma(kc[k][db], sf, dq[db]);
+                }
             }
         }
     }
@@ -328,7 +450,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
         }
         __syncthreads();
         const int n = 2 * a.M + 1;
-        float *const dst = a.partial + ((size_t)h * a.B * nqb + (size_t)b * nqb + qb) * n;
+        const int nqb = (a.Lq + BAND_ROWS - 1) / BAND_ROWS;
+        float *const dst = a.partial + ((size_t)h * a.B * nqb + (size_t)b * nqb + at.i_lo / BAND_ROWS) * n;
         for (int e = threadIdx.x; e < n; e += 256) {
             float v = 0.f;
 #pragma unroll
@@ -369,8 +492,15 @@ template <typename T, int DP, int MODE, bool BIAS, bool DTABLE> static int launc
         const size_t lds = images + (size_t)band_t<T>::nbuf(DP) * 2 * BAND_TILE * sizeof(float) + bl;
         auto kern = band_attn_dkv_kernel<T, DP, MODE, BIAS>;
         if (int rc = allow_lds(kern, lds)) return rc;
-        kern<<<dim3((unsigned)((long long)a.B * a.Hkv * ((a.Lk + BAND_ROWS - 1) / BAND_ROWS))), 256, lds, st>>>(a);
+        const long long nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS, heads = (long long)a.B * a.Hkv;
+        kern<<<dim3((unsigned)(heads * (a.sink_blocks * a.sink_chunks + (nkb - a.sink_blocks) * a.chunks))), 256, lds, st>>>(a);
         if (int rc = check_launch("dsw_band_attn_bwd (dk, dv)")) return rc;
+        const long long joined = heads * (a.chunks > 1 ? nkb : a.sink_chunks > 1 ? a.sink_blocks : 0);
+        if (joined) {
+            if (joined * a.D >= (1LL << 31)) return fail(DSW_EUNSUPPORTED, "dsw_band_attn_bwd: %lld shared key blocks", joined);
+            band_attn_join_dkv_kernel<T><<<dim3((unsigned)(joined * a.D)), 256, 0, st>>>(a);  // (2 * 128 * D elements per block)
+            if (int rc = check_launch("dsw_band_attn_bwd (join)")) return rc;
+        }
     }
     if (a.Lq) {
         const size_t lds = images + bl + (DTABLE ? 8 * bl : 0);
@@ -392,6 +522,7 @@ extern "C" size_t dsw_band_attn_bwd_workspace(const dsw_band_desc *d) {
     BandArgs a;
     if (band_make_args("dsw_band_attn_bwd_workspace", d, a)) return 0;
     size_t n = round16((size_t)a.B * a.Hq * a.Lq);
+    n += (size_t)band_chunks(a, d->dtype).shares * 2 * BAND_ROWS * a.D;
     if (a.table) n += (size_t)a.Hq * ((size_t)a.B * ((a.Lq + BAND_ROWS - 1) / BAND_ROWS) + 1) * (2 * a.M + 1);
     return n * sizeof(float);
 }
@@ -420,7 +551,10 @@ extern "C" int dsw_band_attn_bwd(const dsw_band_desc *d, const void *q, const ds
     a.lse = const_cast<float *>(lse);
     a.out32 = const_cast<float *>(out32);
     a.delta = static_cast<float *>(workspace);
-    a.partial = a.delta + round16((size_t)a.B * a.Hq * a.Lq);
+    const BandChunks chunks = band_chunks(a, d->dtype);
+    a.sink_blocks = chunks.sink_blocks, a.sink_chunks = chunks.sink_chunks, a.chunks = chunks.chunks;
+    a.shares = a.delta + round16((size_t)a.B * a.Hq * a.Lq);
+    a.partial = a.shares + (size_t)chunks.shares * 2 * BAND_ROWS * a.D;
     hipStream_t st = as_stream(stream);
     if (!no_rows) {
         const long long rows = (long long)a.B * a.Lq * a.Hq;

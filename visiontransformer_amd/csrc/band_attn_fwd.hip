@@ -11,177 +11,219 @@
 namespace dsw {
 
 template <typename T, int DP, int MODE, bool BIAS, bool EXACT>
-__global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void band_attn_fwd_kernel(const BandArgs a) {
-    constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE);
+__global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof(T) == 4 || EXACT ? 2 : 3)) void band_attn_fwd_kernel(const BandArgs a_) {
+    constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE), C = DP / 16;
+    using Stage = BandStage<T, DP, MODE>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     T *const lds = reinterpret_cast<T *>(smem);  // [NB][K | V]
     float *const bias = reinterpret_cast<float *>(lds + NB * 2 * ELEMS);
-
-    const int nqb = (a.Lq + BAND_ROWS - 1) / BAND_ROWS;
-    const int idx = xcd_remap(blockIdx.x, gridDim.x);
-    const int g = idx % a.G, rest = idx / a.G;
-    const int qb = nqb - 1 - rest % nqb, bh = rest / nqb;  // (the last rows of a causal call have the most to do: first)
-    const int hk = bh % a.Hkv, b = bh / a.Hkv, h = hk * a.G + g;
     const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const BandSeq sq = band_seq(a, b);
-    const int i_lo = qb * BAND_ROWS, i0 = i_lo + 32 * wave, i = i0 + l31;
-    const bool row_on = i < sq.qn, wave_on = i0 < sq.qn;
-    const int p = sq.off + i, w_lo = sq.off + i0, w_hi = sq.off + min(i0 + 31, sq.qn - 1);
-    const BandTiles tiles = band_tiles<BAND_TILE>(a, sq.kn, sq.off + i_lo, sq.off + min(i_lo + BAND_ROWS, sq.qn) - 1);
 
-    const T *const qrow = band_row<T>(a.q, b, i, h);
-    const T *const kbase = band_row<T>(a.k, b, 0, hk);
-    const T *const vbase = band_row<T>(a.v, b, 0, hk);
-    if constexpr (BIAS) band_stage_bias(a, h, 1, bias, 256);
-
-    typename band_t<T>::frag qf[DP / 16];
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
-        if (row_on) qf[c] = band_load8<MODE>(qrow, 16 * c + 8 * hh, a.D);
-        else band_clear(qf[c]);
-    }
     f32x16 o[DP / 32];
     float m, l;
+    bool safe = false, spoiled;
+    {
+        const BandArgs &a = a_;
+        const BandPlace at(a, blockIdx.x, gridDim.x);
+        const BandSeq &sq = at.sq;
+        const BandTiles &tiles = at.tiles;
+        const bool row_on = at.i < sq.qn;
+        const int p = sq.off + at.i, w_lo = sq.off + at.i0, w_hi = sq.off + min(at.i0 + 31, sq.qn - 1);
+        BandEdges<BAND_TILE> edges;
+        edges.init(a, sq.kn, w_lo, w_hi, at.i0 < sq.qn);
+        const int key_hi = min(sq.kn - 1, p + a.right), key_lo = p - a.left;
+        const float scale = a.c;
+        const int D = a.D, M = a.M;
+        if constexpr (BIAS) band_stage_bias(a, at.h, 1, bias, 256);
 
-    BandStage<T, DP, MODE> ks, vs;
-    ks.init(kbase, a.k.s.l);
-    vs.init(vbase, a.v.s.l);
-    if (MODE == 1 && a.D < DP) {
-        BandStage<T, DP, MODE>::clear(lds, NB * 2 * BAND_TILE, a.D);
-        __syncthreads();
-    }
-    bool safe = false;
-    for (;;) {
-        m = -INFINITY;
-        l = 0.f;
+        typename band_t<T>::frag qf[C];
+        const T *const qrow = band_row<T>(a.q, at.b, at.i, at.h);
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) o[db] = band_zero();
-        bool fresh = true;  // some row has no reference yet
-        if (tiles.count) {
-            ks.fetch(tiles.at(0) * BAND_TILE, sq.kn, a.D, lds);
-            vs.fetch(tiles.at(0) * BAND_TILE, sq.kn, a.D, lds + ELEMS);
+        for (int c = 0; c < C; ++c) {
+            if (row_on) qf[c] = band_load8<MODE>(qrow, 16 * c + 8 * hh, D);
+            else band_clear(qf[c]);
         }
-        for (int it = 0; it < tiles.count; ++it) {
-            T *const K = lds + (NB == 2 ? (it & 1) : 0) * 2 * ELEMS, *const V = K + ELEMS;
-            if constexpr (!BandStage<T, DP, MODE>::DIRECT) {
-                if constexpr (NB == 1) lds_barrier();
-                ks.put(K, a.D);
-                vs.put(V, a.D);
-            } else {
-                band_landed();
-                lds_barrier();
-            }
-            if (it + 1 < tiles.count) {
-                T *const K1 = lds + (NB == 2 ? ((it + 1) & 1) : 0) * 2 * ELEMS;
-                ks.fetch(tiles.at(it + 1) * BAND_TILE, sq.kn, a.D, K1);
-                vs.fetch(tiles.at(it + 1) * BAND_TILE, sq.kn, a.D, K1 + ELEMS);
-            }
-            if constexpr (!BandStage<T, DP, MODE>::DIRECT) lds_barrier();
-            const int j0 = tiles.at(it) * BAND_TILE, j9 = j0 + BAND_TILE - 1;
-            if (!wave_on || j0 > w_hi + a.right || (j9 < w_lo - a.left && j0 >= a.sinks)) continue;
-            const bool full = j9 < sq.kn && j9 <= w_lo + a.right && (j0 >= w_hi - a.left || j9 < a.sinks);
-            f32x16 s[2];
+        Stage ks, vs;
+        ks.init(a.k.s.l, D);
+        vs.init(a.v.s.l, D);
+        if (MODE == 1 && !Stage::DIRECT && D < DP) {
+            Stage::clear(lds, NB * 2 * BAND_TILE, D);
+            __syncthreads();
+        }
+        const T *const kbase = band_row<T>(a.k, at.b, 0, at.hk), *const vbase = band_row<T>(a.v, at.b, 0, at.hk);
+        for (;;) {
+            m = -INFINITY;
+            l = 0.f;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                s[u] = band_zero();
-#pragma unroll
-                for (int c = 0; c < DP / 16; ++c) s[u] = band_mma(band_rows<DP>(K, 32 * u + l31, c, hh), qf[c], s[u]);
+            for (int db = 0; db < DP / 32; ++db) o[db] = band_zero();
+            bool fresh = true;  // some row has no reference yet
+            BandWalk kw, vw;
+            kw.init(kbase, ks.ld, BAND_TILE, tiles);
+            vw.init(vbase, vs.ld, BAND_TILE, tiles);
+            int j0 = tiles.n_sink ? 0 : tiles.first * BAND_TILE;
+            if (tiles.count) {
+                ks.fetch(kw.p, sq.kn - 1 - j0, D, lds);
+                vs.fetch(vw.p, sq.kn - 1 - j0, D, lds + ELEMS);
             }
-            float cs = a.c, bu = 0.f;  // the logits are cs * s + bu
-            if constexpr (BIAS) {
-                if (j9 - w_lo > -a.M && j0 - w_hi < a.M) {
-                    const float *br = bias + (j0 + 4 * hh - p + a.M + BAND_MARGIN);
-                    cs = 1.f;
+            for (int it = 0; it < tiles.count; ++it) {
+                T *const K = lds + (NB == 2 ? (it & 1) : 0) * 2 * ELEMS, *const V = K + ELEMS;
+                if constexpr (Stage::DIRECT) {
+                    band_landed();
+                    lds_barrier();
+                } else {
+                    if constexpr (NB == 1) lds_barrier();
+                    ks.put(K, D);
+                    vs.put(V, D);
+                }
+                const int j1 = it + 1 == tiles.n_sink ? tiles.first * BAND_TILE : j0 + BAND_TILE;
+                if (it + 1 < tiles.count) {
+                    T *const K1 = lds + (NB == 2 ? ((it + 1) & 1) : 0) * 2 * ELEMS;
+                    kw.next(it + 1, tiles);
+                    vw.next(it + 1, tiles);
+                    ks.fetch(kw.p, sq.kn - 1 - j1, D, K1);
+                    vs.fetch(vw.p, sq.kn - 1 - j1, D, K1 + ELEMS);
+                }
+                if constexpr (!Stage::DIRECT) lds_barrier();
+                const int j = j0;
+                j0 = j1;
+                if (edges.none(j)) continue;
+
+                // LDS reads are issued well ahead of the products that need them (left alone, each comes right in front of its product)
+                f32x16 s[2];
+                {
+                    typename band_t<T>::frag kf[2][C];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                        for (int c = 0; c < C; ++c) kf[u][c] = band_rows<DP>(K, 32 * u + l31, c, hh);
+                        if (DP == 128 || u == 1) __builtin_amdgcn_sched_barrier(0);
+                        if (DP == 128) {
+                            s[u] = band_zero();
+#pragma unroll
+                            for (int c = 0; c < C; ++c) s[u] = band_mma(kf[u][c], qf[c], s[u]);
+                        }
+                    }
+                    if (DP < 128) {
+                        s[0] = s[1] = band_zero();
+#pragma unroll
+                        for (int c = 0; c < C; ++c)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) s[u] = band_mma(kf[u][c], qf[c], s[u]);
+                    }
+                }
+                float cs = scale, bu = 0.f;  // the logits are cs * s + bu
+                if constexpr (BIAS) {
+                    if (j + BAND_TILE - 1 - w_lo > -M && j - w_hi < M) {
+                        const float *br = bias + (j + 4 * hh - p + M + BAND_MARGIN);
+                        cs = 1.f;
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[u][r] = __builtin_fmaf(s[u][r], scale, br[32 * u + rho(r)]);
+                    } else {
+                        bu = bias[j > w_hi ? 2 * (M + BAND_MARGIN) : 0];  // (all distances clipped: one bias)
+                    }
+                }
+                if (edges.cut_hi(j)) {
+                    const int hi = key_hi - j - 4 * hh;
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[u][r] = __builtin_fmaf(s[u][r], a.c, br[32 * u + rho(r)]);
-                } else {
-                    bu = bias[j0 > w_hi ? 2 * (a.M + BAND_MARGIN) : 0];  // (all distances clipped: one bias)
+                        for (int r = 0; r < 16; ++r) s[u][r] = 32 * u + rho(r) <= hi ? s[u][r] : -INFINITY;
+                }
+                if (edges.cut_lo(j)) {
+                    const int lo = key_lo - j - 4 * hh, first = edges.sinks - j - 4 * hh;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            s[u][r] = (int)(32 * u + rho(r) >= lo) | (int)(32 * u + rho(r) < first) ? s[u][r] : -INFINITY;
+                }
+                if (fresh || safe) {
+                    float x = s[0][0];
+#pragma unroll
+                    for (int r = 1; r < 32; ++r) x = fmaxf(x, s[r >> 4][r & 15]);
+                    x = max_across_halves(__builtin_fmaf(x, cs, bu));
+                    const float mn = m == -INFINITY || safe ? fmaxf(m, x) : m;
+                    const float alpha = mn == m || m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                    m = mn;
+                    l *= alpha;
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+                    fresh = __any((int)row_on & (int)(m == -INFINITY));
+                }
+                const float shift = bu - (m == -INFINITY ? 0.f : m);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    typename band_t<T>::frag vf[2][DP / 32];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int db = 0; db < DP / 32; ++db) vf[k][db] = band_cols<DP>(V, 32 * u + 16 * k, db, lane);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], cs, shift));
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        typename band_t<T>::frag pf, rf;
+                        band_pack(s[u], k, pf);
+                        l = band_sum(pf, l);
+                        if constexpr (EXACT) {
+                            band_pack_rest(s[u], k, pf, rf);
+                            l = band_sum(rf, l);
+                        }
+#pragma unroll
+                        for (int db = 0; db < DP / 32; ++db) {
+                            o[db] = band_mma(vf[k][db], pf, o[db]);
+                            if constexpr (EXACT) o[db] = band_mma(vf[k][db], rf, o[db]);
+                        }
+                    }
+                }
+                if (__any(l > 0x1p60f)) {  // far above the reference: move it up
+                    const float up = l > 0x1p60f ? 0x1p-60f : 1.f, both = fminf(up, __shfl_xor(up, 32, 64));
+                    m += both < 1.f ? 60.f : 0.f;
+                    l *= both;
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[db][r] *= both;
                 }
             }
-            if (!full) {
-                const BandMask mask = band_row_mask(a, p, sq.kn, j0 + 4 * hh);
+            float bad = l * 0.f;
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+            for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[u][r] = mask.sees(32 * u + rho(r)) ? s[u][r] : -INFINITY;
-            }
-            if (fresh || safe) {
-                float x = s[0][0];
-#pragma unroll
-                for (int r = 1; r < 32; ++r) x = fmaxf(x, s[r >> 4][r & 15]);
-                x = max_across_halves(__builtin_fmaf(x, cs, bu));
-                const float mn = m == -INFINITY || safe ? fmaxf(m, x) : m;
-                const float alpha = mn == m || m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
-                l *= alpha;
-#pragma unroll
-                for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-                fresh = __any((int)row_on & (int)(m == -INFINITY));
-            }
-            const float shift = bu - (m == -INFINITY ? 0.f : m);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], cs, shift));
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    typename band_t<T>::frag pf, rf;
-                    band_pack(s[u], k, pf);
-                    l = band_sum(pf, l);
-                    if constexpr (EXACT) {
-                        band_pack_rest(s[u], k, pf, rf);
-                        l = band_sum(rf, l);
-                    }
-#pragma unroll
-                    for (int db = 0; db < DP / 32; ++db) {
-                        const auto vf = band_cols<DP>(V, 32 * u + 16 * k, db, lane);
-                        o[db] = band_mma(vf, pf, o[db]);
-                        if constexpr (EXACT) o[db] = band_mma(vf, rf, o[db]);
-                    }
-                }
-            }
-            if (__any(l > 0x1p60f)) {  // far above the reference: move it up
-                const float up = l > 0x1p60f ? 0x1p-60f : 1.f, both = fminf(up, __shfl_xor(up, 32, 64));
-                m += both < 1.f ? 60.f : 0.f;
-                l *= both;
-#pragma unroll
-                for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[db][r] *= both;
-            }
+                for (int r = 0; r < 16; ++r) bad = __builtin_fmaf(o[db][r], 0.f, bad);
+            spoiled = __any((int)row_on & (int)(bad != 0.f));
+            // a second time with the maximum over all keys so far as the reference, if anything overflowed
+            if (safe || !__syncthreads_or(spoiled)) break;
+            safe = true;
         }
-        float bad = l * 0.f;
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) bad = __builtin_fmaf(o[db][r], 0.f, bad);
-        const bool again = __syncthreads_or(row_on && bad != 0.f);
-        if (!again) break;
-        if (safe) {
-            if (__any(row_on && bad != 0.f))
-                band_careful<T, DP, BIAS, BAND_TILE>(a, qrow, kbase, vbase, h, p, row_on, sq.kn, tiles, 0, tiles.count, 1, hh, m, l, o);
-            break;
-        }
-        safe = true;
     }
 
+    auto again = __builtin_amdgcn_kernarg_segment_ptr();
+    int block = blockIdx.x;
+    asm volatile("" : "+s"(again), "+s"(block));  // (the same values, but for all the compiler knows others)
+    const BandArgs &a = *(const BandArgs *)again;
+    const BandPlace at(a, block, gridDim.x);
+    const bool row_on = at.i < at.sq.qn;
+    if (spoiled && safe)
+        band_careful<T, DP, BIAS, BAND_TILE>(a, band_row<T>(a.q, at.b, at.i, at.h), band_row<T>(a.k, at.b, 0, at.hk), band_row<T>(a.v, at.b, 0, at.hk),
+                                             at.h, at.sq.off + at.i, row_on, at.sq.kn, at.tiles, 0, at.tiles.count, 1, hh, m, l, o);
     l += __shfl_xor(l, 32, 64);
     const float inv = !row_on || l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)  // rows behind the sequence: zeros, whatever the tiles held
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[db][r] = row_on ? o[db][r] : 0.f;
-    const bool store = i < a.Lq;
-    band_store_row<T, DP, MODE>(const_cast<T *>(band_row<T>(a.out, b, i, h)), o, inv, a.D, hh, store);
+    const bool store = at.i < a.Lq;
+    band_store_row<T, DP, MODE>(const_cast<T *>(band_row<T>(a.out, at.b, at.i, at.h)), o, inv, a.D, hh, store);
     if constexpr (EXACT)  // (in mode 0 D is a multiple of 8)
-        band_store_row<float, DP, MODE>(a.out32 + (((size_t)b * a.Lq + i) * a.Hq + h) * a.D, o, inv, a.D, hh, store);
+        band_store_row<float, DP, MODE>(a.out32 + (((size_t)at.b * a.Lq + at.i) * a.Hq + at.h) * a.D, o, inv, a.D, hh, store);
     if (a.lse && store && hh == 0)
-        a.lse[((size_t)b * a.Hq + h) * a.Lq + i] = !row_on || l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+        a.lse[((size_t)at.b * a.Hq + at.h) * a.Lq + at.i] = !row_on || l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
 template <typename T, int DP, int MODE, bool BIAS, bool EXACT> static int launch_fwd(const BandArgs &a, hipStream_t st) {
@@ -202,9 +244,12 @@ int band_tensor(const char *who, const char *name, const void *p, const dsw_stri
     t.p = p;
     t.s = s ? *s : dsw_strides{0, 0, 0};
     DSW_REQUIRE(t.s.b >= 0 && t.s.l >= 0 && t.s.h >= 0, "%s: negative stride of %s", who, name);
-    const int size = dtype == DSW_F32 ? 4 : 2, wide = 16 / size;
-    const bool whole = D % wide == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && t.s.b % wide == 0 && t.s.l % wide == 0 && t.s.h % wide == 0;
-    const int m = D < 8 || t.s.l * size * BAND_TILE >= (1LL << 31) ? 2 : whole ? 0 : 1;
+    const int size = dtype == DSW_F32 ? 4 : 2;
+    auto fits = [&](int bytes) {
+        const int n = bytes / size;
+        return D % n == 0 && reinterpret_cast<uintptr_t>(p) % bytes == 0 && t.s.b % n == 0 && t.s.l % n == 0 && t.s.h % n == 0;
+    };
+    const int m = D < 8 || !fits(4) || t.s.l * size * BAND_TILE >= (1LL << 31) ? 2 : fits(16) ? 0 : 1;
     mode = m > mode ? m : mode;
     return DSW_OK;
 }
