@@ -85,6 +85,13 @@ __device__ __forceinline__ float band_sum(const band_t<float>::frag &f, float l)
     return l + (((f.lo.x + f.lo.y) + (f.lo.z + f.lo.w)) + ((f.hi.x + f.hi.y) + (f.hi.z + f.hi.w)));
 }
 
+// element e of a fragment (e known at compile time)
+__device__ __forceinline__ float band_element(const uint4 &f, int e) {
+    const uint32_t w = (&f.x)[e >> 1];
+    return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+}
+__device__ __forceinline__ float band_element(const band_t<float>::frag &f, int e) { return e < 4 ? (&f.lo.x)[e] : (&f.hi.x)[e - 4]; }
+
 __device__ __forceinline__ f32x16 band_zero() {
     f32x16 z;
 #pragma unroll
@@ -440,23 +447,24 @@ template <int SIZE> struct BandEdges {
     __device__ __forceinline__ bool cut_lo(int j0) const { return j0 < lo_ok && j0 + SIZE > sinks; }
 };
 
-// The 128 query rows of a workgroup (forward, dQ).  Made twice, before the loop and after it, from the arguments: what only
+// The query rows of a workgroup (forward, dQ).  Made twice, before the loop and after it, from the arguments: what only
 // the end needs does not have to be kept in scalar registers through the loop, which were spilled for it.
 struct BandPlace {
     int b, h, hk, i_lo, i0, i;
     BandSeq sq;
     BandTiles tiles;
-    __device__ __forceinline__ BandPlace(const BandArgs &a, int block, int blocks) {
-        const int nqb = (a.Lq + BAND_ROWS - 1) / BAND_ROWS;
+    // `rows` of a workgroup: 128, or 64 where two waves share 32
+    __device__ __forceinline__ BandPlace(const BandArgs &a, int block, int blocks, int rows = BAND_ROWS) {
+        const int nqb = (a.Lq + rows - 1) / rows;
         const int idx = xcd_remap(block, blocks);
         const int g = idx % a.G, rest = idx / a.G;
         const int qb = nqb - 1 - rest % nqb, bh = rest / nqb;  // (the last rows of a causal call have the most to do: first)
         hk = bh % a.Hkv, b = bh / a.Hkv, h = hk * a.G + g;
-        i_lo = qb * BAND_ROWS;
-        i0 = i_lo + 32 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        i_lo = qb * rows;
+        i0 = i_lo + 32 * (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & (rows / 32 - 1));
         i = i0 + (threadIdx.x & 31);
         sq = band_seq(a, b);
-        tiles = band_tiles<BAND_TILE>(a, sq.kn, sq.off + i_lo, sq.off + min(i_lo + BAND_ROWS, sq.qn) - 1);
+        tiles = band_tiles<BAND_TILE>(a, sq.kn, sq.off + i_lo, sq.off + min(i_lo + rows, sq.qn) - 1);
     }
 };
 

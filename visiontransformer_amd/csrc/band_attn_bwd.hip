@@ -4,41 +4,12 @@
 //   dq = scale dS k     dk = scale dS^T q     dv = P^T dout     dtable[b, head] = sum of dS over the pairs of bucket b
 //
 // Two kernels that each own what they write, so that no sum depends on the order in which workgroups run: one over
-// key blocks (dk, dv; the query heads that share a key head are walked one after the other and meet in the
-// accumulators), one over row blocks (dq, and the bias gradient by distance).  Both recompute the scores.  Layouts as in
+// row blocks (dq, delta, and the bias gradient by distance), then one over key blocks (dk, dv; the query heads that
+// share a key head are walked one after the other and meet in the accumulators).  Both recompute the scores.  Layouts as in
 // the forward: the 16 registers of a tile's P and dS are the second operand of the products that follow.
 #include "band_attn.hpp"
 
 namespace dsw {
-
-// ---- delta: 16 lanes a row ---------------------------------------------------------------------------------------
-template <typename T, int MODE> __global__ __launch_bounds__(256) void band_attn_delta_kernel(const BandArgs a) {
-    const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const int lane = threadIdx.x & 15;
-    const long long rows = (long long)a.B * a.Lq * a.Hq;
-    float s = 0.f;
-    int b = 0, i = 0, h = 0;
-    if (row < rows) {
-        h = (int)(row % a.Hq);
-        const long long t = row / a.Hq;
-        i = (int)(t % a.Lq), b = (int)(t / a.Lq);
-        if (i < band_seq(a, b).qn) {
-            const T *g = band_row<T>(a.dout, b, i, h), *o = band_row<T>(a.out, b, i, h);
-            const float *o32 = a.out32 ? a.out32 + (size_t)row * a.D : nullptr;
-            if (MODE == 0 && a.D % 8 == 0 && o32 == nullptr) {
-                for (int d = 8 * lane; d < a.D; d += 128) {
-                    const float4 g0 = io<T>::ld4(g + d), g1 = io<T>::ld4(g + d + 4), o0 = io<T>::ld4(o + d), o1 = io<T>::ld4(o + d + 4);
-                    s += ((g0.x * o0.x + g0.y * o0.y) + (g0.z * o0.z + g0.w * o0.w)) + ((g1.x * o1.x + g1.y * o1.y) + (g1.z * o1.z + g1.w * o1.w));
-                }
-            } else {
-                for (int d = lane; d < a.D; d += 16) s = __builtin_fmaf(io<T>::ld(g + d), o32 ? o32[d] : io<T>::ld(o + d), s);
-            }
-        }
-    }
-#pragma unroll
-    for (int k = 8; k > 0; k >>= 1) s += __shfl_xor(s, k, 64);
-    if (row < rows && lane == 0) a.delta[((size_t)b * a.Hq + h) * a.Lq + i] = s;
-}
 
 // ---- dk, dv: 128 keys of a workgroup, 32 per wave -----------------------------------------------------------------
 // A key block's work is its row tiles times the query heads that share the keys.  Blocks of sinks are seen by every row
@@ -243,15 +214,16 @@ template <typename T> __global__ __launch_bounds__(256) void band_attn_join_dkv_
     io<T>::st(const_cast<T *>(band_row<T>(t, b, j, hk)) + d, which ? v : v * a.scale);
 }
 
-// Two workgroups a CU are wanted (one for wide heads and fp32, whose registers allow no more), of at least 8 steps; blocks of
-// sinks are cut into chunks as long as the others' ones.
+// Two workgroups a CU are wanted (one for wide heads and fp32, whose registers allow no more); a run of the work is at least 8
+// steps long (2 in fp32, whose products take 16 times as long), so that its share does not cost more than it brings.  Blocks of
+// sinks are cut into runs as long as the others' ones.
 static BandChunks band_chunks(const BandArgs &a, int dtype) {
     BandChunks c = {0, 1, 1, 0};
     const long long nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS, heads = (long long)a.B * a.Hkv, tiles = (a.Lq + BAND_TILE - 1) / BAND_TILE;
     if (nkb == 0 || heads == 0 || tiles == 0) return c;
     const long long window = (long long)a.left + a.right + BAND_ROWS, reach = window >= a.Lq ? tiles : window / BAND_TILE + 2;
     const long long normal = (reach < tiles ? reach : tiles) * a.G;  // steps of a block in the middle
-    const long long want = a.D > 64 || dtype == DSW_F32 ? 256 : 512, n = (want + heads * nkb - 1) / (heads * nkb), most = normal / 8;
+    const long long want = a.D > 64 || dtype == DSW_F32 ? 256 : 512, n = (want + heads * nkb - 1) / (heads * nkb), most = normal / (dtype == DSW_F32 ? 2 : 8);
     c.chunks = (int)(n < most ? n : most);
     if (c.chunks < 1) c.chunks = 1;
     if (c.chunks > 64) c.chunks = 64;
@@ -264,11 +236,14 @@ static BandChunks band_chunks(const BandArgs &a, int dtype) {
     return c;
 }
 
-// ---- dq: 128 rows of a workgroup, 32 per wave; bias gradient by distance ---------------------------------------------
-template <typename T, int DP, int MODE, bool BIAS, bool DTABLE>
+// ---- dq: 32 rows per wave; delta, which the other kernel reads; bias gradient by distance ---------------------------
+// Four waves of 32 rows each where that fills the chip.  SPLIT, for short calls: 64 rows, and two waves on each 32 that take
+// the first and the second half of every key tile and add their sums at the end.
+template <typename T, int DP, int MODE, bool BIAS, bool DTABLE, bool SPLIT>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void band_attn_dq_kernel(const BandArgs a) {
     constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE), C = DP / 16;
     constexpr bool AHEAD = DP < 128 && sizeof(T) == 2;  // registers for LDS reads well ahead of the products that need them
+    constexpr int ROWS = SPLIT ? BAND_ROWS / 2 : BAND_ROWS;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     T *const lds = reinterpret_cast<T *>(smem);  // [NB][K | V]
     float *const bias = reinterpret_cast<float *>(lds + NB * 2 * ELEMS);
@@ -277,7 +252,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
 
     const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const BandPlace at(a, blockIdx.x, gridDim.x);
+    const BandPlace at(a, blockIdx.x, gridDim.x, ROWS);
     const BandSeq &sq = at.sq;
     const BandTiles &tiles = at.tiles;
     const int b = at.b, h = at.h, i = at.i;
@@ -306,7 +281,27 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
         }
     }
     const size_t stat = ((size_t)b * a.Hq + h) * a.Lq + i;
-    const float nl = row_on ? -a.lse[stat] : -INFINITY, del = row_on ? a.delta[stat] : 0.f;
+    const float nl = row_on ? -a.lse[stat] : -INFINITY;
+    // delta = dout . out, from the result before its rounding where that was kept
+    float del = 0.f;
+    if (row_on) {
+        const T *const orow = band_row<T>(a.out, b, i, h);
+        const float *const o32 = a.out32 ? a.out32 + (((size_t)b * a.Lq + i) * a.Hq + h) * D : nullptr;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int col = 16 * c + 8 * hh;
+            if (o32) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) del = __builtin_fmaf(band_element(gf[c], e), col + e < D ? o32[col + e] : 0.f, del);
+            } else {
+                const auto of = band_load8<MODE>(orow, col, D);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) del = __builtin_fmaf(band_element(gf[c], e), band_element(of, e), del);
+            }
+        }
+    }
+    del += __shfl_xor(del, 32, 64);
+    if (row_on && hh == 0 && wave < ROWS / 32) a.delta[stat] = del;
     f32x16 dq[DP / 32];
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) dq[db] = band_zero();
@@ -349,7 +344,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
         }
         if constexpr (!Stage::DIRECT) lds_barrier();
 #pragma unroll 1
-        for (int u = 0; u < 2; ++u) {
+        for (int u = SPLIT ? wave >> 1 : 0; u < (SPLIT ? (wave >> 1) + 1 : 2); ++u) {
             const int j0 = tile + 32 * u;
             if (edges.none(j0)) continue;
             f32x16 s = band_zero(), dp = band_zero();
@@ -429,7 +424,20 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
             }
         }
     }
-    band_store_row<T, DP, MODE>(const_cast<T *>(band_row<T>(a.dq, b, i, h)), dq, a.scale, a.D, hh, i < a.Lq);
+    if constexpr (SPLIT) {
+        __syncthreads();
+        float *const meet = reinterpret_cast<float *>(smem) + (wave & 1) * 32 * DP + lane;  // [2][registers][lane]
+        if (wave >= 2) {
+#pragma unroll
+            for (int k = 0; k < DP / 2; ++k) meet[64 * k] = dq[k >> 4][k & 15];
+        }
+        __syncthreads();
+        if (wave < 2) {
+#pragma unroll
+            for (int k = 0; k < DP / 2; ++k) dq[k >> 4][k & 15] += meet[64 * k];
+        }
+    }
+    band_store_row<T, DP, MODE>(const_cast<T *>(band_row<T>(a.dq, b, i, h)), dq, a.scale, a.D, hh, i < a.Lq && (!SPLIT || wave < 2));
 
     if constexpr (DTABLE) {
         // clipped distances meet in the two end entries, then the eight tables are added
@@ -450,8 +458,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
         }
         __syncthreads();
         const int n = 2 * a.M + 1;
-        const int nqb = (a.Lq + BAND_ROWS - 1) / BAND_ROWS;
-        float *const dst = a.partial + ((size_t)h * a.B * nqb + (size_t)b * nqb + at.i_lo / BAND_ROWS) * n;
+        const int nqb = (a.Lq + ROWS - 1) / ROWS;
+        float *const dst = a.partial + ((size_t)h * a.B * nqb + (size_t)b * nqb + at.i_lo / ROWS) * n;
         for (int e = threadIdx.x; e < n; e += 256) {
             float v = 0.f;
 #pragma unroll
@@ -485,9 +493,22 @@ template <typename K> static int allow_lds(K kern, size_t lds) {
     return e == hipSuccess ? DSW_OK : fail(DSW_ELAUNCH, "dsw_band_attn_bwd: %zu bytes of LDS: %s", lds, hipGetErrorString(e));
 }
 
+// rows of a dq workgroup: 64 while 128 would leave SIMDs without a wave
+static int band_dq_rows(const BandArgs &a) {
+    return (long long)a.B * a.Hq * ((a.Lq + BAND_ROWS - 1) / BAND_ROWS) < 256 ? BAND_ROWS / 2 : BAND_ROWS;
+}
+
 template <typename T, int DP, int MODE, bool BIAS, bool DTABLE> static int launch_bwd(const BandArgs &a, hipStream_t st) {
     const size_t images = (size_t)band_t<T>::nbuf(DP) * 2 * band_t<T>::template elems<DP>(BAND_TILE) * sizeof(T);
     const size_t bl = BIAS ? (2 * (a.M + BAND_MARGIN) + 1) * sizeof(float) : 0;
+    if (a.Lq) {
+        const size_t lds = images + bl + (DTABLE ? 8 * bl : 0);
+        const bool split = band_dq_rows(a) < BAND_ROWS;
+        auto kern = split ? band_attn_dq_kernel<T, DP, MODE, BIAS, DTABLE, true> : band_attn_dq_kernel<T, DP, MODE, BIAS, DTABLE, false>;
+        if (int rc = allow_lds(kern, lds)) return rc;
+        kern<<<dim3((unsigned)((long long)a.B * a.Hq * ((a.Lq + band_dq_rows(a) - 1) / band_dq_rows(a)))), 256, lds, st>>>(a);
+        if (int rc = check_launch("dsw_band_attn_bwd (dq)")) return rc;
+    }
     if (a.Lk) {
         const size_t lds = images + (size_t)band_t<T>::nbuf(DP) * 2 * BAND_TILE * sizeof(float) + bl;
         auto kern = band_attn_dkv_kernel<T, DP, MODE, BIAS>;
@@ -501,13 +522,6 @@ template <typename T, int DP, int MODE, bool BIAS, bool DTABLE> static int launc
             band_attn_join_dkv_kernel<T><<<dim3((unsigned)(joined * a.D)), 256, 0, st>>>(a);  // (2 * 128 * D elements per block)
             if (int rc = check_launch("dsw_band_attn_bwd (join)")) return rc;
         }
-    }
-    if (a.Lq) {
-        const size_t lds = images + bl + (DTABLE ? 8 * bl : 0);
-        auto kern = band_attn_dq_kernel<T, DP, MODE, BIAS, DTABLE>;
-        if (int rc = allow_lds(kern, lds)) return rc;
-        kern<<<dim3((unsigned)((long long)a.B * a.Hq * ((a.Lq + BAND_ROWS - 1) / BAND_ROWS))), 256, lds, st>>>(a);
-        if (int rc = check_launch("dsw_band_attn_bwd (dq)")) return rc;
     }
     return DSW_OK;
 }
@@ -523,7 +537,7 @@ extern "C" size_t dsw_band_attn_bwd_workspace(const dsw_band_desc *d) {
     if (band_make_args("dsw_band_attn_bwd_workspace", d, a)) return 0;
     size_t n = round16((size_t)a.B * a.Hq * a.Lq);
     n += (size_t)band_chunks(a, d->dtype).shares * 2 * BAND_ROWS * a.D;
-    if (a.table) n += (size_t)a.Hq * ((size_t)a.B * ((a.Lq + BAND_ROWS - 1) / BAND_ROWS) + 1) * (2 * a.M + 1);
+    if (a.table) n += (size_t)a.Hq * ((size_t)a.B * ((a.Lq + band_dq_rows(a) - 1) / band_dq_rows(a)) + 1) * (2 * a.M + 1);
     return n * sizeof(float);
 }
 
@@ -556,21 +570,12 @@ extern "C" int dsw_band_attn_bwd(const dsw_band_desc *d, const void *q, const ds
     a.shares = a.delta + round16((size_t)a.B * a.Hq * a.Lq);
     a.partial = a.shares + (size_t)chunks.shares * 2 * BAND_ROWS * a.D;
     hipStream_t st = as_stream(stream);
-    if (!no_rows) {
-        const long long rows = (long long)a.B * a.Lq * a.Hq;
-        const dim3 grid((unsigned)((rows + 15) / 16));
-        DSW_DISPATCH_DTYPE(d->dtype, T, {
-            if (mode == 0) band_attn_delta_kernel<T, 0><<<grid, 256, 0, st>>>(a);
-            else band_attn_delta_kernel<T, 2><<<grid, 256, 0, st>>>(a);
-        });
-        if ((rc = check_launch("dsw_band_attn_bwd (delta)"))) return rc;
-    }
     DSW_BAND_DISPATCH(d->dtype, a.D, mode, T, DP, MODE, {
         rc = d_table ? launch_bwd<T, DP, MODE, true, true>(a, st)
              : a.table ? launch_bwd<T, DP, MODE, true, false>(a, st) : launch_bwd<T, DP, MODE, false, false>(a, st);
     });
     if (rc || d_table == nullptr) return rc;
-    const int n = 2 * a.M + 1, rows = a.B * ((a.Lq + BAND_ROWS - 1) / BAND_ROWS);
+    const int n = 2 * a.M + 1, rows = a.B * ((a.Lq + band_dq_rows(a) - 1) / band_dq_rows(a));
     float *by_distance = a.partial + (size_t)a.Hq * rows * n;
     band_attn_distance_kernel<<<dim3((n + 31) / 32, a.Hq), 1024, 0, st>>>(a.partial, rows, n, by_distance);
     if ((rc = check_launch("dsw_band_attn_bwd (distances)"))) return rc;

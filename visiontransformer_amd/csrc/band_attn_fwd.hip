@@ -312,7 +312,7 @@ extern "C" int dsw_band_attn_fwd(const dsw_band_desc *d, const void *q, const ds
     a.lse = lse;
     a.out32 = out32;
     hipStream_t st = as_stream(stream);
-    if (lse == nullptr && out32 == nullptr && band_step_plan(*d, a.nrb, a.nsplit)) {
+    if (out32 == nullptr && band_step_plan(*d, a.nrb, a.nsplit)) {
         const size_t need = dsw_band_attn_fwd_workspace(d);
         DSW_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "%s: workspace of %zu bytes, %zu are needed", who, workspace_bytes, need);
         a.partial = static_cast<float *>(workspace);

@@ -1,4 +1,5 @@
-// Attention over token sequences for few query rows: new tokens over a cache (see band_attn.hpp for the mathematics).
+// Attention over token sequences for few query rows: new tokens over a cache, short sequences (see band_attn.hpp for the
+// mathematics).
 //
 // Bound by the bytes of the keys and values, which every query head of a shared key head reads: the Lq * G rows of a key
 // head sit side by side on the lane axis of one 32x32 tile (32 rows to a block).  A workgroup takes one block and one of
@@ -183,7 +184,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
         const float sum = (os[e] + os[n + e]) + (os[2 * n + e] + os[3 * n + e]);
         if (a.nsplit == 1) {
             const int ro = rb * 32 + rl, io_ = ro / a.G, ho = hk * a.G + ro - io_ * a.G;
-            io<T>::st(const_cast<T *>(band_row<T>(a.out, b, io_, ho)) + d, den == 0.f || io_ >= sq.qn ? 0.f : sum / den);
+            const bool off = den == 0.f || io_ >= sq.qn;
+            io<T>::st(const_cast<T *>(band_row<T>(a.out, b, io_, ho)) + d, off ? 0.f : sum / den);
+            if (a.lse && d == 0) a.lse[((size_t)b * a.Hq + ho) * a.Lq + io_] = off ? INFINITY : mx + __builtin_amdgcn_logf(den);
         } else {
             float *const ws = a.partial + (((size_t)bh * a.nrb + rb) * a.nsplit + sp) * 32 * (a.D + 2);
             ws[rl * (a.D + 2) + d] = sum;
@@ -218,14 +221,13 @@ template <typename T> __global__ __launch_bounds__(256) void band_attn_join_kern
     T *out = const_cast<T *>(band_row<T>(a.out, b, i, h));
     if (lane < a.D) io<T>::st(out + lane, off ? 0.f : o0 / den);
     if (lane + 64 < a.D) io<T>::st(out + lane + 64, off ? 0.f : o1 / den);
+    if (a.lse && lane == 0) a.lse[((size_t)b * a.Hq + h) * a.Lq + i] = off ? INFINITY : mt + __builtin_amdgcn_logf(den);
 }
 
-// Few rows: at most 32 rows of a key head, or too few of the other kernel's workgroups to fill the chip while the rows
-// of a key head fit four blocks.
+// Few rows: at most 32 rows of a key head, or too few of the other kernel's workgroups (128 rows of a head) for the chip.
 bool band_step_plan(const dsw_band_desc &d, int &nrb, int &nsplit) {
     if (d.B == 0 || d.Lq == 0 || d.Hq == 0 || d.Hkv == 0) return false;
     const long long R = (long long)d.Lq * (d.Hq / d.Hkv);
-    if (R > 128) return false;
     if (R > 32 && (long long)d.B * d.Hq * ((d.Lq + BAND_ROWS - 1) / BAND_ROWS) >= 256) return false;
     nrb = (int)((R + 31) / 32);
     const long long span = d.left < 0 ? d.Lk : (long long)d.left + d.Lq + (d.right > 0 ? d.right : 0) + d.sinks + 2 * STEP_KEYS;

@@ -2400,11 +2400,13 @@ def _call_on(device, name, *args):
 
 def _head_rows(t):
     """[B, L, H, D] with D contiguous (a copy where it is not), its dsw_strides and address"""
-    if t.stride(3) != 1 and t.shape[3] > 1:
+    b, l, h, d = t.stride()
+    nb, nl, nh, nd = t.shape
+    if d != 1 and nd > 1:
         t = t.contiguous()
+        b, l, h, d = t.stride()
     # (strides of dimensions of one element mean nothing, but would count against the alignment)
-    s = _lib.Strides(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
-    return t, ctypes.byref(s), _c_void_p(t.data_ptr())
+    return t, ctypes.byref(_lib.Strides(b if nb > 1 else 0, l if nl > 1 else 0, h if nh > 1 else 0)), t.data_ptr()
 
 
 def _same_kind(who, named):
@@ -2543,10 +2545,8 @@ class _BandAttnFn(torch.autograd.Function):
         exact = train and ctx.needs_input_grad[3] and q.dtype == torch.bfloat16
         out32 = torch.empty(B, Lq, Hq, D, dtype=torch.float32, device=dev) if exact else None
         if B * Lq * Hq:
-            ws, n = None, 0
-            if not train:
-                n = int(_lib.load().dsw_band_attn_fwd_workspace(ctypes.byref(desc)))
-                ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+            n = 0 if exact else int(_lib.load().dsw_band_attn_fwd_workspace(ctypes.byref(desc)))
+            ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
             _call_on(dev, "dsw_band_attn_fwd", ctypes.byref(desc), pq, sq, pk, sk, pv, sv, po, so, ptr(lse), ptr(out32), ptr(ws), n, stream(dev))
         if train:
             ctx.save_for_backward(q, k, v, tab, buckets, q_lens, k_lens, out, out32, lse)
