@@ -214,7 +214,7 @@ template <typename T> __global__ __launch_bounds__(256) void band_attn_join_dkv_
     io<T>::st(const_cast<T *>(band_row<T>(t, b, j, hk)) + d, which ? v : v * a.scale);
 }
 
-// Two workgroups a CU are wanted (one for wide heads and fp32, whose registers allow no more); a run of the work is at least 8
+// Two workgroups a CU are wanted (one for wide heads, whose registers allow no more); a run of the work is at least 8
 // steps long (2 in fp32, whose products take 16 times as long), so that its share does not cost more than it brings.  Blocks of
 // sinks are cut into runs as long as the others' ones.
 static BandChunks band_chunks(const BandArgs &a, int dtype) {
@@ -223,7 +223,7 @@ static BandChunks band_chunks(const BandArgs &a, int dtype) {
     if (nkb == 0 || heads == 0 || tiles == 0) return c;
     const long long window = (long long)a.left + a.right + BAND_ROWS, reach = window >= a.Lq ? tiles : window / BAND_TILE + 2;
     const long long normal = (reach < tiles ? reach : tiles) * a.G;  // steps of a block in the middle
-    const long long want = a.D > 64 || dtype == DSW_F32 ? 256 : 512, n = (want + heads * nkb - 1) / (heads * nkb), most = normal / (dtype == DSW_F32 ? 2 : 8);
+    const long long want = a.D > 64 ? 256 : 512, n = (want + heads * nkb - 1) / (heads * nkb), most = normal / (dtype == DSW_F32 ? 2 : 8);
     c.chunks = (int)(n < most ? n : most);
     if (c.chunks < 1) c.chunks = 1;
     if (c.chunks > 64) c.chunks = 64;
@@ -248,7 +248,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     T *const lds = reinterpret_cast<T *>(smem);  // [NB][K | V]
     float *const bias = reinterpret_cast<float *>(lds + NB * 2 * ELEMS);
     const int BL = 2 * (a.M + BAND_MARGIN) + 1;
-    float *const sums = bias + BL;  // [4 waves][2 lane halves][BL]: dS by distance
+    // (a table's gradient only) dS of a tile by distance, [4 waves][32 rows][64], and what each wave summed, [4][BL]
+    float *const slant = bias + ((BL + 3) & ~3), *const sums = slant + 4 * 32 * 64;
 
     const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -266,7 +267,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
 
     if constexpr (BIAS) band_stage_bias(a, h, 1, bias, 256);
     if constexpr (DTABLE) {
-        for (int e = threadIdx.x; e < 8 * BL; e += 256) sums[e] = 0.f;
+        for (int e = threadIdx.x; e < 4 * (32 * 64 + BL); e += 256) slant[e] = 0.f;  // (before the first tile's barrier)
     }
     typename band_t<T>::frag qf[C], gf[C];
     const T *const qrow = band_row<T>(a.q, b, i, h), *const grow = band_row<T>(a.dout, b, i, h);
@@ -397,13 +398,21 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] *= dp[r] - del;
             if constexpr (DTABLE) {
-                // the 32 lanes of a half hold one key each time: 32 different distances, in a table that only this wave's
-                // half adds to, one instruction after the other - the order of the sums is fixed
+                // A row's 32 values go one column further left than the row's above, so that the 63 distances of the tile are
+                // columns (the rest of the 64 x 32 stays zero), and a lane sums one: in order, where the atomic additions
+                // of LDS, in no order, took 140 cycles for each of the 16 registers.
                 if (near) {
-                    float *const mine = sums + (2 * wave + hh) * BL + e0;
+                    float *const mine = slant + wave * 32 * 64;
+                    asm volatile("" ::: "memory");
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        __hip_atomic_fetch_add(mine + rho(r), s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                    for (int r = 0; r < 16; ++r) mine[l31 * 63 + 31 + 4 * hh + rho(r)] = s[r];
+                    asm volatile("" ::: "memory");  // (a wave's LDS accesses complete in order)
+                    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) part[k & 3] += mine[64 * k + lane];
+                    float *const at_distance = sums + wave * BL + (j0 - w_lo + lane - 31 + M + BAND_MARGIN);
+                    *at_distance += (part[0] + part[1]) + (part[2] + part[3]);
+                    asm volatile("" ::: "memory");
                 } else {
                     float t = 0.f;
 #pragma unroll
@@ -440,11 +449,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     band_store_row<T, DP, MODE>(const_cast<T *>(band_row<T>(a.dq, b, i, h)), dq, a.scale, a.D, hh, i < a.Lq && (!SPLIT || wave < 2));
 
     if constexpr (DTABLE) {
-        // clipped distances meet in the two end entries, then the eight tables are added
+        // clipped distances meet in the two end entries, then the four waves' sums are added
         far_lo = wave_sum(far_lo);
         far_hi = wave_sum(far_hi);
         __syncthreads();
-        if (threadIdx.x < 16) {
+        if (threadIdx.x < 8) {
             float *const t = sums + (threadIdx.x >> 1) * BL;
             const int e = threadIdx.x & 1 ? BL - 1 - BAND_MARGIN : BAND_MARGIN, dir = threadIdx.x & 1 ? 1 : -1;
             float v = t[e];
@@ -453,18 +462,16 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
         }
         __syncthreads();
         if (lane == 0) {
-            sums[2 * wave * BL + BAND_MARGIN] += far_lo;
-            sums[2 * wave * BL + BL - 1 - BAND_MARGIN] += far_hi;
+            sums[wave * BL + BAND_MARGIN] += far_lo;
+            sums[wave * BL + BL - 1 - BAND_MARGIN] += far_hi;
         }
         __syncthreads();
         const int n = 2 * a.M + 1;
         const int nqb = (a.Lq + ROWS - 1) / ROWS;
         float *const dst = a.partial + ((size_t)h * a.B * nqb + (size_t)b * nqb + at.i_lo / ROWS) * n;
         for (int e = threadIdx.x; e < n; e += 256) {
-            float v = 0.f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v += sums[k * BL + BAND_MARGIN + e];
-            dst[e] = v;
+            const float *const t = sums + BAND_MARGIN + e;
+            dst[e] = (t[0] + t[BL]) + (t[2 * BL] + t[3 * BL]);
         }
     }
 }
@@ -502,7 +509,7 @@ template <typename T, int DP, int MODE, bool BIAS, bool DTABLE> static int launc
     const size_t images = (size_t)band_t<T>::nbuf(DP) * 2 * band_t<T>::template elems<DP>(BAND_TILE) * sizeof(T);
     const size_t bl = BIAS ? (2 * (a.M + BAND_MARGIN) + 1) * sizeof(float) : 0;
     if (a.Lq) {
-        const size_t lds = images + bl + (DTABLE ? 8 * bl : 0);
+        const size_t lds = images + (DTABLE ? ((bl + 15) & ~(size_t)15) + 4 * (32 * 64 * sizeof(float) + bl) : bl);
         const bool split = band_dq_rows(a) < BAND_ROWS;
         auto kern = split ? band_attn_dq_kernel<T, DP, MODE, BIAS, DTABLE, true> : band_attn_dq_kernel<T, DP, MODE, BIAS, DTABLE, false>;
         if (int rc = allow_lds(kern, lds)) return rc;
