@@ -197,21 +197,31 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
     }
 }
 
-// one element of dk or dv per thread: the sum of its block's shares, in their order
-template <typename T> __global__ __launch_bounds__(256) void band_attn_join_dkv_kernel(const BandArgs a) {
+// V elements of a row of dk or dv per thread (4 where every row is a whole number of them): the sum of the block's shares, in
+// their order.  2 * 128 * D elements per block, D / V workgroups.
+template <typename T, int V> __global__ __launch_bounds__(256) void band_attn_join_dkv_kernel(const BandArgs a) {
     const int nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS, n_sink = a.sink_blocks * a.sink_chunks;
     const int blocks = a.chunks > 1 ? nkb : a.sink_blocks, per = a.chunks > 1 ? n_sink + (nkb - a.sink_blocks) * a.chunks : n_sink;
-    const int block = blockIdx.x / a.D, bh = block / blocks, kb = block - bh * blocks, hk = bh % a.Hkv, b = bh / a.Hkv;
+    const int wgs = a.D / V, block = blockIdx.x / wgs, bh = block / blocks, kb = block - bh * blocks, hk = bh % a.Hkv, b = bh / a.Hkv;
     const int nc = kb < a.sink_blocks ? a.sink_chunks : a.chunks;
     const int unit = kb < a.sink_blocks ? kb * a.sink_chunks : n_sink + (kb - a.sink_blocks) * a.chunks;
-    const int size = BAND_ROWS * a.D, e = (blockIdx.x - block * a.D) * 256 + threadIdx.x;  // D workgroups per block
+    const int size = BAND_ROWS * a.D, e = ((blockIdx.x - block * wgs) * 256 + threadIdx.x) * V;
     const int which = e >= size, row = (e - which * size) / a.D, d = e - which * size - row * a.D, j = kb * BAND_ROWS + row;
     if (j >= a.Lk) return;
     const float *src = a.shares + ((size_t)bh * per + unit) * 2 * size + e;
-    float v = 0.f;
-    for (int c = 0; c < nc; ++c) v += src[(size_t)c * 2 * size];
     const BandTensor &t = which ? a.dv : a.dk;
-    io<T>::st(const_cast<T *>(band_row<T>(t, b, j, hk)) + d, which ? v : v * a.scale);
+    T *dst = const_cast<T *>(band_row<T>(t, b, j, hk)) + d;
+    const float mul = which ? 1.f : a.scale;
+    if constexpr (V == 4) {
+        float4 v = f4zero();
+#pragma unroll 4
+        for (int c = 0; c < nc; ++c) v = v + *reinterpret_cast<const float4 *>(src + (size_t)c * 2 * size);
+        io<T>::st4(dst, v * mul);
+    } else {
+        float v = 0.f;
+        for (int c = 0; c < nc; ++c) v += src[(size_t)c * 2 * size];
+        io<T>::st(dst, v * mul);
+    }
 }
 
 // Two workgroups a CU are wanted (one for wide heads, whose registers allow no more); a run of the work is at least 8
@@ -526,7 +536,8 @@ template <typename T, int DP, int MODE, bool BIAS, bool DTABLE> static int launc
         const long long joined = heads * (a.chunks > 1 ? nkb : a.sink_chunks > 1 ? a.sink_blocks : 0);
         if (joined) {
             if (joined * a.D >= (1LL << 31)) return fail(DSW_EUNSUPPORTED, "dsw_band_attn_bwd: %lld shared key blocks", joined);
-            band_attn_join_dkv_kernel<T><<<dim3((unsigned)(joined * a.D)), 256, 0, st>>>(a);  // (2 * 128 * D elements per block)
+            if (MODE == 0) band_attn_join_dkv_kernel<T, 4><<<dim3((unsigned)(joined * (a.D / 4))), 256, 0, st>>>(a);
+            else band_attn_join_dkv_kernel<T, 1><<<dim3((unsigned)(joined * a.D)), 256, 0, st>>>(a);
             if (int rc = check_launch("dsw_band_attn_bwd (join)")) return rc;
         }
     }

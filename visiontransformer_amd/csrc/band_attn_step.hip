@@ -195,33 +195,38 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     }
 }
 
-// one wave joins the shares of one row
+// A workgroup joins the shares of one row: every thread weighs a share or two, then each wave adds every fourth share.
+constexpr int STEP_MAX_SPLITS = 512;
 template <typename T> __global__ __launch_bounds__(256) void band_attn_join_kernel(const BandArgs a) {
-    const long long row_all = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63, R = a.Lq * a.G;
-    if (row_all >= (long long)a.B * a.Hkv * R) return;
-    const int bh = (int)(row_all / R), row = (int)(row_all - (long long)bh * R), b = bh / a.Hkv, hk = bh % a.Hkv;
+    __shared__ float weight[STEP_MAX_SPLITS], red[8], sums[4][128];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, R = a.Lq * a.G;
+    const int bh = blockIdx.x / R, row = blockIdx.x - bh * R, b = bh / a.Hkv, hk = bh % a.Hkv;
     const int i = row / a.G, h = hk * a.G + row - i * a.G, W = a.D + 2;
-    const float *ws = a.partial + (((size_t)bh * a.nrb + row / 32) * a.nsplit) * 32 * W + (row & 31) * W;
-    float mt = -INFINITY;
-    for (int s = lane; s < a.nsplit; s += 64) mt = fmaxf(mt, ws[(size_t)s * 32 * W + a.D]);
-    mt = wave_max(mt);
-    float den = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float *r = ws + (size_t)s * 32 * W;
-        const float ms = r[a.D];
-        if (ms == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(ms - mt);
-        den = __builtin_fmaf(r[a.D + 1], f, den);
-        if (lane < a.D) o0 = __builtin_fmaf(r[lane], f, o0);
-        if (lane + 64 < a.D) o1 = __builtin_fmaf(r[lane + 64], f, o1);
+    const size_t step = (size_t)32 * W;
+    const float *const ws = a.partial + ((size_t)bh * a.nrb + row / 32) * a.nsplit * step + (row & 31) * W;
+    const int s0 = threadIdx.x, s1 = threadIdx.x + 256;
+    const float m0 = s0 < a.nsplit ? ws[s0 * step + a.D] : -INFINITY, m1 = s1 < a.nsplit ? ws[s1 * step + a.D] : -INFINITY;
+    const float d0 = s0 < a.nsplit ? ws[s0 * step + a.D + 1] : 0.f, d1 = s1 < a.nsplit ? ws[s1 * step + a.D + 1] : 0.f;
+    const float mt = block_max(fmaxf(m0, m1), red);
+    const float w0 = m0 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m0 - mt), w1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - mt);
+    if (s0 < a.nsplit) weight[s0] = w0;
+    if (s1 < a.nsplit) weight[s1] = w1;
+    const float den = block_sum(__builtin_fmaf(d0, w0, d1 * w1), red + 4);  // (its barriers cover the weights)
+    float o0 = 0.f, o1 = 0.f;
+    const int c0 = min(lane, a.D - 1), c1 = min(lane + 64, a.D - 1);
+#pragma unroll 4
+    for (int s = wave; s < a.nsplit; s += 4) {
+        // (a share without a visible key weighs nothing, and its sums are zeros)
+        o0 = __builtin_fmaf(ws[s * step + c0], weight[s], o0);
+        o1 = __builtin_fmaf(ws[s * step + c1], weight[s], o1);
     }
-    const BandSeq sq = band_seq(a, b);
-    const bool off = den == 0.f || i >= sq.qn;
-    T *out = const_cast<T *>(band_row<T>(a.out, b, i, h));
-    if (lane < a.D) io<T>::st(out + lane, off ? 0.f : o0 / den);
-    if (lane + 64 < a.D) io<T>::st(out + lane + 64, off ? 0.f : o1 / den);
-    if (a.lse && lane == 0) a.lse[((size_t)b * a.Hq + h) * a.Lq + i] = off ? INFINITY : mt + __builtin_amdgcn_logf(den);
+    sums[wave][lane] = o0;
+    sums[wave][lane + 64] = o1;
+    __syncthreads();
+    const bool off = den == 0.f || i >= band_seq(a, b).qn;
+    const int d = threadIdx.x;
+    if (d < a.D) io<T>::st(const_cast<T *>(band_row<T>(a.out, b, i, h)) + d, off ? 0.f : ((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) / den);
+    if (a.lse && d == 0) a.lse[((size_t)b * a.Hq + h) * a.Lq + i] = off ? INFINITY : mt + __builtin_amdgcn_logf(den);
 }
 
 // Few rows: at most 32 rows of a key head, or too few of the other kernel's workgroups (128 rows of a head) for the chip.
@@ -232,10 +237,13 @@ bool band_step_plan(const dsw_band_desc &d, int &nrb, int &nsplit) {
     nrb = (int)((R + 31) / 32);
     const long long span = d.left < 0 ? d.Lk : (long long)d.left + d.Lq + (d.right > 0 ? d.right : 0) + d.sinks + 2 * STEP_KEYS;
     const long long tiles = ((span < d.Lk ? span : d.Lk) + STEP_KEYS - 1) / STEP_KEYS, units = (long long)d.B * d.Hkv * nrb;
-    long long n = (1024 + units - 1) / units;   // four workgroups a CU
-    const long long most = (tiles + 7) / 8;      // two tiles per wave at least
+    // as many workgroups as are resident at a time (two a CU in wide heads' registers, else four), with two tiles per wave at
+    // least.  One token over 16 x 8 windows of 1028 keys of 128: 31 us at 2 to 4 shares, 35 at 1, 40 at 6 and 8; over 8 x 4
+    // caches of up to 32768 keys of 64: 44 us at 32 shares, 47 at 16 and at 64 (graph replays, with the join).
+    const long long want = d.D > 64 ? 512 : 1024, most = (tiles + 7) / 8;
+    long long n = want / units;
     n = n < most ? n : most;
-    nsplit = (int)(n < 1 ? 1 : n > 512 ? 512 : n);
+    nsplit = (int)(n < 1 ? 1 : n > STEP_MAX_SPLITS ? STEP_MAX_SPLITS : n);
     return true;
 }
 
@@ -254,7 +262,8 @@ template <typename T, int DP, int MODE, bool BIAS> static int launch_step(const 
     int rc = check_launch("dsw_band_attn_fwd");
     if (rc || a.nsplit == 1) return rc;
     const long long rows = (long long)a.B * a.Hkv * R;
-    band_attn_join_kernel<T><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(a);
+    if (rows >= (1LL << 31)) return fail(DSW_EUNSUPPORTED, "dsw_band_attn_fwd: %lld rows", rows);
+    band_attn_join_kernel<T><<<dim3((unsigned)rows), 256, 0, st>>>(a);
     return check_launch("dsw_band_attn_fwd (join)");
 }
 
