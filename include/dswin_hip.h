@@ -667,8 +667,8 @@ int dsw_qk_norm_rotary_fwd(const void *q, const dsw_strides *sq, const void *k, 
                            int axes, int pairs, const void *pos, int pos_bytes, long long pos_batch, int interleaved, void *oq,
                            const dsw_strides *soq, void *ok, const dsw_strides *sok, void *stream);
 /* Its backward: dq, dk from the gradients dyq, dyk of oq, ok (q, k: the inputs of the forward).  partial: NULL, or
- * fp32 [dsw_qk_norm_rotary_blocks(B, L)][2][D], whose column sums (dsw_colsum) are the gradients of wq and wk. */
-int dsw_qk_norm_rotary_blocks(int B, int L);
+ * fp32 [dsw_qk_norm_rotary_blocks(..)][2][D], whose column sums (dsw_colsum) are the gradients of wq and wk. */
+int dsw_qk_norm_rotary_blocks(int dtype, int B, int L, int Hq, int Hkv, int D, int axes, int pairs);
 int dsw_qk_norm_rotary_bwd(const void *q, const dsw_strides *sq, const void *k, const dsw_strides *sk, const void *dyq,
                            const dsw_strides *sdyq, const void *dyk, const dsw_strides *sdyk, int dtype, int B, int L,
                            int Hq, int Hkv, int D, const float *wq, const float *wk, float eps, const float *freqs, int axes,

@@ -129,7 +129,7 @@ SIGNATURES = {
     "dsw_sparse_disc_bwd": (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I,
                                  _P, _P, _P, _P, _P, _P, _P, _P]),
     "dsw_qk_norm_rotary_fwd": (_I, [_P, _P, _P, _P] + [_I] * 6 + [_P, _P, _F, _P, _I, _I, _P, _I, ctypes.c_longlong, _I] + [_P] * 5),
-    "dsw_qk_norm_rotary_blocks": (_I, [_I, _I]),
+    "dsw_qk_norm_rotary_blocks": (_I, [_I] * 8),
     "dsw_band_attn_fwd_workspace": (_Z, [_P]),
     "dsw_band_attn_fwd": (_I, [_P] * 12 + [_Z, _P]),
     "dsw_band_attn_bwd_workspace": (_Z, [_P]),

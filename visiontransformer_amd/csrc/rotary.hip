@@ -130,50 +130,79 @@ template <int Q, bool INTER> __device__ __forceinline__ void rot_turn(float *x, 
     }
 }
 
+// The rows (token, head) of a tile that one group of lanes takes, every G-th of them, without a division per row; where the
+// tile's tokens begin in each tensor is computed once, into LDS.  (With both per row the kernels were bound by integer
+// arithmetic: 83 us forward for 131072 tokens of 12 rows of 30.)
+constexpr int ROT_TOKENS = 32;  // of a tile, at most
+struct RotRows {
+    int t, h, dt, dh, H;
+    __device__ __forceinline__ RotRows(int heads, int grp, int G) {
+        H = heads > 0 ? heads : 1;  // (no heads: the caller takes no rows)
+        dt = G / H, dh = G - dt * H;
+        t = grp / H, h = grp - t * H;
+    }
+    __device__ __forceinline__ void next() {
+        t += dt, h += dh;
+        const bool over = h >= H;
+        h -= over ? H : 0, t += over;
+    }
+};
+// offsets [tensor][token] for x (0, 1), y (2, 3) and, backward, dy (4, 5); a barrier is the caller's
+__device__ __forceinline__ void rot_offsets(const RotArgs &a, long long token0, int nt, int tensors, long long *off) {
+    if (threadIdx.x >= (unsigned)(tensors * ROT_TOKENS)) return;
+    const int k = threadIdx.x / ROT_TOKENS, t = threadIdx.x % ROT_TOKENS;
+    if (t >= nt) return;
+    const long long token = token0 + t, b = token / a.L, l = token - b * a.L;
+    const RotOperand &o = k < 2 ? a.x[k] : k < 4 ? a.y[k - 2] : a.dy[k - 4];
+    off[k * ROT_TOKENS + t] = b * o.s.b + l * o.s.l;
+}
+
 template <typename T, int Q, int NU, bool INTER>
 __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_fwd_kernel(const RotArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int n = a.axes * a.pairs, D = a.D, H = a.Hq + a.Hkv;
+    const int n = a.axes * a.pairs, D = a.D;
     const long long token0 = (long long)blockIdx.x * a.tpw;
     const int nt = (int)(a.tokens - token0 < a.tpw ? a.tokens - token0 : a.tpw);
     float *w = reinterpret_cast<float *>(smem);
     float2 *cs = reinterpret_cast<float2 *>(w + ((2 * D + 3) & ~3));
     const int RL = 1 << a.rl_log, lane = threadIdx.x & (RL - 1), grp = threadIdx.x >> a.rl_log, G = ROT_THREADS >> a.rl_log;
-    const int rows = nt * H;
     const float inv_d = 1.f / (float)D;
-    constexpr int AHEAD = Q == 8 ? 2 : 1;  // rows whose loads are under way together
+    constexpr int AHEAD = 2;  // rows whose loads are under way together
+    __shared__ long long off[4 * ROT_TOKENS];
+    rot_offsets(a, token0, nt, 4, off);
+    __syncthreads();
+    RotRows row(a.Hq + a.Hkv, grp, G);
     bool first = true;
-    for (int r0 = grp; first || r0 < rows; r0 += AHEAD * G) {
+    while (first || row.t < nt) {
         float x[AHEAD][NU][2 * Q];
         T *dst[AHEAD];
+        int tk[AHEAD], kind[AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
-            const int row = r0 + k * G;
             dst[k] = nullptr;
 #pragma unroll
             for (int j = 0; j < NU; ++j)
 #pragma unroll
                 for (int i = 0; i < 2 * Q; ++i) x[k][j][i] = 0.f;
-            if (row >= rows) continue;
-            const int t = row / H;
-            int h = row - t * H;
-            const int which = h >= a.Hq;
-            h -= which ? a.Hq : 0;
-            const long long token = token0 + t, b = token / a.L, l = token - b * a.L;
-            const dsw_strides &si = a.x[which].s, &so = a.y[which].s;
-            const T *src = static_cast<const T *>(a.x[which].p) + b * si.b + l * si.l + h * si.h;
-            dst[k] = static_cast<T *>(const_cast<void *>(a.y[which].p)) + b * so.b + l * so.l + h * so.h;
+            tk[k] = row.t, kind[k] = row.h >= a.Hq;
+            if (row.t < nt) {
+                const int which = kind[k], h = row.h - (which ? a.Hq : 0);
+                const T *src = static_cast<const T *>(which ? a.x[1].p : a.x[0].p) + off[which * ROT_TOKENS + row.t] + h * (which ? a.x[1].s.h : a.x[0].s.h);
+                dst[k] = static_cast<T *>(const_cast<void *>(which ? a.y[1].p : a.y[0].p)) + off[(2 + which) * ROT_TOKENS + row.t] +
+                         h * (which ? a.y[1].s.h : a.y[0].s.h);
 #pragma unroll
-            for (int j = 0; j < NU; ++j) {
-                const int u = lane + j * RL;
-                int ca, cb;
-                bool turned;
-                if (u < a.units) {
-                    const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
-                    piece<T, Q>::ld(src + ca, x[k][j]);
-                    if (two) piece<T, Q>::ld(src + cb, x[k][j] + Q);
+                for (int j = 0; j < NU; ++j) {
+                    const int u = lane + j * RL;
+                    int ca, cb;
+                    bool turned;
+                    if (u < a.units) {
+                        const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
+                        piece<T, Q>::ld(src + ca, x[k][j]);
+                        if (two) piece<T, Q>::ld(src + cb, x[k][j] + Q);
+                    }
                 }
             }
+            row.next();
         }
         if (first) {  // the tables are made while the first rows are on their way
             rot_tables(a, token0, nt, cs, w);
@@ -182,15 +211,14 @@ __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_fwd_kernel(const R
         }
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
-            if (dst[k] == nullptr) continue;
-            const int row = r0 + k * G, t = row / H;
-            const float *wr = w + (row - t * H >= a.Hq ? D : 0);
             float ss = 0.f;
 #pragma unroll
             for (int j = 0; j < NU; ++j)
 #pragma unroll
                 for (int i = 0; i < 2 * Q; ++i) ss = __builtin_fmaf(x[k][j][i], x[k][j][i], ss);
             for (int o = RL >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+            if (dst[k] == nullptr) continue;
+            const float *wr = w + (kind[k] ? D : 0);
             const float r = rsqrtf(ss * inv_d + a.eps);
 #pragma unroll
             for (int j = 0; j < NU; ++j) {
@@ -205,7 +233,7 @@ __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_fwd_kernel(const R
                     v[i] = v[i] * r * wr[ca + i];
                     v[Q + i] = two ? v[Q + i] * r * wr[cb + i] : 0.f;
                 }
-                if (turned) rot_turn<Q, INTER>(v, cs + t * n + Q * u, false);
+                if (turned) rot_turn<Q, INTER>(v, cs + tk[k] * n + Q * u, false);
                 piece<T, Q>::st(dst[k] + ca, v);
                 if (two) piece<T, Q>::st(dst[k] + cb, v + Q);
             }
@@ -223,6 +251,8 @@ __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_bwd_kernel(const R
     float2 *cs = reinterpret_cast<float2 *>(w + ((2 * D + 3) & ~3));
     const int RL = 1 << a.rl_log, lane = threadIdx.x & (RL - 1), grp = threadIdx.x >> a.rl_log, G = ROT_THREADS >> a.rl_log;
     const float inv_d = 1.f / (float)D;
+    constexpr int AHEAD = Q == 8 ? 1 : 2;
+    __shared__ long long off[6 * ROT_TOKENS];
     float dw[2][NU][2 * Q];
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -235,73 +265,92 @@ __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_bwd_kernel(const R
         const long long token0 = tile * a.tpw;
         const int nt = (int)(a.tokens - token0 < a.tpw ? a.tokens - token0 : a.tpw);
         __syncthreads();  // the last tile's readers are done
+        rot_offsets(a, token0, nt, 6, off);
         rot_tables(a, token0, nt, cs, tile == blockIdx.x ? w : nullptr);
         __syncthreads();
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            const int H = m ? a.Hkv : a.Hq, rows = nt * H;
-            const dsw_strides &sx = a.x[m].s, &sg = a.dy[m].s, &so = a.y[m].s;
-            for (int row = grp; row < rows; row += G) {
-                const int t = row / H, h = row - t * H;
-                const long long token = token0 + t, b = token / a.L, l = token - b * a.L;
-                const T *src = static_cast<const T *>(a.x[m].p) + b * sx.b + l * sx.l + h * sx.h;
-                const T *grd = static_cast<const T *>(a.dy[m].p) + b * sg.b + l * sg.l + h * sg.h;
-                T *dst = static_cast<T *>(const_cast<void *>(a.y[m].p)) + b * so.b + l * so.l + h * so.h;
-                float x[NU][2 * Q], g[NU][2 * Q];
-                float ss = 0.f;
+            const int H = m ? a.Hkv : a.Hq;
+            if (H == 0) continue;
+            RotRows row(H, grp, G);
+            while (row.t < nt) {
+                float x[AHEAD][NU][2 * Q], g[AHEAD][NU][2 * Q];
+                T *dst[AHEAD];
+                int tk[AHEAD];
 #pragma unroll
-                for (int j = 0; j < NU; ++j) {
-                    const int u = lane + j * RL;
+                for (int k = 0; k < AHEAD; ++k) {
+                    dst[k] = nullptr;
+                    tk[k] = row.t;
 #pragma unroll
-                    for (int i = 0; i < 2 * Q; ++i) x[j][i] = 0.f, g[j][i] = 0.f;
-                    if (u >= a.units) continue;
-                    int ca, cb;
-                    bool turned;
-                    const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
-                    piece<T, Q>::ld(src + ca, x[j]);
-                    piece<T, Q>::ld(grd + ca, g[j]);
-                    if (two) {
-                        piece<T, Q>::ld(src + cb, x[j] + Q);
-                        piece<T, Q>::ld(grd + cb, g[j] + Q);
+                    for (int j = 0; j < NU; ++j)
+#pragma unroll
+                        for (int i = 0; i < 2 * Q; ++i) x[k][j][i] = 0.f, g[k][j][i] = 0.f;
+                    if (row.t < nt) {
+                        const T *src = static_cast<const T *>(a.x[m].p) + off[m * ROT_TOKENS + row.t] + row.h * a.x[m].s.h;
+                        const T *grd = static_cast<const T *>(a.dy[m].p) + off[(4 + m) * ROT_TOKENS + row.t] + row.h * a.dy[m].s.h;
+                        dst[k] = static_cast<T *>(const_cast<void *>(a.y[m].p)) + off[(2 + m) * ROT_TOKENS + row.t] + row.h * a.y[m].s.h;
+#pragma unroll
+                        for (int j = 0; j < NU; ++j) {
+                            const int u = lane + j * RL;
+                            int ca, cb;
+                            bool turned;
+                            if (u < a.units) {
+                                const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
+                                piece<T, Q>::ld(src + ca, x[k][j]);
+                                piece<T, Q>::ld(grd + ca, g[k][j]);
+                                if (two) {
+                                    piece<T, Q>::ld(src + cb, x[k][j] + Q);
+                                    piece<T, Q>::ld(grd + cb, g[k][j] + Q);
+                                }
+                            }
+                        }
                     }
-                    if (turned) rot_turn<Q, INTER>(g[j], cs + t * n + Q * u, true);
+                    row.next();
                 }
 #pragma unroll
-                for (int j = 0; j < NU; ++j)
+                for (int k = 0; k < AHEAD; ++k) {
+                    float ss = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 2 * Q; ++i) ss = __builtin_fmaf(x[j][i], x[j][i], ss);
-                for (int o = RL >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-                const float r = rsqrtf(ss * inv_d + a.eps);
-                float dot = 0.f;
+                    for (int j = 0; j < NU; ++j)
 #pragma unroll
-                for (int j = 0; j < NU; ++j) {
-                    const int u = lane + j * RL;
-                    if (u >= a.units) continue;
-                    int ca, cb;
-                    bool turned;
-                    const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
+                        for (int i = 0; i < 2 * Q; ++i) ss = __builtin_fmaf(x[k][j][i], x[k][j][i], ss);
+                    for (int o = RL >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+                    const float r = rsqrtf(ss * inv_d + a.eps);
+                    float dot = 0.f;
+                    if (dst[k] != nullptr) {
 #pragma unroll
-                    for (int i = 0; i < 2 * Q; ++i) {
-                        if (i >= Q && !two) continue;
-                        x[j][i] *= r;
-                        dw[m][j][i] = __builtin_fmaf(g[j][i], x[j][i], dw[m][j][i]);
-                        g[j][i] *= w[m * D + (i < Q ? ca + i : cb + i - Q)];
-                        dot = __builtin_fmaf(g[j][i], x[j][i], dot);
+                        for (int j = 0; j < NU; ++j) {
+                            const int u = lane + j * RL;
+                            if (u >= a.units) continue;
+                            int ca, cb;
+                            bool turned;
+                            const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
+                            if (turned) rot_turn<Q, INTER>(g[k][j], cs + tk[k] * n + Q * u, true);
+#pragma unroll
+                            for (int i = 0; i < 2 * Q; ++i) {
+                                const float wv = i < Q ? w[m * D + ca + i] : two ? w[m * D + cb + i - Q] : 0.f;
+                                x[k][j][i] *= r;  // (zero, like g, in a piece that is not there)
+                                dw[m][j][i] = __builtin_fmaf(g[k][j][i], x[k][j][i], dw[m][j][i]);
+                                g[k][j][i] *= wv;
+                                dot = __builtin_fmaf(g[k][j][i], x[k][j][i], dot);
+                            }
+                        }
                     }
-                }
-                for (int o = RL >> 1; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
-                dot *= inv_d;
+                    for (int o = RL >> 1; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
+                    dot *= inv_d;
+                    if (dst[k] == nullptr) continue;
 #pragma unroll
-                for (int j = 0; j < NU; ++j) {
-                    const int u = lane + j * RL;
-                    if (u >= a.units) continue;
-                    int ca, cb;
-                    bool turned;
-                    const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
+                    for (int j = 0; j < NU; ++j) {
+                        const int u = lane + j * RL;
+                        if (u >= a.units) continue;
+                        int ca, cb;
+                        bool turned;
+                        const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
 #pragma unroll
-                    for (int i = 0; i < 2 * Q; ++i) g[j][i] = r * __builtin_fmaf(-x[j][i], dot, g[j][i]);
-                    piece<T, Q>::st(dst + ca, g[j]);
-                    if (two) piece<T, Q>::st(dst + cb, g[j] + Q);
+                        for (int i = 0; i < 2 * Q; ++i) g[k][j][i] = r * __builtin_fmaf(-x[k][j][i], dot, g[k][j][i]);
+                        piece<T, Q>::st(dst[k] + ca, g[k][j]);
+                        if (two) piece<T, Q>::st(dst[k] + cb, g[k][j] + Q);
+                    }
                 }
             }
         }
@@ -333,11 +382,31 @@ __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_bwd_kernel(const R
 
 constexpr int ROT_MAX_D = 128, ROT_BWD_BLOCKS = 2048;
 
-// tokens of a workgroup: eight where that still leaves two thousand workgroups (the angles of a token are computed
-// once per workgroup, whatever it is), fewer for short calls, down to one per new token
-static int rot_tokens_per_wg(long long tokens) {
-    const long long t = tokens / 2048;
-    return t < 1 ? 1 : t > 8 ? 8 : (int)t;
+// Tokens of a tile: eight rows for each group of lanes (sixteen backward, where a tile costs two barriers), so that the
+// angles, computed once per tile, and the tile's start are spread over them, while two thousand workgroups are left; one
+// for new tokens.  131072 tokens of 12 rows of 30, forward: 74 us at 8 tokens, 59 at 16; 32768 tokens of 40 rows of 128: 143 us
+// at 8, 155 at 16.
+static int rot_tokens_per_wg(long long tokens, int heads, int groups, bool bwd) {
+    const long long t = tokens / 2048, want = (bwd ? 16LL : 8LL) * groups / (heads > 0 ? heads : 1);
+    const long long most = want < 4 ? 4 : want > ROT_TOKENS ? ROT_TOKENS : want;
+    return t < 1 ? 1 : t > most ? (int)most : (int)t;
+}
+// The widest piece that a call's sizes allow; its strides and addresses may ask for a narrower one.  (The backward's number of
+// workgroups has to be known before its buffers are there, so it follows from the sizes alone.)
+static int rot_widest(int D, int n, int dtype) {
+    int Q = dtype == DSW_F32 ? 4 : 8;
+    while (Q > 1 && (D % Q || n % Q)) Q >>= 1;
+    return Q;
+}
+static constexpr int rot_units_per_lane(int Q) { return Q == 2 ? 2 : Q == 1 ? 4 : 1; }
+// lanes of a row (narrow pieces: several units per lane, so that a row's fixed costs are paid by fewer lanes)
+static int rot_lanes_log(int D, int Q) {
+    int k = 0;
+    while ((1 << k) * rot_units_per_lane(Q) < (D + 2 * Q - 1) / (2 * Q)) ++k;
+    return k;
+}
+static int rot_tile(long long tokens, int heads, int D, int n, int dtype, bool bwd) {
+    return rot_tokens_per_wg(tokens, heads, ROT_THREADS >> rot_lanes_log(D, rot_widest(D, n, dtype)), bwd);
 }
 
 static bool operand_ok(const RotOperand &o, int heads, long long q, int size) {
@@ -362,8 +431,8 @@ static int rot_check(const char *who, RotArgs &a, int dtype, int B, bool bwd, in
         DSW_REQUIRE(h == 0 || (a.x[m].p && a.y[m].p && (!bwd || a.dy[m].p)), "%s: null pointer", who);
     }
     const int n = a.axes * a.pairs, size = dtype == DSW_F32 ? 4 : 2;
-    for (Q = dtype == DSW_F32 ? 4 : 8; Q > 1; Q >>= 1) {
-        bool ok = a.D % Q == 0 && n % Q == 0;
+    for (Q = rot_widest(a.D, n, dtype); Q > 1; Q >>= 1) {
+        bool ok = true;
         for (int m = 0; m < 2 && ok; ++m) {
             const int h = m ? a.Hkv : a.Hq;
             ok = operand_ok(a.x[m], h, Q, size) && operand_ok(a.y[m], h, Q, size) && (!bwd || operand_ok(a.dy[m], h, Q, size));
@@ -371,9 +440,8 @@ static int rot_check(const char *who, RotArgs &a, int dtype, int B, bool bwd, in
         if (ok) break;
     }
     a.units = (a.D + 2 * Q - 1) / (2 * Q);
-    a.rl_log = 0;
-    while ((1 << a.rl_log) < a.units && a.rl_log < 4) ++a.rl_log;
-    a.tpw = rot_tokens_per_wg(a.tokens);
+    a.rl_log = rot_lanes_log(a.D, Q);
+    a.tpw = rot_tile(a.tokens, a.Hq + a.Hkv, a.D, n, dtype, bwd);
     return DSW_OK;
 }
 
@@ -398,8 +466,8 @@ static int rot_dispatch(const RotArgs &a, int dtype, int Q, bool bwd, bool inter
     if (dtype == DSW_BF16 && Q == 8) return rot_launch<bf16_t, 8, 1>(a, bwd, interleaved, st);
     DSW_DISPATCH_DTYPE(dtype, T, {
         if (Q == 4) return rot_launch<T, 4, 1>(a, bwd, interleaved, st);
-        if (Q == 2) return rot_launch<T, 2, 2>(a, bwd, interleaved, st);
-        return rot_launch<T, 1, 4>(a, bwd, interleaved, st);
+        if (Q == 2) return rot_launch<T, 2, rot_units_per_lane(2)>(a, bwd, interleaved, st);
+        return rot_launch<T, 1, rot_units_per_lane(1)>(a, bwd, interleaved, st);
     });
     return DSW_OK;
 }
@@ -423,11 +491,13 @@ extern "C" int dsw_qk_norm_rotary_fwd(const void *q, const dsw_strides *sq, cons
     return rot_dispatch(a, dtype, Q, false, interleaved != 0, as_stream(stream));
 }
 
-extern "C" int dsw_qk_norm_rotary_blocks(int B, int L) {
+extern "C" int dsw_qk_norm_rotary_blocks(int dtype, int B, int L, int Hq, int Hkv, int D, int axes, int pairs) {
     const long long tokens = (long long)B * L;
-    if (B < 0 || L < 0 || tokens >= (1LL << 31)) return 0;
-    const int tpw = rot_tokens_per_wg(tokens);
-    const long long tiles = (tokens + tpw - 1) / tpw;
+    if (B < 0 || L < 0 || tokens >= (1LL << 31) || Hq < 0 || Hkv < 0 || (long long)Hq + Hkv > 4096 || D < 1 || D > ROT_MAX_D || axes < 0 ||
+        pairs < 0 || 2LL * axes * pairs > D)
+        return 0;
+    const int tile = rot_tile(tokens, Hq + Hkv, D, axes * pairs, dtype, true);
+    const long long tiles = (tokens + tile - 1) / tile;
     return (int)(tiles < ROT_BWD_BLOCKS ? tiles : ROT_BWD_BLOCKS);
 }
 

@@ -2470,7 +2470,8 @@ class _QKNormRotaryFn(torch.autograd.Function):
         dq, sdq, pdq = _head_rows(torch.empty(B, L, Hq, D, dtype=q.dtype, device=dev))
         dk, sdk, pdk = _head_rows(torch.empty(B, L, Hkv, D, dtype=q.dtype, device=dev))
         want_w = (wq is not None and ctx.needs_input_grad[2]) or (wk is not None and ctx.needs_input_grad[3])
-        blocks = _lib.load().dsw_qk_norm_rotary_blocks(B, L)
+        axes, pairs = (0, 0) if freqs is None else freqs.shape
+        blocks = _lib.load().dsw_qk_norm_rotary_blocks(dtype_code(q.dtype), B, L, Hq, Hkv, D, axes, pairs)
         partial = torch.empty(blocks, 2 * D, dtype=torch.float32, device=dev) if want_w and blocks else None
         if B * L:
             spec = _QKNormRotaryFn._spec(q, Hkv, wq, wk, freqs, positions, *ctx.settings)
