@@ -467,3 +467,120 @@ def test_qk_norm_rotary(cuda0, case, positions, dtype):
     with torch.no_grad():
         again = K.qk_norm_rotary(*[t.detach() for t in order], **kw)
     assert torch.equal(again[0], got["q"]) and torch.equal(again[1], got["k"])
+
+
+# ----------------------------------------------------------------------------------------------
+# the operators together: sequence.BandedMSA
+# ----------------------------------------------------------------------------------------------
+def _module_in_64_bits(mod, x, positions, lens=None):
+    """BandedMSA by plain tensor operations in the dtype of its (double) parameters"""
+    B, L, C = x.shape
+    h, g, d = mod.num_heads, mod.kv_heads, mod.head_dim
+    qkv = torch.nn.functional.linear(x, mod.qkv.weight, mod.qkv.bias).unflatten(-1, (h + 2 * g, d))
+    q, k, v = qkv.split((h, g, g), dim=2)
+    f = mod.rotary_freqs.double()
+    ang = (positions.double().view(-1, L, f.shape[0], 1) * f).flatten(-2)
+    q, k = (S.rotary(t, w, ang, f.numel(), mod.eps, False) for t, w in ((q, mod.q_norm), (k, mod.k_norm)))
+    rep = h // g
+    k, v = k.repeat_interleave(rep, 2), v.repeat_interleave(rep, 2)
+    s = torch.einsum("bihd,bjhd->bhij", q, k) * d ** -0.5
+    if mod.pe is not None:
+        M = mod.pe.max_distance
+        rel = (torch.arange(L)[None, :] - torch.arange(L)[:, None]).clamp(-M, M) + M
+        s = s + mod.pe.table()[mod.pe.buckets.long()[rel]].permute(2, 0, 1)
+    vis = torch.stack([S.visible(L, L, n, n, mod.window[0], mod.window[1], mod.sinks)[0] for n in (lens or [L] * B)])[:, None]
+    s = s.masked_fill(~vis, -math.inf)
+    p = torch.where(vis, torch.exp(s - s.amax(-1, keepdim=True).clamp(min=-1e300)), 0.0)
+    p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
+    z = torch.einsum("bhij,bjhd->bihd", p, v).reshape(B, L, C)
+    return torch.nn.functional.linear(z, mod.out_proj.weight, mod.out_proj.bias)
+
+
+def _module(**kw):
+    from visiontransformer_amd.sequence import BandedMSA
+    torch.manual_seed(3)
+    mod = BandedMSA(**kw)
+    with torch.no_grad():
+        for p in mod.parameters():
+            p.add_(torch.randn_like(p) * 0.1)
+    return mod
+
+
+@pytest.mark.parametrize("kw,L,lens", [
+    (dict(dim=180, num_heads=6, window=(40, 40), sinks=4, rotary_axes=2, num_buckets=16, max_distance=32), 144, None),
+    (dict(dim=128, num_heads=4, kv_heads=2, window=(60, 0), sinks=2, num_buckets=8, max_distance=64), 130, [130, 17]),
+    (dict(dim=64, num_heads=4, rotary_pairs=5), 70, [70, 0]),
+])
+def test_banded_msa_trains(cuda0, kw, L, lens):
+    """fp32: output and every gradient against double.  Both Linears are fp32 sums of dim products, the attention's bounds are
+    a few dozen roundings: 2^-24 * (2 dim + 400) of each tensor's norm is taken, some twenty times what errors of random
+    sign add up to."""
+    import copy
+    mod = _module(**kw)
+    ref = copy.deepcopy(mod).double()
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randn(2, L, kw["dim"], generator=gen)
+    g = torch.randn(2, L, kw["dim"], generator=gen)
+    axes = mod.rotary_axes
+    pos = torch.stack([torch.arange(L) // 12, torch.arange(L) % 12], -1) if axes == 2 else torch.arange(L)[:, None]
+    xd = x.double().requires_grad_()
+    yd = _module_in_64_bits(ref, xd, pos[None], lens)
+    want = torch.autograd.grad(yd, [xd] + list(ref.parameters()), g.double())
+    mod = mod.to(cuda0)
+    xg = x.to(cuda0).requires_grad_()
+    y = mod(xg, positions=pos.to(cuda0) if axes == 2 else None, lens=None if lens is None else torch.tensor(lens, device=cuda0))
+    got = torch.autograd.grad(y, [xg] + list(mod.parameters()), g.to(cuda0))
+    tol = 2.0 ** -24 * (2 * kw["dim"] + 400)
+    names = ["x"] + [n for n, _ in mod.named_parameters()]
+    for name, a, b in [("y", y, yd)] + list(zip(names, got, want)):
+        err = float((a.detach().double().cpu() - b.detach()).norm() / b.detach().norm().clamp(min=1e-30))
+        assert err <= tol, (name, err, tol)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_new_tokens_behind_a_cache_equal_the_whole_sequence(cuda0, dtype):
+    """a padded prompt, then tokens one by one (and three at once), against the module on the whole sequences.  fp32: both
+    ways compute the same sums in other orders; bf16: they differ by roundings of intermediates of 2^-8 each (projection,
+    norm, probabilities, result, projection)."""
+    from visiontransformer_amd.sequence import KVCache
+    mod = _module(dim=128, num_heads=4, kv_heads=2, window=(20, 0), sinks=2, num_buckets=8, max_distance=64).to(cuda0).to(dtype).eval()
+    assert mod.rotary_freqs.dtype == torch.float32
+    gen = torch.Generator().manual_seed(2)
+    lens, extra = [37, 50], 9
+    x = torch.randn(2, 50 + extra, 128, generator=gen).to(dtype).to(cuda0)
+    with torch.no_grad():
+        cache = KVCache(2, 70, 2, 32, dtype=dtype, device=cuda0)
+        cache.k.fill_(float("nan"))
+        cache.v.fill_(float("nan"))
+        first = mod(x[:, :50], lens=torch.tensor(lens, device=cuda0), cache=cache)
+        assert cache.lens.tolist() == lens
+        steps, at = [], 0
+        for n in (1, 1, 3, 1, 3):
+            new = torch.stack([x[b, lens[b] + at:lens[b] + at + n] for b in range(2)])
+            steps.append(mod(new, cache=cache))
+            at += n
+        steps = torch.cat(steps, 1)
+        tol = 2e-5 if dtype == FP else 5 * 2.0 ** -8
+        for b in range(2):
+            whole = mod(x[b:b + 1, :lens[b] + extra])[0]
+            for got, want in ((first[b, :lens[b]], whole[:lens[b]]), (steps[b], whole[lens[b]:])):
+                err = float((got.double() - want.double()).norm() / want.double().norm())
+                assert err <= tol, (b, err)
+        with pytest.raises(RuntimeError, match="capacity"):
+            mod(x[:, :20], cache=cache)
+    with pytest.raises(RuntimeError, match="inference"):
+        mod(x[:, :1], cache=KVCache(2, 4, 2, 32, dtype=dtype, device=cuda0))
+
+
+def test_banded_msa_under_autocast(cuda0):
+    """fp32 parameters, bf16 autocast, a training step: finite, close to fp32 (2e-2, the bar of the package's bf16 runs)"""
+    mod = _module(dim=180, num_heads=6, window=(64, 64), sinks=4, num_buckets=16, max_distance=32).to(cuda0)
+    x = torch.randn(2, 200, 180, generator=torch.Generator().manual_seed(4)).to(cuda0).requires_grad_()
+    g = torch.randn(2, 200, 180, generator=torch.Generator().manual_seed(5)).to(cuda0)
+    outs = []
+    for on in (False, True):
+        with torch.autocast("cuda", dtype=BF, enabled=on):
+            y = mod(x)
+        outs.append([y] + list(torch.autograd.grad(y, [x] + list(mod.parameters()), g.to(y.dtype))))
+    for a, b in zip(*outs):
+        assert float((a.double() - b.double()).norm() / a.double().norm()) <= 2e-2

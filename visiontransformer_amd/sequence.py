@@ -1,0 +1,165 @@
+"""Attention over token sequences: modules over functional.qk_norm_rotary and functional.band_attention.
+
+The windowed modules of dswin.py and msft.py let a token see its 8x8 or 16x16 window.  BandedMSA stands beside them for
+tokens that have to see further: the tokens of a map in raster order (or of any sequence), each seeing the tokens up to
+`left` before and `right` behind it and a few first tokens (registers, sinks) that stay visible; with queries and keys
+normalised per head and rotated by position, and a learned bias by distance.  No counterpart in the reference.
+"""
+import torch
+from torch import nn
+
+from . import functional as K
+
+
+def bucket_of_distance(num_buckets, max_distance, bidirectional):
+    """bucket of every distance key - query from -max_distance to max_distance (farther ones are clipped): half of a side's
+    buckets count the nearest distances one by one, the other half grow with the logarithm up to max_distance.  Both
+    directions get half of the buckets each; one-sided, keys ahead fall into bucket 0.  The borders are decided in whole
+    numbers: bucket near + k begins at the smallest n with (n / near)^(side - near) >= (max_distance / near)^k."""
+    side = num_buckets // 2 if bidirectional else num_buckets
+    near = side // 2
+    if near < 1 or side <= near or (bidirectional and num_buckets % 2) or max_distance <= near:
+        raise ValueError("bucket_of_distance: %d buckets up to distance %d%s" % (num_buckets, max_distance, ", both directions" if bidirectional else ""))
+    of = list(range(near))
+    k = 0
+    for n in range(near, max_distance + 1):
+        while near + k + 1 < side and n ** (side - near) * near ** (k + 1) >= max_distance ** (k + 1) * near ** (side - near):
+            k += 1
+        of.append(near + k)
+    behind = [of[-r] for r in range(-max_distance, 1)]
+    ahead = [of[r] + side if bidirectional else 0 for r in range(1, max_distance + 1)]
+    return torch.tensor(behind + ahead, dtype=torch.int32)
+
+
+def rotary_frequencies(pairs, axes=1, base=10000.0):
+    """fp32 [axes, pairs] radians per step: base^(-i / pairs) on every axis"""
+    f = float(base) ** (-torch.arange(pairs, dtype=torch.float64) / max(pairs, 1))
+    return f.float().expand(axes, pairs).contiguous()
+
+
+class BucketedPositionBias(nn.Module):
+    """Bias table [num_buckets, heads] + int32 bucket map over distances, the counterpart of
+    dswin.RelativePositionalEncoding for sequences.  band_attention reads both (`table()`, `buckets`) and never forms the
+    expanded bias; forward() returns it, [1, heads, q_len, k_len], for callers that want it (the queries being the last
+    q_len of k_len tokens)."""
+
+    def __init__(self, num_heads, num_buckets=32, max_distance=128, bidirectional=True):
+        super().__init__()
+        self.position_bias_table = nn.Parameter(torch.zeros(num_buckets, num_heads))
+        self.register_buffer("buckets", bucket_of_distance(num_buckets, max_distance, bidirectional), persistent=False)
+        self.max_distance = max_distance
+        nn.init.trunc_normal_(self.position_bias_table, std=.02, a=-2., b=2.)
+
+    def table(self):
+        return self.position_bias_table
+
+    def forward(self, q_len, k_len):
+        dev = self.buckets.device
+        rel = torch.arange(k_len, device=dev)[None, :] - torch.arange(k_len - q_len, k_len, device=dev)[:, None]
+        M = self.max_distance
+        return self.position_bias_table[self.buckets.long()[rel.clamp(-M, M) + M]].permute(2, 0, 1).unsqueeze(0)
+
+
+class KVCache:
+    """Keys and values of up to `capacity` tokens per sequence, [B, heads, capacity, D] (a head's rows together), with the
+    number of tokens of each sequence on the device.  Rows behind a sequence are never read, so nothing is cleared.
+
+    append() writes new tokens behind what each sequence holds, without a host synchronisation; the host keeps only the
+    largest count, and refuses what would not fit.  Inside a captured graph the device counts advance with every replay
+    and the host's does not: a loop of replays has to count for itself and stay within `capacity`."""
+
+    def __init__(self, batch, capacity, num_heads, head_dim, dtype=torch.bfloat16, device="cuda"):
+        self.k = torch.empty(batch, num_heads, capacity, head_dim, dtype=dtype, device=device)
+        self.v = torch.empty_like(self.k)
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.capacity = capacity
+        self.longest = 0
+
+    def append(self, k, v, lens=None):
+        """k, v [B, n, heads, D]; lens int [B] (device): how many of the n tokens count per sequence, None: all of them"""
+        B, n = k.shape[:2]
+        if (k.shape != v.shape or B != self.k.shape[0] or k.shape[2:] != (self.k.shape[1], self.k.shape[3]) or k.dtype != self.k.dtype
+                or v.dtype != self.k.dtype):
+            raise RuntimeError("visiontransformer_amd: KVCache: %s %s tokens for a cache of %s %s" % (tuple(k.shape), k.dtype, tuple(self.k.shape), self.k.dtype))
+        if self.longest + n > self.capacity:
+            raise RuntimeError("visiontransformer_amd: KVCache: %d + %d tokens exceed the capacity of %d" % (self.longest, n, self.capacity))
+        if n:
+            # (tokens beyond a sequence's count go to places behind it, which the next ones overwrite)
+            place = (self.lens.long()[:, None] + torch.arange(n, device=self.lens.device)).clamp(max=self.capacity - 1)
+            rows = torch.arange(B, device=self.lens.device)[:, None]
+            self.k.transpose(1, 2)[rows, place] = k
+            self.v.transpose(1, 2)[rows, place] = v
+        self.lens += n if lens is None else lens.to(torch.int32).clamp(0, n)
+        self.longest += n
+        return self
+
+    def tokens(self):
+        """k, v as [B, capacity, heads, D] views"""
+        return self.k.transpose(1, 2), self.v.transpose(1, 2)
+
+
+class BandedMSA(nn.Module):
+    """Multi-head attention of a token sequence over a sliding window with sinks: qkv Linear, per-head norm and rotation of
+    queries and keys (one kernel), attention (one kernel), out_proj.
+
+    window = (left, right), None: no limit; sinks: first tokens that stay visible.  kv_heads < num_heads: query heads share
+    key heads.  qk_norm: learned RMS norm of every head's query and key rows.  rotary_axes: 0 (no rotation), 1 (position in
+    the sequence) or more (coordinates, e.g. row and column); rotary_pairs pairs of columns per axis (default: as many as
+    fit).  num_buckets > 0: learned bias by distance (BucketedPositionBias; one-sided when right is 0)."""
+
+    def __init__(self, dim, num_heads=4, kv_heads=None, window=(None, None), sinks=0, qk_norm=True, rotary_axes=1, rotary_pairs=None,
+                 rotary_base=10000.0, num_buckets=0, max_distance=128, eps=1e-6):
+        super().__init__()
+        kv_heads = num_heads if kv_heads is None else kv_heads
+        assert dim % num_heads == 0, f"dim ({dim}) must be divisible by num_heads ({num_heads})"
+        assert num_heads % kv_heads == 0, f"num_heads ({num_heads}) must be a multiple of kv_heads ({kv_heads})"
+        self.num_heads, self.kv_heads, self.head_dim = num_heads, kv_heads, dim // num_heads
+        self.window, self.sinks, self.eps = tuple(window), sinks, eps
+        self.qkv = nn.Linear(dim, (num_heads + 2 * kv_heads) * self.head_dim)
+        self.out_proj = nn.Linear(dim, dim)
+        self.q_norm = nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
+        self.k_norm = nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
+        assert qk_norm or not rotary_axes, "the rotation runs in the kernel of the norm (qk_norm)"
+        self.rotary_axes = rotary_axes
+        pairs = (self.head_dim // (2 * rotary_axes) if rotary_pairs is None else rotary_pairs) if rotary_axes else 0
+        self.register_buffer("rotary_freqs", rotary_frequencies(pairs, rotary_axes, rotary_base) if pairs else None, persistent=False)
+        self.pe = BucketedPositionBias(num_heads, num_buckets, max_distance, bidirectional=window[1] != 0) if num_buckets else None
+
+    def _apply(self, fn, *args, **kwargs):
+        # (module.to(bfloat16) and the like leave the frequencies in fp32: the angles of far positions need them)
+        freqs = self.rotary_freqs
+        super()._apply(fn, *args, **kwargs)
+        if freqs is not None and self.rotary_freqs.dtype != torch.float32:
+            self.rotary_freqs = freqs.to(self.rotary_freqs.device)
+        return self
+
+    def forward(self, x, positions=None, lens=None, cache=None):
+        """x [B, L, C] -> [B, L, C].  positions: int [L] / [B, L] (rotary_axes 1) or [L, A] / [B, L, A] (A axes), None: the
+        token's index (behind what the cache holds).  lens int [B]: tokens of each sequence of a padded batch; rows behind
+        them come out as out_proj's bias.  cache (a KVCache, inference): the tokens are appended to it and attend to all that
+        it holds; with lens, the batch must be as long as its longest sequence."""
+        B, L, C = x.shape
+        h, g, d = self.num_heads, self.kv_heads, self.head_dim
+        qkv = K.linear(x, self.qkv).unflatten(-1, (h + 2 * g, d))
+        q, k, v = qkv.split((h, g, g), dim=2)
+        if self.q_norm is not None:
+            if positions is None and cache is not None and self.rotary_freqs is not None:
+                positions = cache.lens.long()[:, None] + torch.arange(L, device=x.device)
+                if self.rotary_axes > 1:
+                    raise RuntimeError("visiontransformer_amd: BandedMSA: coordinates of new tokens behind a cache have to be given")
+            freqs = self.rotary_freqs
+            if freqs is not None and self.rotary_axes == 1:
+                freqs = freqs[0]
+            q, k = K.qk_norm_rotary(q, k, self.q_norm, self.k_norm, freqs, positions if freqs is not None else None, eps=self.eps)
+        elif positions is not None:
+            raise RuntimeError("visiontransformer_amd: BandedMSA: positions given to a module without rotation")
+        q_lens = k_lens = lens
+        if cache is not None:
+            if torch.is_grad_enabled() and qkv.requires_grad:
+                raise RuntimeError("visiontransformer_amd: BandedMSA: a cache is for inference (torch.no_grad())")
+            cache.append(k, v, lens)
+            k, v = cache.tokens()
+            k_lens = cache.lens
+        bias = (None, None) if self.pe is None else (self.pe.table(), self.pe.buckets)
+        z = K.band_attention(q, k, v, window=self.window, sinks=self.sinks, q_lens=q_lens, k_lens=k_lens, bias_table=bias[0], bias_buckets=bias[1])
+        return K.linear(z.reshape(B, L, C), self.out_proj)
