@@ -95,12 +95,12 @@ def attention(q, k, v, left, right, sinks, scale, q_lens=None, k_lens=None, tabl
             delta = (G * O).sum(-1, keepdim=True)
             dS = P * (dP - delta)
             # how far delta may be off: with the rounded result, and with the fp32 copy that a wanted table gradient keeps
-            # (probabilities in two 16-bit parts: u^2)
+            # (probabilities in three parts of 8 bits: u^3)
             def ds_bound(up, ur):
                 d_delta = (G.abs() * ((up + rel_e) * A + ur * O.abs() + 8 * F * A)).sum(-1, keepdim=True) + (D + 4) * F * (G * O).abs().sum(-1, keepdim=True)
                 return P * d_delta + rel_e * P * (dP.abs() + delta.abs()) + (D + 8) * F * P * absGV
             exact = table is not None and table_grad and dtype != torch.float32
-            raw = ds_bound(u * u, 0.0) if exact else ds_bound(u, uo)
+            raw = ds_bound(u ** 3, 0.0) if exact else ds_bound(u, uo)
             bS = u * dS.abs() + raw
             nrow = Lq * (Hq // Hkv)
             res["dq"][0][b, :, h] = dS @ Kb * scale

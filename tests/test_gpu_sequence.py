@@ -247,6 +247,27 @@ def test_gradients_against_differences(cuda0):
     assert abs(got - slope) <= size * 64 * 2.0 ** -24 + 1e-6 * abs(slope), (got, slope)
 
 
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("D", [7, 30, 64, 128])
+def test_rows_that_see_one_key_have_no_gradient_of_their_scores(cuda0, dtype, D):
+    """softmax of one number is constant: dq, dk and the bias' gradient are zeros, not what roundings leave"""
+    K = _K()
+    for L, window in ((1, (None, None)), (150, (0, 0))):
+        q, k, v, dout, gen = _inputs((2, L, 4, D), (2, L, 2, D), dtype, 6)
+        table = torch.randn(8, 4, generator=gen).to(cuda0).requires_grad_()
+        bmap = torch.tensor(S.bucket_map(8, 16, False), dtype=torch.int32, device=cuda0)
+        leaves = [t.to(cuda0).requires_grad_() for t in (q, k, v)] + [table]
+        for kw in (dict(bias_table=table, bias_buckets=bmap), {}):
+            out = K.band_attention(*leaves[:3], window=window, **kw)
+            assert torch.equal(out, leaves[2].repeat_interleave(2, 2))
+            grads = torch.autograd.grad(out, leaves if kw else leaves[:3], dout.to(cuda0))
+            assert all(float(g.abs().max()) == 0.0 for i, g in enumerate(grads) if i != 2)
+            t = None if not kw else table.detach().double().cpu()
+            ref = S.attention(q.double(), k.double(), v.double(), *window, 0, D ** -0.5, table=t, buckets=None if t is None else bmap.cpu(),
+                              dout=dout.double(), dtype=dtype)
+            _within("dv", grads[2], *ref["dv"])   # (a probability of 1 is off by the rounding of its logit, which may be any size)
+
+
 def test_shared_heads_and_broadcast_inputs(cuda0):
     K = _K()
     gen = torch.Generator().manual_seed(2)

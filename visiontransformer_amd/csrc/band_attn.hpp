@@ -85,13 +85,6 @@ __device__ __forceinline__ float band_sum(const band_t<float>::frag &f, float l)
     return l + (((f.lo.x + f.lo.y) + (f.lo.z + f.lo.w)) + ((f.hi.x + f.hi.y) + (f.hi.z + f.hi.w)));
 }
 
-// element e of a fragment (e known at compile time)
-__device__ __forceinline__ float band_element(const uint4 &f, int e) {
-    const uint32_t w = (&f.x)[e >> 1];
-    return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
-}
-__device__ __forceinline__ float band_element(const band_t<float>::frag &f, int e) { return e < 4 ? (&f.lo.x)[e] : (&f.hi.x)[e - 4]; }
-
 __device__ __forceinline__ f32x16 band_zero() {
     f32x16 z;
 #pragma unroll
@@ -108,13 +101,15 @@ __device__ __forceinline__ void band_pack(const f32x16 &s, int c, band_t<float>:
     f.lo = make_float4(s[8 * c], s[8 * c + 1], s[8 * c + 2], s[8 * c + 3]);
     f.hi = make_float4(s[8 * c + 4], s[8 * c + 5], s[8 * c + 6], s[8 * c + 7]);
 }
-// what the rounding of band_pack left behind, rounded in its turn: the two together carry 16 bits
-__device__ __forceinline__ uint32_t band_rest2(float a, float b, uint32_t rounded) {
-    return pack_bf16(a - __uint_as_float(rounded << 16), b - __uint_as_float(rounded & 0xffff0000u));
+// what the rounding of v to a fragment left behind: subtracted from v, and rounded in its turn; with two such rests a
+// fragment carries the 24 bits of fp32
+__device__ __forceinline__ uint32_t band_rest2(float &a, float &b, uint32_t rounded) {
+    a -= __uint_as_float(rounded << 16);
+    b -= __uint_as_float(rounded & 0xffff0000u);
+    return pack_bf16(a, b);
 }
-__device__ __forceinline__ void band_pack_rest(const f32x16 &s, int c, const uint4 &f, uint4 &rest) {
-    rest = make_uint4(band_rest2(s[8 * c], s[8 * c + 1], f.x), band_rest2(s[8 * c + 2], s[8 * c + 3], f.y),
-                      band_rest2(s[8 * c + 4], s[8 * c + 5], f.z), band_rest2(s[8 * c + 6], s[8 * c + 7], f.w));
+__device__ __forceinline__ void band_rest(float *v, const uint4 &f, uint4 &rest) {
+    rest = make_uint4(band_rest2(v[0], v[1], f.x), band_rest2(v[2], v[3], f.y), band_rest2(v[4], v[5], f.z), band_rest2(v[6], v[7], f.w));
 }
 
 // ---- global memory: 8 consecutive elements of a row, zero past D -------------------------------------------------

@@ -293,25 +293,39 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     }
     const size_t stat = ((size_t)b * a.Hq + h) * a.Lq + i;
     const float nl = row_on ? -a.lse[stat] : -INFINITY;
-    // delta = dout . out, from the result before its rounding where that was kept
+    // delta = dout . out, from the result before its rounding where that was kept (in three parts of 8 bits).  It is the
+    // diagonal of a product formed like dout v^T below: for a row that sees a single key, whose result is that key's value,
+    // the two are then the same number and dS is exactly zero.
     float del = 0.f;
-    if (row_on) {
+    {
+        f32x16 d = band_zero();
         const T *const orow = band_row<T>(a.out, b, i, h);
         const float *const o32 = a.out32 ? a.out32 + (((size_t)b * a.Lq + i) * a.Hq + h) * D : nullptr;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int col = 16 * c + 8 * hh;
-            if (o32) {
+            if constexpr (DTABLE && sizeof(T) == 2) {
+                float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) del = __builtin_fmaf(band_element(gf[c], e), col + e < D ? o32[col + e] : 0.f, del);
+                for (int e = 0; e < 8; ++e) v[e] = row_on && col + e < D ? o32[col + e] : 0.f;
+                uint4 part = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])), next;
+                d = band_mma(part, gf[c], d);
+                band_rest(v, part, next);
+                d = band_mma(next, gf[c], d);
+                band_rest(v, next, part);
+                d = band_mma(part, gf[c], d);
             } else {
-                const auto of = band_load8<MODE>(orow, col, D);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) del = __builtin_fmaf(band_element(gf[c], e), band_element(of, e), del);
+                typename band_t<T>::frag of;
+                band_clear(of);
+                if (row_on) of = band_load8<MODE>(orow, col, D);
+                d = band_mma(of, gf[c], d);
             }
         }
+        float mine = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mine = rho(r) + 4 * hh == l31 ? d[r] : mine;
+        del = mine + __shfl_xor(mine, 32, 64);  // (in one of the two halves, zero in the other)
     }
-    del += __shfl_xor(del, 32, 64);
     if (row_on && hh == 0 && wave < ROWS / 32) a.delta[stat] = del;
     f32x16 dq[DP / 32];
 #pragma unroll
@@ -578,6 +592,7 @@ extern "C" int dsw_band_attn_bwd(const dsw_band_desc *d, const void *q, const ds
         return rc;
     DSW_REQUIRE(no_rows || lse, "%s: null lse", who);
     DSW_REQUIRE(d_table == nullptr || a.table, "%s: a gradient for a table that is not there", who);
+    DSW_REQUIRE(d_table == nullptr || no_rows || d->dtype == DSW_F32 || out32, "%s: the table's gradient needs the forward's out32", who);
     const size_t need = dsw_band_attn_bwd_workspace(d);
     DSW_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "%s: workspace of %zu bytes, %zu are needed", who, workspace_bytes, need);
     a.lse = const_cast<float *>(lse);

@@ -167,17 +167,25 @@ __global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof
                     for (int r = 0; r < 16; ++r) s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], cs, shift));
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        typename band_t<T>::frag pf, rf;
+                        typename band_t<T>::frag pf;
                         band_pack(s[u], k, pf);
                         l = band_sum(pf, l);
-                        if constexpr (EXACT) {
-                            band_pack_rest(s[u], k, pf, rf);
-                            l = band_sum(rf, l);
-                        }
 #pragma unroll
-                        for (int db = 0; db < DP / 32; ++db) {
-                            o[db] = band_mma(vf[k][db], pf, o[db]);
-                            if constexpr (EXACT) o[db] = band_mma(vf[k][db], rf, o[db]);
+                        for (int db = 0; db < DP / 32; ++db) o[db] = band_mma(vf[k][db], pf, o[db]);
+                        if constexpr (EXACT) {  // the probabilities' other 16 bits
+                            uint4 rf;
+                            float rest[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) rest[e] = s[u][8 * k + e];
+                            band_rest(rest, pf, rf);
+                            l = band_sum(rf, l);
+#pragma unroll
+                            for (int db = 0; db < DP / 32; ++db) o[db] = band_mma(vf[k][db], rf, o[db]);
+                            uint4 rf2;
+                            band_rest(rest, rf, rf2);
+                            l = band_sum(rf2, l);
+#pragma unroll
+                            for (int db = 0; db < DP / 32; ++db) o[db] = band_mma(vf[k][db], rf2, o[db]);
                         }
                     }
                 }
