@@ -2409,6 +2409,19 @@ def _head_rows(t):
     return t, ctypes.byref(_lib.Strides(b if nb > 1 else 0, l if nl > 1 else 0, h if nh > 1 else 0)), t.data_ptr()
 
 
+def _new_rows(B, L, H, D, dtype, device):
+    """a new [B, L, H, D] tensor, with what _head_rows gives for it"""
+    t = torch.empty(B, L, H, D, dtype=dtype, device=device)
+    return t, ctypes.byref(_lib.Strides(L * H * D if B > 1 else 0, H * D if L > 1 else 0, D if H > 1 else 0)), t.data_ptr()
+
+
+def _as_f32(t):
+    """t's values as a contiguous fp32 tensor (t itself where it is one)"""
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().float().contiguous()
+
+
 def _same_kind(who, named):
     """all tensors 4-D, of one supported dtype, on one GPU"""
     first = next(iter(named.values()))
@@ -2418,7 +2431,7 @@ def _same_kind(who, named):
             _fail(who, "%s must be [batch, tokens, heads, head dim], got %s" % (name, tuple(t.shape)))
         if t.dtype != first.dtype or t.device != first.device:
             _fail(who, "%s is %s on %s, the others %s on %s" % (name, t.dtype, t.device, first.dtype, first.device))
-    dtype_code(first.dtype)
+    dtype_code(first.dtype)   # (raises for types that are not built)
 
 
 def _device_ints(who, name, t, device, shapes):
@@ -2446,9 +2459,9 @@ class _QKNormRotaryFn(torch.autograd.Function):
         Hkv, dev = k.shape[2], q.device
         q, sq, pq = _head_rows(q)
         k, sk, pk = _head_rows(k)
-        wq, wk = (None if w is None else w.detach().float().contiguous() for w in (q_weight, k_weight))
-        oq, soq, poq = _head_rows(torch.empty(B, L, Hq, D, dtype=q.dtype, device=dev))
-        ok, sok, pok = _head_rows(torch.empty(B, L, Hkv, D, dtype=q.dtype, device=dev))
+        wq, wk = _as_f32(q_weight), _as_f32(k_weight)
+        oq, soq, poq = _new_rows(B, L, Hq, D, q.dtype, dev)
+        ok, sok, pok = _new_rows(B, L, Hkv, D, q.dtype, dev)
         if B * L:
             spec = _QKNormRotaryFn._spec(q, Hkv, wq, wk, freqs, positions, eps, interleaved)
             _call_on(dev, "dsw_qk_norm_rotary_fwd", pq, sq, pk, sk, *spec, poq, soq, pok, sok, stream(dev))
@@ -2467,8 +2480,8 @@ class _QKNormRotaryFn(torch.autograd.Function):
         _, sk, pk = _head_rows(k)
         dyq, sdyq, pdyq = _head_rows(dyq.to(q.dtype))
         dyk, sdyk, pdyk = _head_rows(dyk.to(q.dtype))
-        dq, sdq, pdq = _head_rows(torch.empty(B, L, Hq, D, dtype=q.dtype, device=dev))
-        dk, sdk, pdk = _head_rows(torch.empty(B, L, Hkv, D, dtype=q.dtype, device=dev))
+        dq, sdq, pdq = _new_rows(B, L, Hq, D, q.dtype, dev)
+        dk, sdk, pdk = _new_rows(B, L, Hkv, D, q.dtype, dev)
         want_w = (wq is not None and ctx.needs_input_grad[2]) or (wk is not None and ctx.needs_input_grad[3])
         axes, pairs = (0, 0) if freqs is None else freqs.shape
         blocks = _lib.load().dsw_qk_norm_rotary_blocks(dtype_code(q.dtype), B, L, Hq, Hkv, D, axes, pairs)
@@ -2511,16 +2524,32 @@ def qk_norm_rotary(q, k, q_weight=None, k_weight=None, freqs=None, positions=Non
         if freqs.dim() not in (1, 2) or freqs.dtype != torch.float32 or freqs.device != q.device:
             _fail(who, "freqs must be fp32 [pairs] or [axes, pairs] on %s, got %s %s on %s" % (q.device, freqs.dtype, tuple(freqs.shape), freqs.device))
         flat = freqs.dim() == 1
-        freqs = freqs.detach().reshape((1, -1) if flat else freqs.shape).contiguous()
+        if flat or freqs.requires_grad or not freqs.is_contiguous():
+            freqs = freqs.detach().reshape((1, -1) if flat else freqs.shape).contiguous()
         A = freqs.shape[0]
         if 2 * freqs.numel() > D:
             _fail(who, "%d pairs on %d axes need more than the %d columns of a head" % (freqs.shape[1], A, D))
         positions = _device_ints(who, "positions", positions, q.device, ((L,), (B, L)) if flat else ((L, A), (B, L, A)))
-        if positions is not None:
+        if positions is not None and (flat or not positions.is_contiguous()):
             positions = (positions.unsqueeze(-1) if flat else positions).contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         return _QKNormRotaryFn.apply(q, k, q_weight, k_weight, freqs, positions, float(eps), bool(interleaved))
     return _QKNormRotaryFn.forward(_NO_GRAD, q, k, q_weight, k_weight, freqs, positions, float(eps), bool(interleaved))
+
+
+_WORKSPACE_BYTES = {}
+
+
+def _workspace(way, desc):
+    """bytes of workspace of a call, by its sizes alone"""
+    key = (way, desc.dtype, desc.B, desc.Lq, desc.Lk, desc.Hq, desc.Hkv, desc.D, desc.left, desc.right, desc.sinks, bool(desc.bias_table),
+           desc.max_distance)
+    n = _WORKSPACE_BYTES.get(key)
+    if n is None:
+        if len(_WORKSPACE_BYTES) > 4096:     # (sequences of ever new lengths)
+            _WORKSPACE_BYTES.clear()
+        n = _WORKSPACE_BYTES[key] = int(getattr(_lib.load(), "dsw_band_attn_%s_workspace" % way)(ctypes.byref(desc)))
+    return n
 
 
 class _BandAttnFn(torch.autograd.Function):
@@ -2537,8 +2566,8 @@ class _BandAttnFn(torch.autograd.Function):
         q, sq, pq = _head_rows(q)
         k, sk, pk = _head_rows(k)
         v, sv, pv = _head_rows(v)
-        tab = None if table is None else table.detach().float().contiguous()
-        out, so, po = _head_rows(torch.empty(B, Lq, Hq, D, dtype=q.dtype, device=dev))
+        tab = _as_f32(table)
+        out, so, po = _new_rows(B, Lq, Hq, D, q.dtype, dev)
         settings = (left, right, sinks, scale)
         desc = _BandAttnFn._desc(q, k, tab, buckets, q_lens, k_lens, *settings)
         train = any(ctx.needs_input_grad[:4])
@@ -2546,7 +2575,7 @@ class _BandAttnFn(torch.autograd.Function):
         lse = torch.empty(B, Hq, Lq, dtype=torch.float32, device=dev) if train else None
         out32 = torch.empty(B, Lq, Hq, D, dtype=torch.float32, device=dev) if exact else None
         if B * Lq * Hq:
-            n = 0 if exact else int(_lib.load().dsw_band_attn_fwd_workspace(ctypes.byref(desc)))
+            n = 0 if exact else _workspace("fwd", desc)
             ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
             _call_on(dev, "dsw_band_attn_fwd", ctypes.byref(desc), pq, sq, pk, sk, pv, sv, po, so, ptr(lse), ptr(out32), ptr(ws), n, stream(dev))
         if train:
@@ -2560,7 +2589,8 @@ class _BandAttnFn(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, tab, buckets, q_lens, k_lens, out, out32, lse = ctx.saved_tensors
         dev = q.device
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v)]
+        made = [_new_rows(*t.shape, t.dtype, dev) for t in (q, k, v)]
+        grads = [t[0] for t in made]
         d_tab = torch.empty_like(tab) if tab is not None and ctx.needs_input_grad[3] else None
         if q.shape[0] * q.shape[2] * max(q.shape[1], k.shape[1]):
             operands = []
@@ -2569,10 +2599,10 @@ class _BandAttnFn(torch.autograd.Function):
             operands.append(ptr(out32))
             dout, s, p = _head_rows(dout.to(q.dtype))
             operands += [p, s, ptr(lse)]
-            for t in grads:
-                operands += _head_rows(t)[:0:-1]
+            for t in made:
+                operands += t[:0:-1]
             desc = _BandAttnFn._desc(q, k, tab, buckets, q_lens, k_lens, *ctx.settings)
-            n = int(_lib.load().dsw_band_attn_bwd_workspace(ctypes.byref(desc)))
+            n = _workspace("bwd", desc)
             ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
             _call_on(dev, "dsw_band_attn_bwd", ctypes.byref(desc), *operands, ptr(d_tab), ptr(ws), n, stream(dev))
         elif d_tab is not None:
