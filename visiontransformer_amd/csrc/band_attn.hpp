@@ -113,16 +113,20 @@ __device__ __forceinline__ void band_rest(float *v, const uint4 &f, uint4 &rest)
 }
 
 // ---- global memory: 8 consecutive elements of a row, zero past D -------------------------------------------------
-struct __attribute__((packed, aligned(2))) band_u16x8 { uint32_t x, y, z, w; };   // (unaligned vector accesses are legal)
-struct __attribute__((packed, aligned(4))) band_f32x4 { float x, y, z, w; };
+struct __attribute__((packed, aligned(4))) band_u16x8 { uint32_t x, y, z, w; };
+struct __attribute__((packed, aligned(4))) band_f32x4 { float x, y, z, w; };   // (unaligned vector accesses are legal)
 
 template <int MODE> __device__ __forceinline__ uint4 band_load8(const bf16_t *row, int col, int D) {
     if constexpr (MODE == 0) return col < D ? *reinterpret_cast<const uint4 *>(row + col) : make_uint4(0u, 0u, 0u, 0u);
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = col + 2 * i < D ? row[col + 2 * i] : 0u, hi = col + 2 * i + 1 < D ? row[col + 2 * i + 1] : 0u;
-        w[i] = lo | (hi << 16);
+        if constexpr (MODE == 1) {
+            w[i] = col + 2 * i < D ? *reinterpret_cast<const uint32_t *>(row + col + 2 * i) : 0u;
+        } else {
+            const uint32_t lo = col + 2 * i < D ? row[col + 2 * i] : 0u, hi = col + 2 * i + 1 < D ? row[col + 2 * i + 1] : 0u;
+            w[i] = lo | (hi << 16);
+        }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
@@ -140,7 +144,7 @@ template <int MODE> __device__ __forceinline__ band_t<float>::frag band_load8(co
     f.hi = make_float4(v[4], v[5], v[6], v[7]);
     return f;
 }
-// the piece at column `at` itself, at any alignment, all 8 elements inside the row
+// the piece at p, all 8 elements inside the row
 __device__ __forceinline__ uint4 band_piece(const bf16_t *p) {
     const band_u16x8 t = *reinterpret_cast<const band_u16x8 *>(p);
     return make_uint4(t.x, t.y, t.z, t.w);
@@ -157,14 +161,13 @@ __device__ __forceinline__ void band_clear(band_t<float>::frag &f) { f.lo = f4ze
 
 template <int MODE> __device__ __forceinline__ void band_store8(bf16_t *row, int col, const float *v, int D) {
     const uint4 u = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-    if (MODE == 0 || col + 8 <= D) {
-        if (MODE != 0) {
-            band_u16x8 t;
-            t.x = u.x, t.y = u.y, t.z = u.z, t.w = u.w;
-            *reinterpret_cast<band_u16x8 *>(row + col) = t;
-        } else if (col < D) {
-            *reinterpret_cast<uint4 *>(row + col) = u;
-        }
+    if constexpr (MODE == 0) {
+        if (col < D) *reinterpret_cast<uint4 *>(row + col) = u;
+    } else if constexpr (MODE == 1) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (col + 2 * i < D) *reinterpret_cast<uint32_t *>(row + col + 2 * i) = w[i];
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
