@@ -5,13 +5,18 @@
 //   (c, c + axes * pairs), or (2c, 2c + 1) when interleaved, and turns by pos[token][a] * freqs[a][i]
 //   backward: du = dy turned back, dw = sum over rows of du * x * r, dn = du * w, dx = r (dn - x r mean(dn * x r))
 //
-// Memory-bound: forward reads x and writes y, backward reads x and dy and writes dx, with some 20 vector instructions
-// per 16 bytes.  The angles need the accurate path (positions in the millions: the product with the frequency is
+// Forward reads x and writes y, backward reads x and dy and writes dx: bound by memory where pieces of 16 bytes are
+// possible (4 sequences of 8192 tokens, 40 rows of 128, bf16: 671 MB in 134 us, 5.0 TB/s, the rate of a plain copy), by
+// vector instructions and by the number of narrow accesses where they are not (heads of 30, 131072 tokens of 12 rows:
+// forward 189 MB in 48 us, backward 283 MB in 80 us, 3.5 to 3.9 TB/s).  The angles need the accurate path (positions in
+// the millions: the product with the frequency is
 // taken in 64 bits and reduced to a part of one turn before sine and cosine), which costs more than a row's norm; they
 // are the same for all heads of a token, so a workgroup takes all heads of a few tokens and keeps the sines and cosines
 // in LDS.  A row is held by RL lanes in units of two Q-element pieces, chosen so that both columns of a pair are
 // in one lane: the rotation needs no exchange, the norm log2(RL) of them.  Q is the widest piece (16 bytes at most)
-// that the head dim, the pair count, the strides and the addresses allow; Q = 1 takes any of them.
+// that the head dim, the pair count, the strides and the addresses allow; Q = 1 takes any of them.  Loads and sums run
+// without branches, over masked registers: with branches around the pieces that a row does not have, and the weights'
+// sums joined by exchanges, the two kernels took 57 and 107 us.
 #include "common.hpp"
 
 namespace dsw {
@@ -31,52 +36,63 @@ struct RotArgs {
     float *partial;          // backward: [blocks][2][D] or null
     long long tokens;
     int L, Hq, Hkv, D, axes, pairs, rl_log, units, tpw;
+    int mul_n, mul_pairs;    // e / n = e * mul_n >> 18 for e below 2^11 and n up to 64; c / pairs = c * mul_pairs >> 16 for c below 64
     float eps;
 };
 
-template <typename T, int Q> struct piece;  // Q consecutive elements, aligned to their size (16 bytes at most)
-template <> struct piece<bf16_t, 8> {
-    __device__ static __forceinline__ void ld(const bf16_t *p, float *v) {
-        const uint4 u = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// Q consecutive elements, aligned to their size (16 bytes at most): loaded as WORDS registers, unpacked later
+template <typename T, int Q> struct piece;
+template <int Q> struct piece<bf16_t, Q> {
+    static constexpr int WORDS = Q == 1 ? 1 : Q / 2;
+    __device__ static __forceinline__ void ld(const bf16_t *p, uint32_t *w) {
+        if constexpr (Q == 8) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(p);
+            w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+        } else if constexpr (Q == 4) {
+            const uint2 u = *reinterpret_cast<const uint2 *>(p);
+            w[0] = u.x, w[1] = u.y;
+        } else if constexpr (Q == 2) {
+            w[0] = *reinterpret_cast<const uint32_t *>(p);
+        } else {
+            w[0] = *p;
+        }
+    }
+    __device__ static __forceinline__ void unpack(const uint32_t *w, float *v) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        for (int i = 0; i < WORDS; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            if constexpr (Q > 1) v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
     }
     __device__ static __forceinline__ void st(bf16_t *p, const float *v) {
-        *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+        if constexpr (Q == 8) *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+        else if constexpr (Q == 4) *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+        else if constexpr (Q == 2) *reinterpret_cast<uint32_t *>(p) = pack_bf16(v[0], v[1]);
+        else *p = f32_to_bf16(v[0]);
     }
 };
-template <> struct piece<bf16_t, 4> {
-    __device__ static __forceinline__ void ld(const bf16_t *p, float *v) {
-        const float4 f = io<bf16_t>::ld4(p);
-        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+template <int Q> struct piece<float, Q> {
+    static constexpr int WORDS = Q;
+    __device__ static __forceinline__ void ld(const float *p, uint32_t *w) {
+        if constexpr (Q == 4) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(p);
+            w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+        } else if constexpr (Q == 2) {
+            const uint2 u = *reinterpret_cast<const uint2 *>(p);
+            w[0] = u.x, w[1] = u.y;
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t *>(p);
+        }
     }
-    __device__ static __forceinline__ void st(bf16_t *p, const float *v) { io<bf16_t>::st4(p, make_float4(v[0], v[1], v[2], v[3])); }
-};
-template <> struct piece<bf16_t, 2> {
-    __device__ static __forceinline__ void ld(const bf16_t *p, float *v) {
-        const uint32_t u = *reinterpret_cast<const uint32_t *>(p);
-        v[0] = __uint_as_float(u << 16), v[1] = __uint_as_float(u & 0xffff0000u);
+    __device__ static __forceinline__ void unpack(const uint32_t *w, float *v) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i) v[i] = __uint_as_float(w[i]);
     }
-    __device__ static __forceinline__ void st(bf16_t *p, const float *v) { *reinterpret_cast<uint32_t *>(p) = pack_bf16(v[0], v[1]); }
-};
-template <> struct piece<float, 4> {
-    __device__ static __forceinline__ void ld(const float *p, float *v) {
-        const float4 f = *reinterpret_cast<const float4 *>(p);
-        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    __device__ static __forceinline__ void st(float *p, const float *v) {
+        if constexpr (Q == 4) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        else if constexpr (Q == 2) *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
+        else *p = v[0];
     }
-    __device__ static __forceinline__ void st(float *p, const float *v) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
-};
-template <> struct piece<float, 2> {
-    __device__ static __forceinline__ void ld(const float *p, float *v) {
-        const float2 f = *reinterpret_cast<const float2 *>(p);
-        v[0] = f.x, v[1] = f.y;
-    }
-    __device__ static __forceinline__ void st(float *p, const float *v) { *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]); }
-};
-template <typename T> struct piece<T, 1> {
-    __device__ static __forceinline__ void ld(const T *p, float *v) { v[0] = io<T>::ld(p); }
-    __device__ static __forceinline__ void st(T *p, const float *v) { io<T>::st(p, v[0]); }
 };
 
 constexpr int ROT_THREADS = 256;
@@ -86,8 +102,8 @@ constexpr int ROT_THREADS = 256;
 __device__ __forceinline__ void rot_tables(const RotArgs &a, long long token0, int nt, float2 *cs, float *w) {
     const int n = a.axes * a.pairs;
     for (int e = threadIdx.x; e < nt * n; e += ROT_THREADS) {
-        const int t = e / n, c = e - t * n, ax = c / a.pairs;
-        const long long token = token0 + t, b = token / a.L;
+        const int t = (int)((unsigned)e * (unsigned)a.mul_n >> 18), c = e - t * n, ax = c * a.mul_pairs >> 16;
+        const unsigned token = (unsigned)token0 + t, b = token / (unsigned)a.L;  // (fewer than 2^31 tokens)
         const int l = (int)(token - b * a.L);
         const long long at = b * a.pos_batch + (long long)l * a.axes + ax;
         const long long pos = !a.pos ? l : a.pos_bytes == 8 ? static_cast<const long long *>(a.pos)[at] : static_cast<const int *>(a.pos)[at];
@@ -105,17 +121,64 @@ __device__ __forceinline__ void rot_tables(const RotArgs &a, long long token0, i
         }
 }
 
-// columns of unit u: two pieces of Q elements; returns whether the second one exists
-template <int Q, bool INTER> __device__ __forceinline__ bool rot_columns(int u, int n, int D, int &ca, int &cb, bool &turned) {
-    turned = Q * u < n;
-    if (turned) {
-        ca = INTER ? 2 * Q * u : Q * u;
-        cb = INTER ? ca + Q : n + Q * u;
-    } else {
-        ca = 2 * n + 2 * (Q * u - n);
-        cb = ca + Q;
+// The units of a lane, the same in all its rows: the columns of their two pieces and which of them exist.  A piece that does
+// not is loaded from the row's start and masked to zero: loads under branches are waited for one by one.
+template <int Q, int NU, bool INTER> struct RotUnits {
+    int ca[NU], cb[NU], at[NU];  // at: first pair of the unit
+    uint32_t ma[NU], mb[NU];     // all ones where the piece exists
+    bool one[NU], two[NU], turned[NU];
+    __device__ __forceinline__ RotUnits(int lane, int RL, int units, int n, int D) {
+#pragma unroll
+        for (int j = 0; j < NU; ++j) {
+            const int u = lane + j * RL;
+            at[j] = Q * u;
+            turned[j] = Q * u < n;
+            ca[j] = turned[j] ? (INTER ? 2 * Q * u : Q * u) : 2 * Q * u;
+            cb[j] = turned[j] && !INTER ? n + Q * u : ca[j] + Q;
+            one[j] = u < units;
+            two[j] = one[j] && cb[j] < D;
+            turned[j] = turned[j] && one[j];
+            ma[j] = one[j] ? ~0u : 0u, mb[j] = two[j] ? ~0u : 0u;
+            if (!one[j]) ca[j] = 0;
+            if (!two[j]) cb[j] = 0;
+        }
     }
-    return cb < D;
+    template <typename T> __device__ __forceinline__ void ld(const T *row, uint32_t (*w)[2 * piece<T, Q>::WORDS]) const {
+#pragma unroll
+        for (int j = 0; j < NU; ++j) {
+            piece<T, Q>::ld(row + ca[j], w[j]);
+            piece<T, Q>::ld(row + cb[j], w[j] + piece<T, Q>::WORDS);
+        }
+    }
+    template <typename T> __device__ __forceinline__ void unpack(const uint32_t (*w)[2 * piece<T, Q>::WORDS], uint32_t row, float (*v)[2 * Q]) const {
+        constexpr int N = piece<T, Q>::WORDS;
+#pragma unroll
+        for (int j = 0; j < NU; ++j) {
+            uint32_t m[2 * N];
+#pragma unroll
+            for (int i = 0; i < 2 * N; ++i) m[i] = w[j][i] & (i < N ? ma[j] : mb[j]) & row;
+            piece<T, Q>::unpack(m, v[j]);
+            piece<T, Q>::unpack(m + N, v[j] + Q);
+        }
+    }
+    template <typename T> __device__ __forceinline__ void st(T *row, const float (*v)[2 * Q]) const {
+#pragma unroll
+        for (int j = 0; j < NU; ++j) {
+            if (one[j]) piece<T, Q>::st(row + ca[j], v[j]);
+            if (two[j]) piece<T, Q>::st(row + cb[j], v[j] + Q);
+        }
+    }
+};
+// the sum over the 2^rl_log lanes of a row (16 at most), in all of them
+template <int CTRL> __device__ __forceinline__ float rot_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float rot_row_sum(float v, int rl_log) {
+    if (rl_log > 0) v = rot_add<0xb1>(v);   // neighbours
+    if (rl_log > 1) v = rot_add<0x4e>(v);   // pairs of a quad
+    if (rl_log > 2) v = rot_add<0x141>(v);  // quads of eight lanes
+    if (rl_log > 3) v = rot_add<0x140>(v);  // eights of sixteen
+    return v;
 }
 // turn the pairs of a unit; inv: back
 template <int Q, bool INTER> __device__ __forceinline__ void rot_turn(float *x, const float2 *cs, bool inv) {
@@ -152,7 +215,7 @@ __device__ __forceinline__ void rot_offsets(const RotArgs &a, long long token0, 
     if (threadIdx.x >= (unsigned)(tensors * ROT_TOKENS)) return;
     const int k = threadIdx.x / ROT_TOKENS, t = threadIdx.x % ROT_TOKENS;
     if (t >= nt) return;
-    const long long token = token0 + t, b = token / a.L, l = token - b * a.L;
+    const unsigned token = (unsigned)token0 + t, b = token / (unsigned)a.L, l = token - b * a.L;
     const RotOperand &o = k < 2 ? a.x[k] : k < 4 ? a.y[k - 2] : a.dy[k - 4];
     off[k * ROT_TOKENS + t] = b * o.s.b + l * o.s.l;
 }
@@ -167,41 +230,25 @@ __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_fwd_kernel(const R
     float2 *cs = reinterpret_cast<float2 *>(w + ((2 * D + 3) & ~3));
     const int RL = 1 << a.rl_log, lane = threadIdx.x & (RL - 1), grp = threadIdx.x >> a.rl_log, G = ROT_THREADS >> a.rl_log;
     const float inv_d = 1.f / (float)D;
-    constexpr int AHEAD = 2;  // rows whose loads are under way together
+    constexpr int AHEAD = 2;  // rows whose loads are under way together (one: the same; four: 52 us for 48)
     __shared__ long long off[4 * ROT_TOKENS];
     rot_offsets(a, token0, nt, 4, off);
     __syncthreads();
+    const RotUnits<Q, NU, INTER> un(lane, RL, a.units, n, D);
     RotRows row(a.Hq + a.Hkv, grp, G);
     bool first = true;
     while (first || row.t < nt) {
-        float x[AHEAD][NU][2 * Q];
+        uint32_t raw[AHEAD][NU][2 * piece<T, Q>::WORDS];
         T *dst[AHEAD];
         int tk[AHEAD], kind[AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
-            dst[k] = nullptr;
-#pragma unroll
-            for (int j = 0; j < NU; ++j)
-#pragma unroll
-                for (int i = 0; i < 2 * Q; ++i) x[k][j][i] = 0.f;
             tk[k] = row.t, kind[k] = row.h >= a.Hq;
-            if (row.t < nt) {
-                const int which = kind[k], h = row.h - (which ? a.Hq : 0);
-                const T *src = static_cast<const T *>(which ? a.x[1].p : a.x[0].p) + off[which * ROT_TOKENS + row.t] + h * (which ? a.x[1].s.h : a.x[0].s.h);
-                dst[k] = static_cast<T *>(const_cast<void *>(which ? a.y[1].p : a.y[0].p)) + off[(2 + which) * ROT_TOKENS + row.t] +
-                         h * (which ? a.y[1].s.h : a.y[0].s.h);
-#pragma unroll
-                for (int j = 0; j < NU; ++j) {
-                    const int u = lane + j * RL;
-                    int ca, cb;
-                    bool turned;
-                    if (u < a.units) {
-                        const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
-                        piece<T, Q>::ld(src + ca, x[k][j]);
-                        if (two) piece<T, Q>::ld(src + cb, x[k][j] + Q);
-                    }
-                }
-            }
+            const int which = kind[k], h = row.h - (which ? a.Hq : 0), t = min(row.t, nt - 1);  // (past the tile: any of its rows)
+            const T *src = static_cast<const T *>(which ? a.x[1].p : a.x[0].p) + off[which * ROT_TOKENS + t] + h * (which ? a.x[1].s.h : a.x[0].s.h);
+            dst[k] = static_cast<T *>(const_cast<void *>(which ? a.y[1].p : a.y[0].p)) + off[(2 + which) * ROT_TOKENS + t] +
+                     h * (which ? a.y[1].s.h : a.y[0].s.h);
+            un.ld(src, raw[k]);
             row.next();
         }
         if (first) {  // the tables are made while the first rows are on their way
@@ -211,32 +258,27 @@ __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_fwd_kernel(const R
         }
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
+            float x[NU][2 * Q];
+            un.template unpack<T>(raw[k], ~0u, x);
             float ss = 0.f;
 #pragma unroll
             for (int j = 0; j < NU; ++j)
 #pragma unroll
-                for (int i = 0; i < 2 * Q; ++i) ss = __builtin_fmaf(x[k][j][i], x[k][j][i], ss);
-            for (int o = RL >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-            if (dst[k] == nullptr) continue;
+                for (int i = 0; i < 2 * Q; ++i) ss = __builtin_fmaf(x[j][i], x[j][i], ss);
+            ss = rot_row_sum(ss, a.rl_log);
+            if (tk[k] >= nt) continue;
             const float *wr = w + (kind[k] ? D : 0);
             const float r = rsqrtf(ss * inv_d + a.eps);
 #pragma unroll
             for (int j = 0; j < NU; ++j) {
-                const int u = lane + j * RL;
-                if (u >= a.units) continue;
-                int ca, cb;
-                bool turned;
-                const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
-                float *v = x[k][j];
 #pragma unroll
                 for (int i = 0; i < Q; ++i) {
-                    v[i] = v[i] * r * wr[ca + i];
-                    v[Q + i] = two ? v[Q + i] * r * wr[cb + i] : 0.f;
+                    x[j][i] *= r * wr[un.ca[j] + i];
+                    x[j][Q + i] *= r * wr[un.cb[j] + i];
                 }
-                if (turned) rot_turn<Q, INTER>(v, cs + tk[k] * n + Q * u, false);
-                piece<T, Q>::st(dst[k] + ca, v);
-                if (two) piece<T, Q>::st(dst[k] + cb, v + Q);
+                if (un.turned[j]) rot_turn<Q, INTER>(x[j], cs + tk[k] * n + un.at[j], false);
             }
+            un.st(dst[k], x);
         }
     }
 }
@@ -251,8 +293,9 @@ __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_bwd_kernel(const R
     float2 *cs = reinterpret_cast<float2 *>(w + ((2 * D + 3) & ~3));
     const int RL = 1 << a.rl_log, lane = threadIdx.x & (RL - 1), grp = threadIdx.x >> a.rl_log, G = ROT_THREADS >> a.rl_log;
     const float inv_d = 1.f / (float)D;
-    constexpr int AHEAD = Q == 8 ? 1 : 2;
+    constexpr int AHEAD = 1;  // rows whose loads are under way together (two: 82 us for 80, four: 86; the registers cost waves)
     __shared__ long long off[6 * ROT_TOKENS];
+    const RotUnits<Q, NU, INTER> un(lane, RL, a.units, n, D);
     float dw[2][NU][2 * Q];
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -260,124 +303,85 @@ __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_bwd_kernel(const R
         for (int j = 0; j < NU; ++j)
 #pragma unroll
             for (int i = 0; i < 2 * Q; ++i) dw[m][j][i] = 0.f;
-    const long long tiles = (a.tokens + a.tpw - 1) / a.tpw;
-    for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const long long token0 = tile * a.tpw;
+    const int tiles = (int)((a.tokens + a.tpw - 1) / a.tpw);
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const long long token0 = (long long)tile * a.tpw;
         const int nt = (int)(a.tokens - token0 < a.tpw ? a.tokens - token0 : a.tpw);
         __syncthreads();  // the last tile's readers are done
         rot_offsets(a, token0, nt, 6, off);
-        rot_tables(a, token0, nt, cs, tile == blockIdx.x ? w : nullptr);
+        rot_tables(a, token0, nt, cs, tile == (int)blockIdx.x ? w : nullptr);
         __syncthreads();
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             const int H = m ? a.Hkv : a.Hq;
             if (H == 0) continue;
+            const float *wr = w + m * D;
             RotRows row(H, grp, G);
             while (row.t < nt) {
-                float x[AHEAD][NU][2 * Q], g[AHEAD][NU][2 * Q];
+                uint32_t rx[AHEAD][NU][2 * piece<T, Q>::WORDS], rg[AHEAD][NU][2 * piece<T, Q>::WORDS];
                 T *dst[AHEAD];
                 int tk[AHEAD];
 #pragma unroll
                 for (int k = 0; k < AHEAD; ++k) {
-                    dst[k] = nullptr;
                     tk[k] = row.t;
-#pragma unroll
-                    for (int j = 0; j < NU; ++j)
-#pragma unroll
-                        for (int i = 0; i < 2 * Q; ++i) x[k][j][i] = 0.f, g[k][j][i] = 0.f;
-                    if (row.t < nt) {
-                        const T *src = static_cast<const T *>(a.x[m].p) + off[m * ROT_TOKENS + row.t] + row.h * a.x[m].s.h;
-                        const T *grd = static_cast<const T *>(a.dy[m].p) + off[(4 + m) * ROT_TOKENS + row.t] + row.h * a.dy[m].s.h;
-                        dst[k] = static_cast<T *>(const_cast<void *>(a.y[m].p)) + off[(2 + m) * ROT_TOKENS + row.t] + row.h * a.y[m].s.h;
-#pragma unroll
-                        for (int j = 0; j < NU; ++j) {
-                            const int u = lane + j * RL;
-                            int ca, cb;
-                            bool turned;
-                            if (u < a.units) {
-                                const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
-                                piece<T, Q>::ld(src + ca, x[k][j]);
-                                piece<T, Q>::ld(grd + ca, g[k][j]);
-                                if (two) {
-                                    piece<T, Q>::ld(src + cb, x[k][j] + Q);
-                                    piece<T, Q>::ld(grd + cb, g[k][j] + Q);
-                                }
-                            }
-                        }
-                    }
+                    const int t = min(row.t, nt - 1);  // (past the tile: any of its rows)
+                    un.ld(static_cast<const T *>(a.x[m].p) + off[m * ROT_TOKENS + t] + row.h * a.x[m].s.h, rx[k]);
+                    un.ld(static_cast<const T *>(a.dy[m].p) + off[(4 + m) * ROT_TOKENS + t] + row.h * a.dy[m].s.h, rg[k]);
+                    dst[k] = static_cast<T *>(const_cast<void *>(a.y[m].p)) + off[(2 + m) * ROT_TOKENS + t] + row.h * a.y[m].s.h;
                     row.next();
                 }
 #pragma unroll
                 for (int k = 0; k < AHEAD; ++k) {
+                    float x[NU][2 * Q], g[NU][2 * Q];
+                    const uint32_t on = tk[k] < nt ? ~0u : 0u;  // (past the tile: zeros, which add nothing to the weights' gradients)
+                    un.template unpack<T>(rx[k], on, x);
+                    un.template unpack<T>(rg[k], on, g);
                     float ss = 0.f;
 #pragma unroll
                     for (int j = 0; j < NU; ++j)
 #pragma unroll
-                        for (int i = 0; i < 2 * Q; ++i) ss = __builtin_fmaf(x[k][j][i], x[k][j][i], ss);
-                    for (int o = RL >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-                    const float r = rsqrtf(ss * inv_d + a.eps);
+                        for (int i = 0; i < 2 * Q; ++i) ss = __builtin_fmaf(x[j][i], x[j][i], ss);
+                    const float r = rsqrtf(rot_row_sum(ss, a.rl_log) * inv_d + a.eps);
                     float dot = 0.f;
-                    if (dst[k] != nullptr) {
-#pragma unroll
-                        for (int j = 0; j < NU; ++j) {
-                            const int u = lane + j * RL;
-                            if (u >= a.units) continue;
-                            int ca, cb;
-                            bool turned;
-                            const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
-                            if (turned) rot_turn<Q, INTER>(g[k][j], cs + tk[k] * n + Q * u, true);
-#pragma unroll
-                            for (int i = 0; i < 2 * Q; ++i) {
-                                const float wv = i < Q ? w[m * D + ca + i] : two ? w[m * D + cb + i - Q] : 0.f;
-                                x[k][j][i] *= r;  // (zero, like g, in a piece that is not there)
-                                dw[m][j][i] = __builtin_fmaf(g[k][j][i], x[k][j][i], dw[m][j][i]);
-                                g[k][j][i] *= wv;
-                                dot = __builtin_fmaf(g[k][j][i], x[k][j][i], dot);
-                            }
-                        }
-                    }
-                    for (int o = RL >> 1; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
-                    dot *= inv_d;
-                    if (dst[k] == nullptr) continue;
 #pragma unroll
                     for (int j = 0; j < NU; ++j) {
-                        const int u = lane + j * RL;
-                        if (u >= a.units) continue;
-                        int ca, cb;
-                        bool turned;
-                        const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
+                        if (un.turned[j]) rot_turn<Q, INTER>(g[j], cs + min(tk[k], nt - 1) * n + un.at[j], true);
 #pragma unroll
-                        for (int i = 0; i < 2 * Q; ++i) g[k][j][i] = r * __builtin_fmaf(-x[k][j][i], dot, g[k][j][i]);
-                        piece<T, Q>::st(dst[k] + ca, g[k][j]);
-                        if (two) piece<T, Q>::st(dst[k] + cb, g[k][j] + Q);
+                        for (int i = 0; i < 2 * Q; ++i) {
+                            x[j][i] *= r;  // (zero, like g, in a piece that is not there)
+                            dw[m][j][i] = __builtin_fmaf(g[j][i], x[j][i], dw[m][j][i]);
+                            g[j][i] *= wr[i < Q ? un.ca[j] + i : un.cb[j] + i - Q];
+                            dot = __builtin_fmaf(g[j][i], x[j][i], dot);
+                        }
                     }
+                    dot = rot_row_sum(dot, a.rl_log) * inv_d;
+#pragma unroll
+                    for (int j = 0; j < NU; ++j)
+#pragma unroll
+                        for (int i = 0; i < 2 * Q; ++i) g[j][i] = r * __builtin_fmaf(-x[j][i], dot, g[j][i]);
+                    if (tk[k] < nt) un.st(dst[k], g);
                 }
             }
         }
     }
     if (a.partial == nullptr) return;
-    // the groups of a wave, then the four waves
+    // the groups' shares through LDS: [group][2][D], summed in a fixed order by four threads for each entry
     __syncthreads();
-    float *red = reinterpret_cast<float *>(smem);  // [4][2][D]
+    float *red = reinterpret_cast<float *>(smem);
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int j = 0; j < NU; ++j)
 #pragma unroll
-            for (int i = 0; i < 2 * Q; ++i) {
-                float v = dw[m][j][i];
-                for (int o = RL; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-                const int u = lane + j * RL;
-                int ca, cb;
-                bool turned;
-                if ((threadIdx.x & 63) < RL && u < a.units) {
-                    const bool two = rot_columns<Q, INTER>(u, n, D, ca, cb, turned);
-                    if (i < Q || two) red[((threadIdx.x >> 6) * 2 + m) * D + (i < Q ? ca + i : cb + i - Q)] = v;
-                }
-            }
+            for (int i = 0; i < 2 * Q; ++i)
+                if (i < Q ? un.one[j] : un.two[j]) red[(grp * 2 + m) * D + (i < Q ? un.ca[j] + i : un.cb[j] + i - Q)] = dw[m][j][i];
     __syncthreads();
-    for (int e = threadIdx.x; e < 2 * D; e += ROT_THREADS)
-        a.partial[(size_t)blockIdx.x * 2 * D + e] = (red[e] + red[2 * D + e]) + (red[4 * D + e] + red[6 * D + e]);
+    for (int e = threadIdx.x >> 2; e < 2 * D; e += ROT_THREADS >> 2) {
+        float v = 0.f;
+        for (int g = threadIdx.x & 3; g < G; g += 4) v += red[g * 2 * D + e];
+        v = rot_row_sum(v, 2);
+        if ((threadIdx.x & 3) == 0) a.partial[(size_t)blockIdx.x * 2 * D + e] = v;
+    }
 }
 
 constexpr int ROT_MAX_D = 128, ROT_BWD_BLOCKS = 2048;
@@ -442,6 +446,7 @@ static int rot_check(const char *who, RotArgs &a, int dtype, int B, bool bwd, in
     a.units = (a.D + 2 * Q - 1) / (2 * Q);
     a.rl_log = rot_lanes_log(a.D, Q);
     a.tpw = rot_tile(a.tokens, a.Hq + a.Hkv, a.D, n, dtype, bwd);
+    if (n) a.mul_n = (1 << 18) / n + 1, a.mul_pairs = (1 << 16) / a.pairs + 1;
     return DSW_OK;
 }
 
@@ -450,7 +455,8 @@ static int rot_launch(const RotArgs &a, bool bwd, bool interleaved, hipStream_t 
     const long long tiles = (a.tokens + a.tpw - 1) / a.tpw;
     size_t lds = ((2 * a.D + 3) & ~3) * 4 + (size_t)a.tpw * a.axes * a.pairs * 8;
     if (bwd) {
-        if (lds < (size_t)8 * a.D * 4) lds = (size_t)8 * a.D * 4;
+        const size_t shares = (size_t)(ROT_THREADS >> a.rl_log) * 2 * a.D * 4;  // (32 KB at most)
+        if (a.partial && lds < shares) lds = shares;
         const dim3 grid((unsigned)(tiles < ROT_BWD_BLOCKS ? tiles : ROT_BWD_BLOCKS));
         if (interleaved) qk_norm_rotary_bwd_kernel<T, Q, NU, true><<<grid, ROT_THREADS, lds, st>>>(a);
         else qk_norm_rotary_bwd_kernel<T, Q, NU, false><<<grid, ROT_THREADS, lds, st>>>(a);
