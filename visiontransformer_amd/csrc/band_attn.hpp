@@ -447,6 +447,18 @@ template <int SIZE> struct BandEdges {
 
 // The query rows of a workgroup (forward, dQ).  Made twice, before the loop and after it, from the arguments: what only
 // the end needs does not have to be kept in scalar registers through the loop, which were spilled for it.
+// Which piece of work a workgroup takes, of `per` pieces for each (sequence, key head): hardware deals workgroups to the
+// eight XCDs in turn, and those of one key head belong on one of them, whose L2 then holds the keys once.  Key heads are dealt
+// in turn as well, so that sequences of unequal lengths, or empty ones, spread over all XCDs (a run of neighbours for
+// each XCD: dq 65 us for 41, dk and dv 63 for 52, three sequences of 0, 680 and 1021 tokens, fp32, 6 heads of 32); what is left
+// of them after whole rounds of eight is cut into eight runs.
+__device__ __forceinline__ int band_piece_of(int block, int blocks, int per) {
+    const int whole = blocks / per / 8 * 8 * per;
+    if (block >= whole) return whole + xcd_remap(block - whole, blocks - whole);
+    const int at = block >> 3, round = at / per;
+    return (round * 8 + (block & 7)) * per + (at - round * per);
+}
+
 struct BandPlace {
     int b, h, hk, i_lo, i0, i;
     BandSeq sq;
@@ -454,7 +466,7 @@ struct BandPlace {
     // `rows` of a workgroup: 128, or 64 where two waves share 32
     __device__ __forceinline__ BandPlace(const BandArgs &a, int block, int blocks, int rows = BAND_ROWS) {
         const int nqb = (a.Lq + rows - 1) / rows;
-        const int idx = xcd_remap(block, blocks);
+        const int idx = band_piece_of(block, blocks, nqb * a.G);
         const int g = idx % a.G, rest = idx / a.G;
         const int qb = nqb - 1 - rest % nqb, bh = rest / nqb;  // (the last rows of a causal call have the most to do: first)
         hk = bh % a.Hkv, b = bh / a.Hkv, h = hk * a.G + g;

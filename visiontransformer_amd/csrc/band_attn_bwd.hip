@@ -19,7 +19,7 @@ namespace dsw {
 template <typename T, int DP, int MODE, bool BIAS>
 __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void band_attn_dkv_kernel(const BandArgs a) {
     constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE), C = DP / 16;
-    constexpr bool AHEAD = DP < 128 && sizeof(T) == 2;  // registers for LDS reads well ahead of the products that need them
+    constexpr bool AHEAD = DP < 128 && (sizeof(T) == 2 || DP == 32);  // registers for LDS reads well ahead of the products that need them
     using Stage = BandStage<T, DP, MODE>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     T *const lds = reinterpret_cast<T *>(smem);                        // [NB][Q | dO]
@@ -27,7 +27,7 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
     float *const bias = stats + NB * 2 * BAND_TILE;
 
     const int nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS, units = a.sink_blocks * a.sink_chunks + (nkb - a.sink_blocks) * a.chunks;
-    const int idx = xcd_remap(blockIdx.x, gridDim.x);
+    const int idx = band_piece_of(blockIdx.x, gridDim.x, units);
     const int bh = idx / units, unit = idx - bh * units, hk = bh % a.Hkv, b = bh / a.Hkv;
     const bool of_sinks = unit < a.sink_blocks * a.sink_chunks;
     const int nc = of_sinks ? a.sink_chunks : a.chunks, left_over = unit - (of_sinks ? 0 : a.sink_blocks * a.sink_chunks);
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
                     *reinterpret_cast<float4 *>(nl + 4 * k) = *reinterpret_cast<const float4 *>(S + 32 * u + 8 * k + 4 * hh);
                     *reinterpret_cast<float4 *>(del + 4 * k) = *reinterpret_cast<const float4 *>(S + BAND_TILE + 32 * u + 8 * k + 4 * hh);
                 }
-                if (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+                if (sizeof(T) == 2 || DP == 32) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
                     s = band_mma(qf[c], kf[c], s);
@@ -225,7 +225,8 @@ template <typename T, int V> __global__ __launch_bounds__(256) void band_attn_jo
 }
 
 // Two workgroups a CU are wanted (one for wide heads, whose registers allow no more); a run of the work is at least 8
-// steps long (2 in fp32, whose products take 16 times as long), so that its share does not cost more than it brings.  Blocks of
+// steps long, so that its share does not cost more than it brings.  In fp32, whose products take 16 times as long, runs of 2
+// steps pay, and so does a finer cut (4 a CU: 63 us for 68 for 3 x 1021 tokens, 6 heads of 32).  Blocks of
 // sinks are cut into runs as long as the others' ones.
 static BandChunks band_chunks(const BandArgs &a, int dtype) {
     BandChunks c = {0, 1, 1, 0};
@@ -233,7 +234,7 @@ static BandChunks band_chunks(const BandArgs &a, int dtype) {
     if (nkb == 0 || heads == 0 || tiles == 0) return c;
     const long long window = (long long)a.left + a.right + BAND_ROWS, reach = window >= a.Lq ? tiles : window / BAND_TILE + 2;
     const long long normal = (reach < tiles ? reach : tiles) * a.G;  // steps of a block in the middle
-    const long long want = a.D > 64 ? 256 : 512, n = (want + heads * nkb - 1) / (heads * nkb), most = normal / (dtype == DSW_F32 ? 2 : 8);
+    const long long want = dtype == DSW_F32 ? 1024 : a.D > 64 ? 256 : 512, n = (want + heads * nkb - 1) / (heads * nkb), most = normal / (dtype == DSW_F32 ? 2 : 8);
     c.chunks = (int)(n < most ? n : most);
     if (c.chunks < 1) c.chunks = 1;
     if (c.chunks > 64) c.chunks = 64;
@@ -252,7 +253,7 @@ static BandChunks band_chunks(const BandArgs &a, int dtype) {
 template <typename T, int DP, int MODE, bool BIAS, bool DTABLE, bool SPLIT>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void band_attn_dq_kernel(const BandArgs a) {
     constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE), C = DP / 16;
-    constexpr bool AHEAD = DP < 128 && sizeof(T) == 2;  // registers for LDS reads well ahead of the products that need them
+    constexpr bool AHEAD = DP < 128 && (sizeof(T) == 2 || DP == 32);  // registers for LDS reads well ahead of the products that need them
     constexpr int ROWS = SPLIT ? BAND_ROWS / 2 : BAND_ROWS;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     T *const lds = reinterpret_cast<T *>(smem);  // [NB][K | V]
