@@ -666,14 +666,15 @@ int dsw_qk_norm_rotary_fwd(const void *q, const dsw_strides *sq, const void *k, 
                            int L, int Hq, int Hkv, int D, const float *wq, const float *wk, float eps, const float *freqs,
                            int axes, int pairs, const void *pos, int pos_bytes, long long pos_batch, int interleaved, void *oq,
                            const dsw_strides *soq, void *ok, const dsw_strides *sok, void *stream);
-/* Its backward: dq, dk from the gradients dyq, dyk of oq, ok (q, k: the inputs of the forward).  partial: NULL, or
- * fp32 [dsw_qk_norm_rotary_blocks(..)][2][D], whose column sums (dsw_colsum) are the gradients of wq and wk. */
+/* Its backward: dq, dk from the gradients dyq, dyk of oq, ok (q, k: the inputs of the forward).  dw: NULL, or fp32
+ * [2][D], the gradients of wq and wk (unwritten where B * L or Hq + Hkv is 0); then partial is its workspace, fp32
+ * [dsw_qk_norm_rotary_blocks(..)][2][D]. */
 int dsw_qk_norm_rotary_blocks(int dtype, int B, int L, int Hq, int Hkv, int D, int axes, int pairs);
 int dsw_qk_norm_rotary_bwd(const void *q, const dsw_strides *sq, const void *k, const dsw_strides *sk, const void *dyq,
                            const dsw_strides *sdyq, const void *dyk, const dsw_strides *sdyk, int dtype, int B, int L,
                            int Hq, int Hkv, int D, const float *wq, const float *wk, float eps, const float *freqs, int axes,
                            int pairs, const void *pos, int pos_bytes, long long pos_batch, int interleaved, void *dq, const dsw_strides *sdq,
-                           void *dk, const dsw_strides *sdk, float *partial, void *stream);
+                           void *dk, const dsw_strides *sdk, float *partial, float *dw, void *stream);
 
 /* Softmax attention with a sliding window of keys and a few first keys (sinks) that stay visible.  Query row i of
  * sequence b stands at p = k_len - q_len + i (q_len <= Lq rows, k_len <= Lk keys); key j < k_len is visible to it when

@@ -134,7 +134,7 @@ SIGNATURES = {
     "dsw_band_attn_fwd": (_I, [_P] * 12 + [_Z, _P]),
     "dsw_band_attn_bwd_workspace": (_Z, [_P]),
     "dsw_band_attn_bwd": (_I, [_P] * 21 + [_Z, _P]),
-    "dsw_qk_norm_rotary_bwd": (_I, [_P] * 8 + [_I] * 6 + [_P, _P, _F, _P, _I, _I, _P, _I, ctypes.c_longlong, _I] + [_P] * 6),
+    "dsw_qk_norm_rotary_bwd": (_I, [_P] * 8 + [_I] * 6 + [_P, _P, _F, _P, _I, _I, _P, _I, ctypes.c_longlong, _I] + [_P] * 7),
 }
 
 

@@ -501,22 +501,37 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     }
 }
 
-// by_distance[head][2 M + 1] = sum over the head's row blocks
-__global__ __launch_bounds__(1024) void band_attn_distance_kernel(const float *__restrict__ partial, int rows, int n, float *__restrict__ dst) {
-    __shared__ float red[32][33];
-    int col;
-    float total;
-    if (column_sum_32<32>(partial + (size_t)blockIdx.y * rows * n, rows, n, red, col, total)) dst[(size_t)blockIdx.y * n + col] = total;
-}
-// one wave per (bucket, head)
-__global__ __launch_bounds__(64) void band_attn_table_kernel(const float *__restrict__ by_distance, const int *__restrict__ buckets, int n,
-                                                             int n_buckets, int heads, float *__restrict__ d_table) {
-    const int bucket = blockIdx.x, h = blockIdx.y;
+// d_table[bucket][head] = the sum of the head's `rows` row blocks over the distances of the bucket: the distances listed in
+// their order, then all pairs of a block and a listed distance over 256 threads, so that buckets of one distance and of
+// hundreds keep them all busy.  (Sums by distance first and by bucket in a second launch took the same time, and one more launch.)
+__global__ __launch_bounds__(256) void band_attn_table_kernel(const float *__restrict__ partial, const int *__restrict__ buckets, int rows, int n,
+                                                              int n_buckets, int heads, float *__restrict__ d_table) {
+    __shared__ int list[2 * BAND_MAX_DISTANCE + 1], length;
+    __shared__ float red[4];
+    const int bucket = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63;
+    if (threadIdx.x < 64) {
+        int at = 0;
+        for (int e0 = 0; e0 < n; e0 += 64) {
+            const bool in = e0 + lane < n && min(max(buckets[e0 + lane], 0), n_buckets - 1) == bucket;
+            const unsigned long long all = __ballot(in);
+            if (in) list[at + __popcll(all & ((1ull << lane) - 1))] = e0 + lane;
+            at += __popcll(all);
+        }
+        if (lane == 0) length = at;
+    }
+    __syncthreads();
+    const float *const src = partial + (size_t)h * rows * n;
+    const unsigned cnt = length, pairs = cnt * (unsigned)rows;  // (the caller sees to it that n * rows fits)
     float v = 0.f;
-    for (int e = threadIdx.x; e < n; e += 64)
-        if (min(max(buckets[e], 0), n_buckets - 1) == bucket) v += by_distance[(size_t)h * n + e];
+#pragma unroll 4
+    for (unsigned k = threadIdx.x; k < pairs; k += 256) {
+        const unsigned r = k / cnt;
+        v += src[(size_t)r * n + list[k - r * cnt]];
+    }
     v = wave_sum(v);
-    if (threadIdx.x == 0) d_table[(size_t)bucket * heads + h] = v;
+    if (lane == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) d_table[(size_t)bucket * heads + h] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 template <typename K> static int allow_lds(K kern, size_t lds) {
@@ -570,7 +585,7 @@ extern "C" size_t dsw_band_attn_bwd_workspace(const dsw_band_desc *d) {
     if (band_make_args("dsw_band_attn_bwd_workspace", d, a)) return 0;
     size_t n = round16((size_t)a.B * a.Hq * a.Lq);
     n += (size_t)band_chunks(a, d->dtype).shares * 2 * BAND_ROWS * a.D;
-    if (a.table) n += (size_t)a.Hq * ((size_t)a.B * ((a.Lq + band_dq_rows(a) - 1) / band_dq_rows(a)) + 1) * (2 * a.M + 1);
+    if (a.table) n += (size_t)a.Hq * ((size_t)a.B * ((a.Lq + band_dq_rows(a) - 1) / band_dq_rows(a))) * (2 * a.M + 1);
     return n * sizeof(float);
 }
 
@@ -594,6 +609,10 @@ extern "C" int dsw_band_attn_bwd(const dsw_band_desc *d, const void *q, const ds
     DSW_REQUIRE(no_rows || lse, "%s: null lse", who);
     DSW_REQUIRE(d_table == nullptr || a.table, "%s: a gradient for a table that is not there", who);
     DSW_REQUIRE(d_table == nullptr || no_rows || d->dtype == DSW_F32 || out32, "%s: the table's gradient needs the forward's out32", who);
+    const int n = 2 * a.M + 1;
+    const long long rows = (long long)a.B * ((a.Lq + band_dq_rows(a) - 1) / band_dq_rows(a));
+    if (d_table && (rows * n >= (1LL << 31) || a.Hq > 65535))
+        return fail(DSW_EUNSUPPORTED, "%s: a table's gradient over %lld row blocks of %d heads", who, rows, a.Hq);
     const size_t need = dsw_band_attn_bwd_workspace(d);
     DSW_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "%s: workspace of %zu bytes, %zu are needed", who, workspace_bytes, need);
     a.lse = const_cast<float *>(lse);
@@ -609,10 +628,6 @@ extern "C" int dsw_band_attn_bwd(const dsw_band_desc *d, const void *q, const ds
              : a.table ? launch_bwd<T, DP, MODE, true, false>(a, st) : launch_bwd<T, DP, MODE, false, false>(a, st);
     });
     if (rc || d_table == nullptr) return rc;
-    const int n = 2 * a.M + 1, rows = a.B * ((a.Lq + band_dq_rows(a) - 1) / band_dq_rows(a));
-    float *by_distance = a.partial + (size_t)a.Hq * rows * n;
-    band_attn_distance_kernel<<<dim3((n + 31) / 32, a.Hq), 1024, 0, st>>>(a.partial, rows, n, by_distance);
-    if ((rc = check_launch("dsw_band_attn_bwd (distances)"))) return rc;
-    band_attn_table_kernel<<<dim3(a.n_buckets, a.Hq), 64, 0, st>>>(by_distance, a.buckets, n, a.n_buckets, a.Hq, d_table);
+    band_attn_table_kernel<<<dim3(a.n_buckets, a.Hq), 256, 0, st>>>(a.partial, a.buckets, (int)rows, n, a.n_buckets, a.Hq, d_table);
     return check_launch("dsw_band_attn_bwd (table)");
 }

@@ -384,7 +384,15 @@ __global__ __launch_bounds__(ROT_THREADS) void qk_norm_rotary_bwd_kernel(const R
     }
 }
 
-constexpr int ROT_MAX_D = 128, ROT_BWD_BLOCKS = 2048;
+// dw[2][D]: the workgroups' rows of `partial`, added in a fixed order
+__global__ __launch_bounds__(1024) void qk_norm_rotary_weights_kernel(const float *__restrict__ partial, int rows, int cols, float *__restrict__ dw) {
+    __shared__ float red[32][33];
+    int col;
+    float total;
+    if (column_sum_32<32>(partial, rows, cols, red, col, total)) dw[col] = total;
+}
+
+constexpr int ROT_MAX_D = 128, ROT_BWD_BLOCKS = 1024;  // (four of 256 threads a CU)
 
 // Tokens of a tile: eight rows for each group of lanes (sixteen backward, where a tile costs two barriers), so that the
 // angles, computed once per tile, and the tile's start are spread over them, while two thousand workgroups are left; one
@@ -511,14 +519,19 @@ extern "C" int dsw_qk_norm_rotary_bwd(const void *q, const dsw_strides *sq, cons
                                       const dsw_strides *sdyq, const void *dyk, const dsw_strides *sdyk, int dtype, int B, int L,
                                       int Hq, int Hkv, int D, const float *wq, const float *wk, float eps, const float *freqs,
                                       int axes, int pairs, const void *pos, int pos_bytes, long long pos_batch, int interleaved, void *dq,
-                                      const dsw_strides *sdq, void *dk, const dsw_strides *sdk, float *partial, void *stream) {
+                                      const dsw_strides *sdq, void *dk, const dsw_strides *sdk, float *partial, float *dw, void *stream) {
     DSW_REQUIRE(sq && sk && sdyq && sdyk && sdq && sdk, "dsw_qk_norm_rotary_bwd: null strides");
     RotArgs a = {};
     a.x[0] = {q, *sq}, a.x[1] = {k, *sk}, a.dy[0] = {dyq, *sdyq}, a.dy[1] = {dyk, *sdyk}, a.y[0] = {dq, *sdq}, a.y[1] = {dk, *sdk};
     a.w[0] = wq, a.w[1] = wk, a.freqs = freqs, a.pos = pos, a.pos_bytes = pos_bytes, a.pos_batch = pos_batch, a.partial = partial;
     a.L = L, a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.axes = axes, a.pairs = pairs, a.eps = eps;
     int Q = 1;
-    const int rc = rot_check("dsw_qk_norm_rotary_bwd", a, dtype, B, true, Q);
+    int rc = rot_check("dsw_qk_norm_rotary_bwd", a, dtype, B, true, Q);
+    DSW_REQUIRE((partial == nullptr) == (dw == nullptr), "dsw_qk_norm_rotary_bwd: partial and dw go together");
     if (rc || a.tokens == 0 || Hq + Hkv == 0) return rc;
-    return rot_dispatch(a, dtype, Q, true, interleaved != 0, as_stream(stream));
+    rc = rot_dispatch(a, dtype, Q, true, interleaved != 0, as_stream(stream));
+    if (rc || dw == nullptr) return rc;
+    const int rows = dsw_qk_norm_rotary_blocks(dtype, B, L, Hq, Hkv, D, axes, pairs);
+    qk_norm_rotary_weights_kernel<<<dim3((2 * D + 31) / 32), 1024, 0, as_stream(stream)>>>(partial, rows, 2 * D, dw);
+    return check_launch("dsw_qk_norm_rotary_bwd (weights)");
 }

@@ -2485,16 +2485,16 @@ class _QKNormRotaryFn(torch.autograd.Function):
         want_w = (wq is not None and ctx.needs_input_grad[2]) or (wk is not None and ctx.needs_input_grad[3])
         axes, pairs = (0, 0) if freqs is None else freqs.shape
         blocks = _lib.load().dsw_qk_norm_rotary_blocks(dtype_code(q.dtype), B, L, Hq, Hkv, D, axes, pairs)
-        partial = torch.empty(blocks, 2 * D, dtype=torch.float32, device=dev) if want_w and blocks else None
+        both = partial = None
+        if want_w:   # the workgroups' shares and, behind them, the two gradients
+            ran = B * L * (Hq + Hkv) > 0
+            both = (torch.empty if ran else torch.zeros)((blocks if ran else 0) + 1, 2, D, dtype=torch.float32, device=dev)
+            partial, both = (both.data_ptr() if ran else None), both[-1]
         if B * L:
             spec = _QKNormRotaryFn._spec(q, Hkv, wq, wk, freqs, positions, *ctx.settings)
             _call_on(dev, "dsw_qk_norm_rotary_bwd", pq, sq, pk, sk, pdyq, sdyq, pdyk, sdyk, *spec, pdq, sdq, pdk, sdk,
-                     ptr(partial), stream(dev))
-        dw = (None, None)
-        if want_w:
-            with torch.cuda.device(dev):
-                both = torch.zeros(2 * D, device=dev) if partial is None else colsum(partial)
-            dw = tuple(both[i * D:(i + 1) * D].to(t) if w is not None else None for i, (w, t) in enumerate(zip((wq, wk), ctx.weight_dtypes)))
+                     partial, both.data_ptr() if partial else None, stream(dev))
+        dw = [None if w is None or both is None else both[i].to(t) for i, (w, t) in enumerate(zip((wq, wk), ctx.weight_dtypes))]
         return dq, dk, dw[0], dw[1], None, None, None, None
 
 
