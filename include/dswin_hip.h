@@ -693,9 +693,10 @@ typedef struct {
     int n_buckets, max_distance; /* M <= 512 */
 } dsw_band_desc;
 
-/* lse: fp32 [B, Hq, Lq] for the backward or NULL; out32: NULL, or (bf16 calls with a bias table that wants a gradient)
- * fp32 [B, Lq, Hq, D], the result before its rounding, which the table's gradient needs.  Without it, calls of few
- * query rows (new tokens over a cache, short sequences) split the keys over workgroups; workspace holds their shares. */
+/* lse: fp32 [B, Hq, Lq] for the backward ([2, B, Hq, Lq] where there is a bias table) or NULL; out32: NULL, or (bf16 calls
+ * with a bias table that wants a gradient) fp32 [B, Lq, Hq, D], the result before its rounding, which the table's gradient
+ * needs.  Without it, calls of few query rows (new tokens over a cache, short sequences) split the keys over workgroups;
+ * workspace holds their shares. */
 size_t dsw_band_attn_fwd_workspace(const dsw_band_desc *d);
 int dsw_band_attn_fwd(const dsw_band_desc *d, const void *q, const dsw_strides *sq, const void *k, const dsw_strides *sk,
                       const void *v, const dsw_strides *sv, void *out, const dsw_strides *so, float *lse, float *out32,

@@ -138,6 +138,40 @@ def test_bias_without_its_gradient(cuda0, dtype):
     _check_attention(cuda0, BIAS_CASES[1][0], dtype, 13, 32, 128, table_grad=False)
 
 
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("value", [float("-inf"), torch.finfo(torch.float32).min, -1e9, -1e4])
+@pytest.mark.parametrize("masked", [70, 129])
+@pytest.mark.parametrize("table_grad", [True, False])
+def test_masks_in_a_bias_table(cuda0, dtype, value, masked, table_grad):
+    """A table that masks the nearest `masked` distances of a causal call (129: all of them), so that the first rows see
+    nothing else.  -inf takes those keys away: the reference leaves them out of the window.  A finite value leaves the softmax
+    of the scores to rows that have nothing better and nothing to the others; the reference has it as -100, whose weight of
+    4e-44 beside any other is far below its bounds."""
+    K = _K()
+    B, L, Hq, Hkv, D, M = 1, 300, 2, 1, 64, 128
+    q, k, v, dout, gen = _inputs((B, L, Hq, D), (B, L, Hkv, D), dtype, 31)
+    table = torch.randn(4, Hq, generator=gen) * 0.7
+    bmap = torch.tensor([0 if -masked < d <= 0 else 1 + (d & 1) for d in range(-M, M + 1)], dtype=torch.int32)
+    table[0] = value
+    instead = table.double()
+    instead[0] = -100.0
+    gone = value == float("-inf")
+    ref = S.attention(q.double(), k.double(), v.double(), None, (-masked if masked <= M else -10 ** 6) if gone else 0, 0, D ** -0.5, None, None,
+                      instead, bmap, dout.double(), dtype, table_grad)
+    leaves = [t.to(cuda0).requires_grad_() for t in (q, k, v)] + [table.to(cuda0).requires_grad_(table_grad)]
+    kw = dict(window=(None, 0), bias_table=leaves[3], bias_buckets=bmap.to(cuda0))
+    out = K.band_attention(*leaves[:3], **kw)
+    grads = torch.autograd.grad(out, leaves[:4 if table_grad else 3], dout.to(cuda0))
+    _within("out", out, *ref["out"])
+    for name, g in zip(("dq", "dk", "dv", "dtable"), grads):
+        _within(name, g, *ref[name])
+    with torch.no_grad():
+        _within("out (no grad)", K.band_attention(*leaves[:3], **kw), *ref["out"])
+    if gone:
+        rows = L if masked > M else masked
+        assert not out[:, :rows].any() and not grads[0][:, :rows].any()
+
+
 #  rows over a cache: B Lq Lk Hq Hkv D left right sinks
 STEPS = [
     (3, 1, 1000, 4, 1, 64, None, 0, 0), (2, 1, 5000, 8, 8, 128, 1023, 0, 4), (1, 1, 1, 2, 2, 30, 5, 0, 0),
@@ -266,6 +300,21 @@ def test_rows_that_see_one_key_have_no_gradient_of_their_scores(cuda0, dtype, D)
             ref = S.attention(q.double(), k.double(), v.double(), *window, 0, D ** -0.5, table=t, buckets=None if t is None else bmap.cpu(),
                               dout=dout.double(), dtype=dtype)
             _within("dv", grads[2], *ref["dv"])   # (a probability of 1 is off by the rounding of its logit, which may be any size)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_long_calls_of_rows_that_see_one_key(cuda0, dtype):
+    """the same where the row blocks fill the chip: another forward kernel"""
+    K = _K()
+    q, k, v, dout, gen = _inputs((1, 4200, 8, 32), (1, 4200, 8, 32), dtype, 8)
+    table = torch.randn(8, 8, generator=gen).to(cuda0).requires_grad_()
+    bmap = torch.tensor(S.bucket_map(8, 16, False), dtype=torch.int32, device=cuda0)
+    leaves = [t.to(cuda0).requires_grad_() for t in (q, k, v)] + [table]
+    for kw in (dict(bias_table=table, bias_buckets=bmap), {}):
+        out = K.band_attention(*leaves[:3], window=(0, 0), **kw)
+        assert torch.equal(out, leaves[2])
+        grads = torch.autograd.grad(out, leaves if kw else leaves[:3], dout.to(cuda0))
+        assert all(float(g.abs().max()) == 0.0 for i, g in enumerate(grads) if i != 2)
 
 
 def test_shared_heads_and_broadcast_inputs(cuda0):

@@ -6,6 +6,8 @@
 // All products run on 32x32 MFMA tiles with the softmax rows on the lane axis of the accumulators, so that the
 // probabilities of a tile are, as they stand in the registers, the second operand of the product behind them.
 #pragma once
+#include <cfloat>
+
 #include "attn_common.hpp"
 
 namespace dsw {
@@ -35,6 +37,7 @@ struct BandArgs {
     const int *buckets;  // [2 M + 1]
     int n_buckets, M;
     float *lse;          // [B][Hq][Lq], base 2; +inf for rows without a visible key (2^(x - inf) = 0 in the backward)
+    float *top;          // with a bias table: [B][Hq][Lq], taken out of lse (see band_keep)
     float *out32;        // [B][Lq][Hq][D] or null
     float *delta;        // [B][Hq][Lq]
     float *partial;      // step kernel: see there; dQ kernel: bias gradients by distance
@@ -412,7 +415,23 @@ struct BandWalk {
 __device__ __forceinline__ float band_bias_at(const BandArgs &a, int head, int rel) {
     const int m = min(max(rel, -a.M), a.M) + a.M;
     const int bucket = min(max(a.buckets[m], 0), a.n_buckets - 1);
-    return a.table[(size_t)bucket * a.Hq + head] * LOG2E;
+    const float v = a.table[(size_t)bucket * a.Hq + head];
+    // (finite entries stay finite: the type's lowest value masks like any other large negative one)
+    return __builtin_isinf(v) ? v : v != v ? v : fminf(fmaxf(v * LOG2E, -FLT_MAX), FLT_MAX);
+}
+// A finite bias, however low, only ever weighs a key against others.  So that a row of which nothing else is left still gets
+// the softmax of its scores, a reference (the row's maximum, or near it) that is far from zero is taken from the bias before
+// the score comes to it, in the backward too, which for the same reason finds it apart from log2(l).  A moderate one
+// is taken from the sum, as rounded: the exponent of a row's only key is then zero, and its result the key's value.
+__device__ __forceinline__ bool band_remote(float top) { return __any(fabsf(top) > 1024.f); }
+// log2(e) * logit - top
+__device__ __forceinline__ float band_exponent(float s, float c, float bias, float top, bool remote) {
+    return remote ? __builtin_fmaf(s, c, bias - top) : __builtin_fmaf(s, c, bias) - top;
+}
+__device__ __forceinline__ void band_keep(const BandArgs &a, size_t at, bool off, float top, float l) {
+    const float log_l = off ? INFINITY : __builtin_amdgcn_logf(l);
+    if (a.top) a.top[at] = off ? 0.f : top;
+    a.lse[at] = a.top || off ? log_l : top + log_l;
 }
 __device__ __forceinline__ void band_stage_bias(const BandArgs &a, int head, int sign, float *dst, int threads) {
     const int n = 2 * (a.M + BAND_MARGIN) + 1;
@@ -499,11 +518,10 @@ __device__ __forceinline__ void band_careful(const BandArgs &a, const T *qrow, c
             if (vis)
                 for (int d = hh; d < a.D; d += 2) s = __builtin_fmaf(io<T>::ld(qrow + d), io<T>::ld(kr + d), s);
             s += __shfl_xor(s, 32, 64);
-            float x = s * a.c;
-            if constexpr (BIAS) x += vis ? band_bias_at(a, head, j - p) : 0.f;
+            const float bias = BIAS && vis ? band_bias_at(a, head, j - p) : 0.f, x = __builtin_fmaf(s, a.c, bias);
             const float mn = vis ? fmaxf(m, x) : m;
             const float alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-            const float e = vis ? __builtin_amdgcn_exp2f(x - mn) : 0.f;
+            const float e = vis && x != -INFINITY ? __builtin_amdgcn_exp2f(band_exponent(s, a.c, bias, mn, band_remote(vis ? mn : 0.f))) : 0.f;
             m = mn;
             l = l * alpha + (hh == 0 ? e : 0.f);
 #pragma unroll

@@ -20,11 +20,12 @@ template <typename T, int DP, int MODE, bool BIAS>
 __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void band_attn_dkv_kernel(const BandArgs a) {
     constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE), C = DP / 16;
     constexpr bool AHEAD = DP < 128 && (sizeof(T) == 2 || DP == 32);  // registers for LDS reads well ahead of the products that need them
+    constexpr int STATS = BIAS ? 4 : 2;
     using Stage = BandStage<T, DP, MODE>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     T *const lds = reinterpret_cast<T *>(smem);                        // [NB][Q | dO]
-    float *const stats = reinterpret_cast<float *>(lds + NB * 2 * ELEMS);  // [NB][-lse | delta][64]
-    float *const bias = stats + NB * 2 * BAND_TILE;
+    float *const stats = reinterpret_cast<float *>(lds + NB * 2 * ELEMS);  // [NB][-lse - top | delta | top | -lse][64]
+    float *const bias = stats + NB * STATS * BAND_TILE;
 
     const int nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS, units = a.sink_blocks * a.sink_chunks + (nkb - a.sink_blocks) * a.chunks;
     const int idx = band_piece_of(blockIdx.x, gridDim.x, units);
@@ -72,12 +73,13 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
     gs.init(a.dout.s.l, a.D);
     auto fetch = [&](int tile, int h, T *image) {
         const int i0 = tile * BAND_TILE;
-        if (threadIdx.x < 2 * BAND_TILE) {
+        if (threadIdx.x < STATS * BAND_TILE) {
             const int i = i0 + (threadIdx.x & (BAND_TILE - 1));
-            const bool of_lse = threadIdx.x < BAND_TILE;
-            const float *src = (of_lse ? a.lse : a.delta) + ((size_t)b * a.Hq + h) * a.Lq;
-            const float v = src[min(i, sq.qn - 1)];
-            st = of_lse ? (i < sq.qn ? -v : -INFINITY) : v;
+            const int stat = threadIdx.x / BAND_TILE;
+            const size_t at = ((size_t)b * a.Hq + h) * a.Lq + min(i, sq.qn - 1);
+            st = (stat == 1 ? a.delta : stat == 2 ? a.top : a.lse)[at];
+            if (BIAS && stat == 0) st += a.top[at];
+            if (stat == 0 || stat == 3) st = i < sq.qn ? -st : -INFINITY;
         }
         qs.fetch(reinterpret_cast<const char *>(band_row<T>(a.q, b, i0, h)), sq.qn - 1 - i0, a.D, image);
         gs.fetch(reinterpret_cast<const char *>(band_row<T>(a.dout, b, i0, h)), sq.qn - 1 - i0, a.D, image + ELEMS);
@@ -87,7 +89,7 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
     bool new_head = true;
     for (int step = begin; step < end; ++step) {
         T *const Q = lds + (NB == 2 ? ((step - begin) & 1) : 0) * 2 * ELEMS, *const G = Q + ELEMS;
-        float *const S = stats + (NB == 2 ? ((step - begin) & 1) : 0) * 2 * BAND_TILE;
+        float *const S = stats + (NB == 2 ? ((step - begin) & 1) : 0) * STATS * BAND_TILE;
         if constexpr (NB == 1) lds_barrier();
         if constexpr (BIAS) {
             if (new_head) {
@@ -101,7 +103,7 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
             qs.put(Q, a.D);
             gs.put(G, a.D);
         }
-        if (threadIdx.x < 2 * BAND_TILE) S[threadIdx.x] = st;
+        if (threadIdx.x < STATS * BAND_TILE) S[threadIdx.x] = st;
         if constexpr (Stage::DIRECT) lds_barrier();
         const int i0 = tile * BAND_TILE;
         new_head = tile + 1 == first + n_tiles;
@@ -136,7 +138,7 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
                 }
             }
             typename band_t<T>::frag gc[2][DP / 32], qc[2][DP / 32];
-            if (AHEAD) {
+            auto columns_ahead = [&]() {
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -144,9 +146,23 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
                         gc[k][db] = band_cols<DP>(G, 32 * u + 16 * k, db, lane);
                         qc[k][db] = band_cols<DP>(Q, 32 * u + 16 * k, db, lane);
                     }
-            }
+            };
+            if (AHEAD && !BIAS) columns_ahead();
+            float cs = a.c;
             if constexpr (BIAS) {
-                if (j_lo - p_hi < a.M && j_hi - p_lo > -a.M) {
+                const bool near = j_lo - p_hi < a.M && j_hi - p_lo > -a.M;
+                if (band_remote(S[2 * BAND_TILE + 32 * u + l31])) {
+                    // top and lse apart, and one row after the other: this is rare, and must not cost registers
+                    cs = 1.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int row = 32 * u + 4 * hh + rho(r), e = near ? p_lo + 4 * hh + rho(r) - j + a.M + BAND_MARGIN : j_lo > p_hi ? 0 : 2 * (a.M + BAND_MARGIN);
+                        s[r] = band_exponent(s[r], a.c, bias[e], S[2 * BAND_TILE + row], true);
+                        nl[r] = S[3 * BAND_TILE + row];
+                        asm volatile("" ::: "memory");
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                } else if (near) {
                     const float *br = bias + (p_lo + 4 * hh - j + a.M + BAND_MARGIN);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) nl[r] += br[rho(r)];
@@ -156,8 +172,9 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
                     for (int r = 0; r < 16; ++r) nl[r] += bu;
                 }
             }
+            if (AHEAD && BIAS) columns_ahead();  // (behind the bias, which has no registers to spare)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, nl[r]));
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], cs, nl[r]));
             if (!full) {
                 // the mask from the key's side: position p sees key j when p >= j - right and (p <= j + left or j < sinks)
                 const int p_min = key_on ? j - a.right - p_lo - 4 * hh : BAND_FAR, p_max = j < a.sinks ? BAND_FAR : j + a.left - p_lo - 4 * hh;
@@ -293,7 +310,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
         }
     }
     const size_t stat = ((size_t)b * a.Hq + h) * a.Lq + i;
-    const float nl = row_on ? -a.lse[stat] : -INFINITY;
+    const float nl = row_on ? -a.lse[stat] : -INFINITY, top = BIAS && row_on ? a.top[stat] : 0.f;
+    const bool remote = BIAS && band_remote(top);
     // delta = dout . out, from the result before its rounding where that was kept (in three parts of 8 bits).  It is the
     // diagonal of a product formed like dout v^T below: for a row that sees a single key, whose result is that key's value,
     // the two are then the same number and dS is exactly zero.
@@ -402,10 +420,15 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
                 near = j0 + 31 - w_lo > -M && j0 - w_hi < M;
                 if (near) {
                     cs = 1.f;
+                    if (remote) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], scale, bias[e0 + rho(r)]);
+                        for (int r = 0; r < 16; ++r) s[r] = band_exponent(s[r], scale, bias[e0 + rho(r)], top, true);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[r] = band_exponent(s[r], scale, bias[e0 + rho(r)], top, false);
+                    }
                 } else {
-                    shift += bias[j0 > w_hi ? BL - 1 : 0];
+                    shift += bias[j0 > w_hi ? BL - 1 : 0] - top;
                 }
             }
 #pragma unroll
@@ -557,7 +580,7 @@ template <typename T, int DP, int MODE, bool BIAS, bool DTABLE> static int launc
         if (int rc = check_launch("dsw_band_attn_bwd (dq)")) return rc;
     }
     if (a.Lk) {
-        const size_t lds = images + (size_t)band_t<T>::nbuf(DP) * 2 * BAND_TILE * sizeof(float) + bl;
+        const size_t lds = images + (size_t)band_t<T>::nbuf(DP) * (BIAS ? 4 : 2) * BAND_TILE * sizeof(float) + bl;
         auto kern = band_attn_dkv_kernel<T, DP, MODE, BIAS>;
         if (int rc = allow_lds(kern, lds)) return rc;
         const long long nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS, heads = (long long)a.B * a.Hkv;
@@ -616,6 +639,7 @@ extern "C" int dsw_band_attn_bwd(const dsw_band_desc *d, const void *q, const ds
     const size_t need = dsw_band_attn_bwd_workspace(d);
     DSW_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "%s: workspace of %zu bytes, %zu are needed", who, workspace_bytes, need);
     a.lse = const_cast<float *>(lse);
+    a.top = a.table && lse ? a.lse + (size_t)a.B * a.Hq * a.Lq : nullptr;
     a.out32 = const_cast<float *>(out32);
     a.delta = static_cast<float *>(workspace);
     const BandChunks chunks = band_chunks(a, d->dtype);

@@ -13,6 +13,7 @@ namespace dsw {
 template <typename T, int DP, int MODE, bool BIAS, bool EXACT>
 __global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof(T) == 4 || EXACT ? 2 : 3)) void band_attn_fwd_kernel(const BandArgs a_) {
     constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE), C = DP / 16;
+    constexpr bool KEEP = sizeof(T) == 4 || EXACT;  // (probabilities that are not rounded to bf16: see band_exponent)
     using Stage = BandStage<T, DP, MODE>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     T *const lds = reinterpret_cast<T *>(smem);  // [NB][K | V]
@@ -111,19 +112,6 @@ __global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof
                             for (int u = 0; u < 2; ++u) s[u] = band_mma(kf[u][c], qf[c], s[u]);
                     }
                 }
-                float cs = scale, bu = 0.f;  // the logits are cs * s + bu
-                if constexpr (BIAS) {
-                    if (j + BAND_TILE - 1 - w_lo > -M && j - w_hi < M) {
-                        const float *br = bias + (j + 4 * hh - p + M + BAND_MARGIN);
-                        cs = 1.f;
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) s[u][r] = __builtin_fmaf(s[u][r], scale, br[32 * u + rho(r)]);
-                    } else {
-                        bu = bias[j > w_hi ? 2 * (M + BAND_MARGIN) : 0];  // (all distances clipped: one bias)
-                    }
-                }
                 if (edges.cut_hi(j)) {
                     const int hi = key_hi - j - 4 * hh;
 #pragma unroll
@@ -139,11 +127,26 @@ __global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof
                         for (int r = 0; r < 16; ++r)
                             s[u][r] = (int)(32 * u + rho(r) >= lo) | (int)(32 * u + rho(r) < first) ? s[u][r] : -INFINITY;
                 }
+                // the logits are scale * s + bu, or, where distances of the tile are not clipped, scale * s + br[..]
+                float bu = 0.f;
+                const float *const br = bias + (j + 4 * hh - p + M + BAND_MARGIN);
+                bool near = false;
+                if constexpr (BIAS) {
+                    near = j + BAND_TILE - 1 - w_lo > -M && j - w_hi < M;
+                    if (!near) bu = bias[j > w_hi ? 2 * (M + BAND_MARGIN) : 0];
+                }
                 if (fresh || safe) {
                     float x = s[0][0];
+                    if (near) {
+                        x = -INFINITY;
 #pragma unroll
-                    for (int r = 1; r < 32; ++r) x = fmaxf(x, s[r >> 4][r & 15]);
-                    x = max_across_halves(__builtin_fmaf(x, cs, bu));
+                        for (int r = 0; r < 32; ++r) x = fmaxf(x, __builtin_fmaf(s[r >> 4][r & 15], scale, br[32 * (r >> 4) + rho(r & 15)]));
+                    } else {
+#pragma unroll
+                        for (int r = 1; r < 32; ++r) x = fmaxf(x, s[r >> 4][r & 15]);
+                        x = __builtin_fmaf(x, scale, bu);
+                    }
+                    x = max_across_halves(x);
                     const float mn = m == -INFINITY || safe ? fmaxf(m, x) : m;
                     const float alpha = mn == m || m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
                     m = mn;
@@ -154,7 +157,31 @@ __global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof
                         for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
                     fresh = __any((int)row_on & (int)(m == -INFINITY));
                 }
-                const float shift = bu - (m == -INFINITY ? 0.f : m);
+                const float mr = m == -INFINITY ? 0.f : m;
+                if constexpr (BIAS || KEEP) {
+                    if (near && !band_remote(mr)) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[u][r] = band_exponent(s[u][r], scale, br[32 * u + rho(r)], mr, false);
+                    } else if (near) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[u][r] = band_exponent(s[u][r], scale, br[32 * u + rho(r)], mr, true);
+                    } else if (!BIAS) {  // (with a bias a row's only key is its own position's: near)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[u][r] = band_exponent(s[u][r], scale, bu, mr, false);
+                    } else {
+                        const float shift = bu - mr;
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[u][r] = __builtin_fmaf(s[u][r], scale, shift);
+                    }
+                }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     typename band_t<T>::frag vf[2][DP / 32];
@@ -164,7 +191,7 @@ __global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof
                         for (int db = 0; db < DP / 32; ++db) vf[k][db] = band_cols<DP>(V, 32 * u + 16 * k, db, lane);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], cs, shift));
+                    for (int r = 0; r < 16; ++r) s[u][r] = __builtin_amdgcn_exp2f(BIAS || KEEP ? s[u][r] : __builtin_fmaf(s[u][r], scale, -mr));
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         typename band_t<T>::frag pf;
@@ -231,7 +258,7 @@ __global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof
     if constexpr (EXACT)  // (in mode 0 D is a multiple of 8)
         band_store_row<float, DP, MODE>(a.out32 + (((size_t)at.b * a.Lq + at.i) * a.Hq + at.h) * a.D, o, inv, a.D, hh, store);
     if (a.lse && store && hh == 0)
-        a.lse[((size_t)at.b * a.Hq + at.h) * a.Lq + at.i] = !row_on || l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+        band_keep(a, ((size_t)at.b * a.Hq + at.h) * a.Lq + at.i, !row_on || l == 0.f, m, l);
 }
 
 template <typename T, int DP, int MODE, bool BIAS, bool EXACT> static int launch_fwd(const BandArgs &a, hipStream_t st) {
@@ -318,6 +345,7 @@ extern "C" int dsw_band_attn_fwd(const dsw_band_desc *d, const void *q, const ds
         return rc;
     DSW_REQUIRE(out32 == nullptr || (a.table && d->dtype == DSW_BF16), "%s: out32 goes with a bias table and bf16 tensors", who);
     a.lse = lse;
+    a.top = lse && a.table ? lse + (size_t)a.B * a.Hq * a.Lq : nullptr;
     a.out32 = out32;
     hipStream_t st = as_stream(stream);
     if (out32 == nullptr && band_step_plan(*d, a.nrb, a.nsplit)) {

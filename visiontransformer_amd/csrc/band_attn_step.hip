@@ -106,14 +106,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
         for (int c = 0; c < DP / 16; ++c) s = band_mma(kf[c], qf[c], s);
         if (t + 4 < t_end) load(tiles.at(t + 4) * STEP_KEYS);
         const BandMask mask = band_row_mask(a, p, sq.kn, j0 + 4 * hh);
-        float x = -INFINITY;
+        float x = -INFINITY, bias[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int j = j0 + rho(r) + 4 * hh;
-            float y = s[r] * a.c;
-            if constexpr (BIAS) y += row < R ? band_bias_at(a, h, j - p) : 0.f;
-            s[r] = mask.sees(rho(r)) ? y : -INFINITY;
-            x = fmaxf(x, s[r]);
+            bias[r] = BIAS && row < R ? band_bias_at(a, h, j - p) : 0.f;
+            s[r] = mask.sees(rho(r)) ? s[r] : -INFINITY;
+            x = fmaxf(x, __builtin_fmaf(s[r], a.c, bias[r]));
         }
         x = max_across_halves(x);
         if (__any(x > m + 8.f)) {
@@ -126,9 +125,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
                 for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
         }
         const float shift = m == -INFINITY ? 0.f : m;
+        const bool remote = BIAS && band_remote(shift);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            s[r] = __builtin_amdgcn_exp2f(s[r] - shift);
+            s[r] = __builtin_amdgcn_exp2f(band_exponent(s[r], a.c, bias[r], shift, remote));
             l += s[r];
         }
 #pragma unroll
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
             const int ro = rb * 32 + rl, io_ = ro / a.G, ho = hk * a.G + ro - io_ * a.G;
             const bool off = den == 0.f || io_ >= sq.qn;
             io<T>::st(const_cast<T *>(band_row<T>(a.out, b, io_, ho)) + d, off ? 0.f : sum / den);
-            if (a.lse && d == 0) a.lse[((size_t)b * a.Hq + ho) * a.Lq + io_] = off ? INFINITY : mx + __builtin_amdgcn_logf(den);
+            if (a.lse && d == 0) band_keep(a, ((size_t)b * a.Hq + ho) * a.Lq + io_, off, mx, den);
         } else {
             float *const ws = a.partial + (((size_t)bh * a.nrb + rb) * a.nsplit + sp) * 32 * (a.D + 2);
             ws[rl * (a.D + 2) + d] = sum;
@@ -226,7 +226,7 @@ template <typename T> __global__ __launch_bounds__(256) void band_attn_join_kern
     const bool off = den == 0.f || i >= band_seq(a, b).qn;
     const int d = threadIdx.x;
     if (d < a.D) io<T>::st(const_cast<T *>(band_row<T>(a.out, b, i, h)) + d, off ? 0.f : ((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) / den);
-    if (a.lse && d == 0) a.lse[((size_t)b * a.Hq + h) * a.Lq + i] = off ? INFINITY : mt + __builtin_amdgcn_logf(den);
+    if (a.lse && d == 0) band_keep(a, ((size_t)b * a.Hq + h) * a.Lq + i, off, mt, den);
 }
 
 // Few rows: at most 32 rows of a key head, or too few of the other kernel's workgroups (128 rows of a head) for the chip.

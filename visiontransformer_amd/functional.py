@@ -2572,7 +2572,7 @@ class _BandAttnFn(torch.autograd.Function):
         desc = _BandAttnFn._desc(q, k, tab, buckets, q_lens, k_lens, *settings)
         train = any(ctx.needs_input_grad[:4])
         exact = train and ctx.needs_input_grad[3] and q.dtype == torch.bfloat16
-        lse = torch.empty(B, Hq, Lq, dtype=torch.float32, device=dev) if train else None
+        lse = torch.empty(1 if tab is None else 2, B, Hq, Lq, dtype=torch.float32, device=dev) if train else None
         out32 = torch.empty(B, Lq, Hq, D, dtype=torch.float32, device=dev) if exact else None
         if B * Lq * Hq:
             n = 0 if exact else _workspace("fwd", desc)
