@@ -144,3 +144,23 @@ def test_cache_refusals_on_the_cpu():
         c.append(z[:1, :1], z[:1, :1])
     with pytest.raises(RuntimeError, match="KVCache"):
         c.append(z[:, :0].half(), z[:, :0].half())
+
+
+def test_cache_counts_and_refusals():
+    from visiontransformer_amd.sequence import KVCache
+    cache = KVCache(2, 8, 3, 4, dtype=torch.float32, device="cpu")
+    k, v = torch.randn(2, 5, 3, 4), torch.randn(2, 5, 3, 4)
+    cache.append(k, v, torch.tensor([2, 2 ** 33], dtype=torch.int64))       # (clamped to the batch's 5, not wrapped)
+    assert cache.lens.tolist() == [2, 5] and cache.longest == 5
+    cache.append(k[:, :3], v[:, :3])
+    assert cache.lens.tolist() == [5, 8]
+    assert torch.equal(cache.tokens()[0][0, :5], torch.cat([k[0, :2], k[0, :3]])) and torch.equal(cache.tokens()[1][1], torch.cat([v[1], v[1, :3]]))
+    fresh = KVCache(2, 8, 3, 4, dtype=torch.float32, device="cpu")
+    for args in ((k.requires_grad_(), v), (k.detach(), v, torch.tensor([1])), (k.detach().double(), v), (k.detach()[:1], v)):
+        with pytest.raises(RuntimeError, match="KVCache"):
+            fresh.append(*args)
+    with pytest.raises(RuntimeError, match="capacity"):
+        cache.append(k.detach()[:, :1], v[:, :1])
+    with torch.no_grad():
+        fresh.append(k, v)
+    assert fresh.lens.tolist() == [5, 5] and not fresh.k.requires_grad

@@ -2626,7 +2626,10 @@ def band_attention(q, k, v, window=(None, None), sinks=0, scale=None, q_lens=Non
 
     bias_table [n, Hq] with bias_buckets int32 [2 M + 1], M <= 512: table[bias_buckets[clip(j - p, -M, M) + M], head] is
     added to the scaled logits (sequence.BucketedPositionBias holds both).  scale: D ** -0.5 by default, positive.
-    Gradients: q, k, v, bias_table.  Calls of few query rows without gradients split the keys over the chip."""
+    An entry of -inf masks its keys; a finite one, however low, only weighs them: a row that sees no others gets the softmax of
+    their scores.
+    Gradients: q, k, v, bias_table (the backward wants finite keys and values in every row before k_len, seen or not).
+    Calls of few query rows, and short ones, split the keys over the chip."""
     who = "band_attention"
     _same_kind(who, {"q": q, "k": k, "v": v})
     B, Lq, Hq, D = q.shape

@@ -64,8 +64,9 @@ class KVCache:
     """Keys and values of up to `capacity` tokens per sequence, [B, heads, capacity, D] (a head's rows together), with the
     number of tokens of each sequence on the device.  Rows behind a sequence are never read, so nothing is cleared.
 
-    append() writes new tokens behind what each sequence holds, without a host synchronisation; the host keeps only the
-    largest count, and refuses what would not fit.  Inside a captured graph the device counts advance with every replay
+    append() writes new tokens behind what each sequence holds, without a host synchronisation; the host keeps only what
+    the longest sequence can hold at most (`longest`, which counts a batch's padding too), and refuses what might not fit.
+    No gradients.  Inside a captured graph the device counts advance with every replay
     and the host's does not: a loop of replays has to count for itself and stay within `capacity`."""
 
     def __init__(self, batch, capacity, num_heads, head_dim, dtype=torch.bfloat16, device="cuda"):
@@ -81,6 +82,10 @@ class KVCache:
         if (k.shape != v.shape or B != self.k.shape[0] or k.shape[2:] != (self.k.shape[1], self.k.shape[3]) or k.dtype != self.k.dtype
                 or v.dtype != self.k.dtype):
             raise RuntimeError("visiontransformer_amd: KVCache: %s %s tokens for a cache of %s %s" % (tuple(k.shape), k.dtype, tuple(self.k.shape), self.k.dtype))
+        if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+            raise RuntimeError("visiontransformer_amd: KVCache: a cache is for inference (torch.no_grad())")
+        if lens is not None and tuple(lens.shape) != (B,):
+            raise RuntimeError("visiontransformer_amd: KVCache: lens must be [%d], got %s" % (B, tuple(lens.shape)))
         if self.longest + n > self.capacity:
             raise RuntimeError("visiontransformer_amd: KVCache: %d + %d tokens exceed the capacity of %d" % (self.longest, n, self.capacity))
         if n:
@@ -89,7 +94,7 @@ class KVCache:
             rows = torch.arange(B, device=self.lens.device)[:, None]
             self.k.transpose(1, 2)[rows, place] = k
             self.v.transpose(1, 2)[rows, place] = v
-        self.lens += n if lens is None else lens.to(torch.int32).clamp(0, n)
+        self.lens += n if lens is None else lens.clamp(0, n).to(torch.int32)
         self.longest += n
         return self
 
