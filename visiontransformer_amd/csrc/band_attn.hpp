@@ -41,7 +41,7 @@ struct BandArgs {
     float *out32;        // [B][Lq][Hq][D] or null
     float *delta;        // [B][Hq][Lq]
     float *partial;      // step kernel: see there; dQ kernel: bias gradients by distance
-    int nsplit, nrb;
+    int nsplit, nrb, staged;  // step kernel; staged: floats of the bias by head and distance in LDS, or 0
     float *shares;       // dK, dV kernel: sums of the blocks that several workgroups share
     int sink_blocks, sink_chunks, chunks;
 };

@@ -20,7 +20,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    T *const V = reinterpret_cast<T *>(smem) + wave * ELEMS;
+    // [heads of the key head][2 M + 1] biases, where two workgroups a CU leave the room; then four V tiles, where the waves' sums
+    // meet in the end
+    float *const bias_of = reinterpret_cast<float *>(smem);
+    unsigned char *const room = smem + (BIAS ? a.staged * sizeof(float) : 0);
+    T *const V = reinterpret_cast<T *>(room) + wave * ELEMS;
 
     const int sp = blockIdx.x % a.nsplit, rest = blockIdx.x / a.nsplit;
     const int rb = rest % a.nrb, bh = rest / a.nrb, hk = bh % a.Hkv, b = bh / a.Hkv;
@@ -35,6 +39,15 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     const int share = (tiles.count + a.nsplit - 1) / a.nsplit, t_end = min((sp + 1) * share, tiles.count);
     const int t_begin = sp * share + wave;
 
+    const float *const bias_row = bias_of + (row - i * a.G) * (2 * a.M + 1) + a.M;
+    if (BIAS && a.staged) {
+        const int n = 2 * a.M + 1;
+        for (int e = threadIdx.x; e < a.G * n; e += 256) {
+            const int g = e / n;
+            bias_of[e] = band_bias_at(a, hk * a.G + g, e - g * n - a.M);
+        }
+        __syncthreads();
+    }
     const T *const qrow = band_row<T>(a.q, b, i, h);
     const T *const kbase = band_row<T>(a.k, b, 0, hk);
     const T *const vbase = band_row<T>(a.v, b, 0, hk);
@@ -110,7 +123,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int j = j0 + rho(r) + 4 * hh;
-            bias[r] = BIAS && row < R ? band_bias_at(a, h, j - p) : 0.f;
+            bias[r] = 0.f;
+            if constexpr (BIAS) {
+                if (a.staged) bias[r] = bias_row[min(max(j - p, -a.M), a.M)];
+                else if (row < R) bias[r] = band_bias_at(a, h, j - p);
+            }
             s[r] = mask.sees(rho(r)) ? s[r] : -INFINITY;
             x = fmaxf(x, __builtin_fmaf(s[r], a.c, bias[r]));
         }
@@ -151,7 +168,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     l += __shfl_xor(l, 32, 64);
     __syncthreads();
     const int nrow = min(32, R - rb * 32);
-    float *const ml = reinterpret_cast<float *>(smem);  // [4][32][2]
+    float *const ml = reinterpret_cast<float *>(room);  // [4][32][2]
     float *const os = ml + 4 * 32 * 2;                   // [4][nrow][D]
     if (hh == 0) ml[(wave * 32 + l31) * 2] = m, ml[(wave * 32 + l31) * 2 + 1] = l;
     __syncthreads();
@@ -235,22 +252,30 @@ bool band_step_plan(const dsw_band_desc &d, int &nrb, int &nsplit) {
     const long long R = (long long)d.Lq * (d.Hq / d.Hkv);
     if (R > 32 && (long long)d.B * d.Hq * ((d.Lq + BAND_ROWS - 1) / BAND_ROWS) >= 256) return false;
     nrb = (int)((R + 31) / 32);
-    const long long span = d.left < 0 ? d.Lk : (long long)d.left + d.Lq + (d.right > 0 ? d.right : 0) + d.sinks + 2 * STEP_KEYS;
+    const long long G = d.Hq / d.Hkv, tokens = d.Lq < 31 / G + 2 ? d.Lq : 31 / G + 2;  // of a block of 32 rows
+    const long long span = d.left < 0 || d.right < 0 ? d.Lk : (long long)d.left + tokens + d.right + d.sinks + 2 * STEP_KEYS;
     const long long tiles = ((span < d.Lk ? span : d.Lk) + STEP_KEYS - 1) / STEP_KEYS, units = (long long)d.B * d.Hkv * nrb;
     // as many workgroups as are resident at a time (two a CU in wide heads' registers, else four), with two tiles per wave at
     // least.  One token over 16 x 8 windows of 1028 keys of 128: 31 us at 2 to 4 shares, 35 at 1, 40 at 6 and 8; over 8 x 4
-    // caches of up to 32768 keys of 64: 44 us at 32 shares, 47 at 16 and at 64 (graph replays, with the join).
-    const long long want = d.D > 64 ? 512 : 1024, most = (tiles + 7) / 8;
+    // caches of up to 32768 keys of 64: 44 us at 32 shares, 47 at 16 and at 64 (graph replays, with the join).  Where there are
+    // several row blocks, one workgroup a CU: their many rows make the join dear (2 x 777 rows of 4 heads of 48, window 255,
+    // fp32: 23.5 us at one share, 23.3 and 12.7 for the join at two).
+    const long long want = nrb > 1 ? 256 : d.D > 64 ? 512 : 1024, most = (tiles + 7) / 8;
     long long n = want / units;
     n = n < most ? n : most;
     nsplit = (int)(n < 1 ? 1 : n > STEP_MAX_SPLITS ? STEP_MAX_SPLITS : n);
     return true;
 }
 
-template <typename T, int DP, int MODE, bool BIAS> static int launch_step(const BandArgs &a, hipStream_t st) {
+// Biases through LDS (two dependent loads for each of a tile's 1024 otherwise: 32 us for 28, 3 x 1098 tokens, 3 heads of 32,
+// window 183, fp32, with three shares) while two workgroups fit on a CU beside the widest one's 66 KB.
+constexpr int STEP_BIAS_FLOATS = 3584;
+template <typename T, int DP, int MODE, bool BIAS> static int launch_step(BandArgs &a, hipStream_t st) {
     const int R = a.Lq * a.G, nrow = R < 32 ? R : 32;
     const size_t tile = (size_t)4 * band_t<T>::template elems<DP>(STEP_KEYS) * sizeof(T);
-    const size_t meet = (size_t)(4 * 32 * 2 + 4 * nrow * a.D) * sizeof(float), lds = tile > meet ? tile : meet;
+    const size_t meet = (size_t)(4 * 32 * 2 + 4 * nrow * a.D) * sizeof(float), n_bias = (size_t)a.G * (2 * a.M + 1);
+    a.staged = BIAS && n_bias <= STEP_BIAS_FLOATS ? (int)((n_bias + 3) & ~(size_t)3) : 0;
+    const size_t lds = (tile > meet ? tile : meet) + a.staged * sizeof(float);
     auto kern = band_attn_step_kernel<T, DP, MODE, BIAS>;
     if (lds > 65536) {
         hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
