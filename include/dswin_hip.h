@@ -6,7 +6,9 @@
  * The reference is pure PyTorch and has no FFI of its own; each entry point below
  * replaces the torch / torchvision call sequence cited next to it.  Conventions:
  *   - every pointer is a DEVICE pointer owned by the caller (nothing is allocated,
- *     freed or retained by the library); `stream` is a hipStream_t passed as void*;
+ *     freed or retained by the library), but for dsw_strides and dsw_band_desc, which
+ *     lie in host memory and are read before the call returns; `stream` is a
+ *     hipStream_t passed as void*;
  *   - every function only enqueues work on `stream` and returns at once, never
  *     synchronises, keeps no mutable global state and may be called concurrently
  *     from several host threads (forward thread and autograd worker threads);
