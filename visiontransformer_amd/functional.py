@@ -2486,14 +2486,14 @@ class _QKNormRotaryFn(torch.autograd.Function):
         axes, pairs = (0, 0) if freqs is None else freqs.shape
         blocks = _lib.load().dsw_qk_norm_rotary_blocks(dtype_code(q.dtype), B, L, Hq, Hkv, D, axes, pairs)
         both = partial = None
-        if want_w:   # the workgroups' shares and, behind them, the two gradients
+        if want_w:
             ran = B * L * (Hq + Hkv) > 0
-            both = (torch.empty if ran else torch.zeros)((blocks if ran else 0) + 1, 2, D, dtype=torch.float32, device=dev)
-            partial, both = (both.data_ptr() if ran else None), both[-1]
+            both = (torch.empty if ran else torch.zeros)(2, D, dtype=torch.float32, device=dev)
+            partial = torch.empty(blocks * 2 * D, dtype=torch.float32, device=dev) if ran else None
         if B * L:
             spec = _QKNormRotaryFn._spec(q, Hkv, wq, wk, freqs, positions, *ctx.settings)
             _call_on(dev, "dsw_qk_norm_rotary_bwd", pq, sq, pk, sk, pdyq, sdyq, pdyk, sdyk, *spec, pdq, sdq, pdk, sdk,
-                     partial, both.data_ptr() if partial else None, stream(dev))
+                     ptr(partial), None if partial is None else both.data_ptr(), stream(dev))
         dw = [None if w is None or both is None else both[i].to(t) for i, (w, t) in enumerate(zip((wq, wk), ctx.weight_dtypes))]
         return dq, dk, dw[0], dw[1], None, None, None, None
 
