@@ -134,6 +134,13 @@ def test_attention_with_bias(cuda0, case, buckets, distance, dtype):
 
 
 @pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("D", [30, 64, 128])
+def test_the_longest_bias_map(cuda0, dtype, D):
+    """512 distances to each side: the most LDS that a call takes"""
+    _check_attention(cuda0, (1, 90, 700, 2, 2, D, None, None, 0, None, "dense"), dtype, 14, 64, 512)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
 def test_bias_without_its_gradient(cuda0, dtype):
     _check_attention(cuda0, BIAS_CASES[1][0], dtype, 13, 32, 128, table_grad=False)
 

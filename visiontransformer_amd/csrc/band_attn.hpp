@@ -536,6 +536,15 @@ __device__ __forceinline__ void band_careful(const BandArgs &a, const T *qrow, c
         }
 }
 
+// Allows a kernel the LDS of its launch: always as much as any of these launches takes, so that calls of different sizes from
+// several threads leave each other's limit alone.
+constexpr size_t BAND_LDS = 128 * 1024;
+template <typename K> int band_allow_lds(const char *who, K kern, size_t lds) {
+    if (lds <= 65536) return DSW_OK;
+    if (lds > BAND_LDS) return fail(DSW_EUNSUPPORTED, "%s: %zu bytes of LDS", who, lds);
+    hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)BAND_LDS);
+    return e == hipSuccess ? DSW_OK : fail(DSW_ELAUNCH, "%s: %zu bytes of LDS: %s", who, lds, hipGetErrorString(e));
+}
 int band_make_args(const char *who, const dsw_band_desc *d, BandArgs &a);
 // fills t and raises `mode` to what the tensor needs
 int band_tensor(const char *who, const char *name, const void *p, const dsw_strides *s, int dtype, int D, bool null_ok, BandTensor &t, int &mode);

@@ -557,12 +557,6 @@ __global__ __launch_bounds__(256) void band_attn_table_kernel(const float *__res
     if (threadIdx.x == 0) d_table[(size_t)bucket * heads + h] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-template <typename K> static int allow_lds(K kern, size_t lds) {
-    if (lds <= 65536) return DSW_OK;
-    hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    return e == hipSuccess ? DSW_OK : fail(DSW_ELAUNCH, "dsw_band_attn_bwd: %zu bytes of LDS: %s", lds, hipGetErrorString(e));
-}
-
 // rows of a dq workgroup: 64 while 128 would leave SIMDs without a wave
 static int band_dq_rows(const BandArgs &a) {
     return (long long)a.B * a.Hq * ((a.Lq + BAND_ROWS - 1) / BAND_ROWS) < 256 ? BAND_ROWS / 2 : BAND_ROWS;
@@ -575,14 +569,14 @@ template <typename T, int DP, int MODE, bool BIAS, bool DTABLE> static int launc
         const size_t lds = images + (DTABLE ? ((bl + 15) & ~(size_t)15) + 4 * (32 * 64 * sizeof(float) + bl) : bl);
         const bool split = band_dq_rows(a) < BAND_ROWS;
         auto kern = split ? band_attn_dq_kernel<T, DP, MODE, BIAS, DTABLE, true> : band_attn_dq_kernel<T, DP, MODE, BIAS, DTABLE, false>;
-        if (int rc = allow_lds(kern, lds)) return rc;
+        if (int rc = band_allow_lds("dsw_band_attn_bwd", kern, lds)) return rc;
         kern<<<dim3((unsigned)((long long)a.B * a.Hq * ((a.Lq + band_dq_rows(a) - 1) / band_dq_rows(a)))), 256, lds, st>>>(a);
         if (int rc = check_launch("dsw_band_attn_bwd (dq)")) return rc;
     }
     if (a.Lk) {
         const size_t lds = images + (size_t)band_t<T>::nbuf(DP) * (BIAS ? 4 : 2) * BAND_TILE * sizeof(float) + bl;
         auto kern = band_attn_dkv_kernel<T, DP, MODE, BIAS>;
-        if (int rc = allow_lds(kern, lds)) return rc;
+        if (int rc = band_allow_lds("dsw_band_attn_bwd", kern, lds)) return rc;
         const long long nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS, heads = (long long)a.B * a.Hkv;
         kern<<<dim3((unsigned)(heads * (a.sink_blocks * a.sink_chunks + (nkb - a.sink_blocks) * a.chunks))), 256, lds, st>>>(a);
         if (int rc = check_launch("dsw_band_attn_bwd (dk, dv)")) return rc;

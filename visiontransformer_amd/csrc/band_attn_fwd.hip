@@ -273,10 +273,7 @@ template <typename T, int DP, int MODE, bool BIAS, bool EXACT> static int launch
     const size_t lds = (size_t)band_t<T>::nbuf(DP) * 2 * band_t<T>::template elems<DP>(BAND_TILE) * sizeof(T) +
                        (BIAS ? (2 * (a.M + BAND_MARGIN) + 1) * sizeof(float) : 0);
     auto kern = band_attn_fwd_kernel<T, DP, MODE, BIAS, EXACT>;
-    if (lds > 65536) {
-        hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (e != hipSuccess) return fail(DSW_ELAUNCH, "dsw_band_attn_fwd: %zu bytes of LDS: %s", lds, hipGetErrorString(e));
-    }
+    if (int rc = band_allow_lds("dsw_band_attn_fwd", kern, lds)) return rc;
     const long long grid = (long long)a.B * a.Hq * ((a.Lq + BAND_ROWS - 1) / BAND_ROWS);
     kern<<<dim3((unsigned)grid), 256, lds, st>>>(a);
     return check_launch("dsw_band_attn_fwd");

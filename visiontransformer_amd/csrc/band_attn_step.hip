@@ -277,10 +277,7 @@ template <typename T, int DP, int MODE, bool BIAS> static int launch_step(BandAr
     a.staged = BIAS && n_bias <= STEP_BIAS_FLOATS ? (int)((n_bias + 3) & ~(size_t)3) : 0;
     const size_t lds = (tile > meet ? tile : meet) + a.staged * sizeof(float);
     auto kern = band_attn_step_kernel<T, DP, MODE, BIAS>;
-    if (lds > 65536) {
-        hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (e != hipSuccess) return fail(DSW_ELAUNCH, "dsw_band_attn_fwd: %zu bytes of LDS: %s", lds, hipGetErrorString(e));
-    }
+    if (int rc = band_allow_lds("dsw_band_attn_fwd", kern, lds)) return rc;
     const long long grid = (long long)a.B * a.Hkv * a.nrb * a.nsplit;
     if (grid >= (1LL << 31)) return fail(DSW_EUNSUPPORTED, "dsw_band_attn_fwd: %lld workgroups", grid);
     kern<<<dim3((unsigned)grid), 256, lds, st>>>(a);
