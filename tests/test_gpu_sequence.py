@@ -549,6 +549,38 @@ def test_qk_norm_rotary(cuda0, case, positions, dtype):
 # ----------------------------------------------------------------------------------------------
 # the operators together: sequence.BandedMSA
 # ----------------------------------------------------------------------------------------------
+def test_qk_norm_rotary_captured_and_replayed(cuda0):
+    """a training pass in a graph, with new inputs and eager work between the replays, against the eager result"""
+    K = _K()
+    gen = torch.Generator(device=cuda0).manual_seed(9)
+    st = {"q": torch.randn(3, 700, 6, 30, device=cuda0, generator=gen).to(BF), "k": torch.randn(3, 700, 2, 30, device=cuda0, generator=gen).to(BF),
+          "wq": torch.randn(30, device=cuda0, generator=gen), "wk": torch.randn(30, device=cuda0, generator=gen)}
+    freqs, pos = torch.rand(2, 7, device=cuda0, generator=gen), torch.randint(0, 64, (700, 2), device=cuda0, generator=gen)
+
+    def work():
+        leaves = [t.detach().requires_grad_() for t in st.values()]
+        out = K.qk_norm_rotary(*leaves, freqs, pos)
+        return [t.detach() for t in out] + list(torch.autograd.grad(out, leaves, (st["q"], st["k"])))
+
+    side = torch.cuda.Stream(cuda0)
+    side.wait_stream(torch.cuda.current_stream(cuda0))
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream(cuda0).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = work()
+    for n in range(4):
+        for t in st.values():
+            t.copy_(torch.randn(t.shape, device=cuda0, generator=gen))
+        pos.add_(17 * n)
+        graph.replay()
+        got = [t.clone() for t in held]
+        for x, y in zip(got, work()):
+            assert torch.equal(x, y)
+        torch.cuda.synchronize()
+
+
 def _module_in_64_bits(mod, x, positions, lens=None):
     """BandedMSA by plain tensor operations in the dtype of its (double) parameters"""
     B, L, C = x.shape
