@@ -428,6 +428,7 @@ __device__ __forceinline__ bool band_remote(float top) { return __any(fabsf(top)
 __device__ __forceinline__ float band_exponent(float s, float c, float bias, float top, bool remote) {
     return remote ? __builtin_fmaf(s, c, bias - top) : __builtin_fmaf(s, c, bias) - top;
 }
+// what a row leaves for its backward: top + log2(l), or with a bias the two apart
 __device__ __forceinline__ void band_keep(const BandArgs &a, size_t at, bool off, float top, float l) {
     const float log_l = off ? INFINITY : __builtin_amdgcn_logf(l);
     if (a.top) a.top[at] = off ? 0.f : top;
