@@ -1,0 +1,56 @@
+"""The token-sequence operators under autograd, what needs no GPU: the library's calls are recorded instead of launched."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """functional with CPU tensors and recorded library calls (name, arguments)"""
+    from visiontransformer_amd import _lib, functional as K
+    made = []
+    monkeypatch.setattr(_lib, "require_cuda", lambda *tensors: None)
+    monkeypatch.setattr(K, "stream", lambda device=None: 0)
+    monkeypatch.setattr(K, "_call_on", lambda device, name, *args: made.append((name, args)))
+    return made
+
+
+def _attention(*args, **kw):
+    from visiontransformer_amd import functional as K
+    return K.band_attention(*args, **kw)
+
+
+def _rotary(*args, **kw):
+    from visiontransformer_amd import functional as K
+    return K.qk_norm_rotary(*args, **kw)[0]
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_forward_mode_derivatives_are_refused(calls, grad, which):
+    """a dual input, with gradients enabled and without: an error, not a result without its tangent"""
+    x = torch.randn(1, 4, 2, 8)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        args = [x.clone(), x.clone(), x.clone()]
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(x))
+        with pytest.raises(NotImplementedError):
+            _attention(*args)
+        if which < 2:
+            with pytest.raises(NotImplementedError):
+                _rotary(*args[:2])
+        weight = forward_ad.make_dual(torch.ones(8), torch.ones(8))
+        with pytest.raises(NotImplementedError):
+            _rotary(x, x, weight)
+        assert _attention(x, x, x).shape == _rotary(x, x).shape == x.shape      # (no dual input: an ordinary call)
+
+
+def test_calls_without_gradients_save_nothing(calls):
+    x = torch.randn(1, 4, 2, 8)
+    for out in (_attention(x, x, x), _rotary(x, x)):
+        assert out.grad_fn is None
+    y = x.clone().requires_grad_()
+    with torch.no_grad():
+        for out in (_attention(y, x, x), _rotary(y, x)):
+            assert not out.requires_grad
+    for out in (_attention(y, x, x), _rotary(y, x)):
+        assert out.grad_fn is not None

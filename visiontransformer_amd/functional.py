@@ -11,6 +11,7 @@ import weakref
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import call, dtype_code, ptr, stream
@@ -2390,6 +2391,13 @@ def _fail(who, text):
     raise RuntimeError("visiontransformer_amd: %s: %s" % (who, text))
 
 
+def _differentiate(*tensors):
+    """whether a call has to go through autograd: gradients are wanted, or forward-mode derivatives may be (which the
+    Function refuses; its forward alone would drop the tangents without a word, also where gradients are disabled)"""
+    return (forward_ad._current_level >= 0
+            or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
+
+
 def _call_on(device, name, *args):
     """call() with `device` as the current one: the tensors' device need not be"""
     if torch.cuda.current_device() == device.index:
@@ -2508,7 +2516,7 @@ def qk_norm_rotary(q, k, q_weight=None, k_weight=None, freqs=None, positions=Non
     pair c = a * P + i of the first 2 A P columns turns by positions[..., a] * freqs[a, i], where a pair is the columns
     (c, c + A P), or (2 c, 2 c + 1) when interleaved; the columns behind them are only normalised.  None: norm only.
     positions: int32 or int64, None: the token's index on every axis.  Angles are taken in 64 bits.
-    Gradients: q, k and the two weights (not freqs)."""
+    Gradients: q, k and the two weights (not freqs); forward-mode derivatives are refused."""
     who = "qk_norm_rotary"
     _same_kind(who, {"q": q, "k": k})
     B, L, _, D = q.shape
@@ -2532,7 +2540,7 @@ def qk_norm_rotary(q, k, q_weight=None, k_weight=None, freqs=None, positions=Non
         positions = _device_ints(who, "positions", positions, q.device, ((L,), (B, L)) if flat else ((L, A), (B, L, A)))
         if positions is not None and (flat or not positions.is_contiguous()):
             positions = (positions.unsqueeze(-1) if flat else positions).contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+    if _differentiate(q, k, q_weight, k_weight):
         return _QKNormRotaryFn.apply(q, k, q_weight, k_weight, freqs, positions, float(eps), bool(interleaved))
     return _QKNormRotaryFn.forward(_NO_GRAD, q, k, q_weight, k_weight, freqs, positions, float(eps), bool(interleaved))
 
@@ -2628,7 +2636,8 @@ def band_attention(q, k, v, window=(None, None), sinks=0, scale=None, q_lens=Non
     added to the scaled logits (sequence.BucketedPositionBias holds both).  scale: D ** -0.5 by default, positive.
     An entry of -inf masks its keys; a finite one, however low, only weighs them: a row that sees no others gets the softmax of
     their scores.
-    Gradients: q, k, v, bias_table (the backward wants finite keys and values in every row before k_len, seen or not).
+    Gradients: q, k, v, bias_table (the backward wants finite keys and values in every row before k_len, seen or
+    not); forward-mode derivatives are refused.
     Calls of few query rows, and short ones, split the keys over the chip."""
     who = "band_attention"
     _same_kind(who, {"q": q, "k": k, "v": v})
@@ -2664,6 +2673,6 @@ def band_attention(q, k, v, window=(None, None), sinks=0, scale=None, q_lens=Non
         bias_buckets = bias_buckets.to(torch.int32).contiguous()
     args = (q, k, v, bias_table, bias_buckets, q_lens, k_lens, -1 if left is None else int(left), -1 if right is None else int(right),
             int(sinks), scale)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias_table)):
+    if _differentiate(q, k, v, bias_table):
         return _BandAttnFn.apply(*args)
     return _BandAttnFn.forward(_NO_GRAD, *args)
