@@ -54,3 +54,38 @@ def test_calls_without_gradients_save_nothing(calls):
             assert not out.requires_grad
     for out in (_attention(y, x, x), _rotary(y, x)):
         assert out.grad_fn is not None
+
+
+def test_copies_of_saved_tensors_live_until_the_launch(calls, monkeypatch):
+    """a hook that returns saved tensors with a strided last dimension: the dense copies that the kernels read are alive when
+    they are launched"""
+    import weakref
+    from visiontransformer_amd import functional as K
+    given = []
+    rows = K._head_rows
+
+    def head_rows(t):
+        r = rows(t)
+        given.append((weakref.ref(r[0]), r[2]))
+        return r
+
+    def launch(device, name, *args):
+        calls.append(name)
+        if name.endswith("_bwd"):
+            for alive, address in given:
+                assert alive() is not None and alive().data_ptr() == address, name
+
+    def strided(t):
+        if t.dim() != 4 or t.shape[-1] != 8:      # (rows of heads only)
+            return t
+        return t.transpose(2, 3).contiguous().transpose(2, 3)
+
+    monkeypatch.setattr(K, "_head_rows", head_rows)
+    monkeypatch.setattr(K, "_call_on", launch)
+    for run in (lambda a, b, c: _attention(a, b, c), lambda a, b, c: _rotary(a, b)):
+        leaves = [torch.randn(1, 4, 2, 8, requires_grad=True) for _ in range(3)]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, strided):
+            out = run(*leaves)
+        given.clear()
+        out.sum().backward()
+    assert [n for n in calls if n.endswith("_bwd")] == ["dsw_band_attn_bwd", "dsw_qk_norm_rotary_bwd"]

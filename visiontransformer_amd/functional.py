@@ -2484,8 +2484,9 @@ class _QKNormRotaryFn(torch.autograd.Function):
         q, k, wq, wk, freqs, positions = ctx.saved_tensors
         B, L, Hq, D = q.shape
         Hkv, dev = k.shape[2], q.device
-        _, sq, pq = _head_rows(q)
-        _, sk, pk = _head_rows(k)
+        # (a hook may hand saved tensors back in other strides: a copy that is made of one has to live until the launch)
+        q, sq, pq = _head_rows(q)
+        k, sk, pk = _head_rows(k)
         dyq, sdyq, pdyq = _head_rows(dyq.to(q.dtype))
         dyk, sdyk, pdyk = _head_rows(dyk.to(q.dtype))
         dq, sdq, pdq = _new_rows(B, L, Hq, D, q.dtype, dev)
@@ -2601,9 +2602,9 @@ class _BandAttnFn(torch.autograd.Function):
         grads = [t[0] for t in made]
         d_tab = torch.empty_like(tab) if tab is not None and ctx.needs_input_grad[3] else None
         if q.shape[0] * q.shape[2] * max(q.shape[1], k.shape[1]):
-            operands = []
-            for t in (q, k, v, out):
-                operands += _head_rows(t)[:0:-1]
+            # (a hook may hand saved tensors back in other strides: a copy that is made of one has to live until the launch)
+            rows = [_head_rows(t) for t in (q, k, v, out)]
+            operands = [x for r in rows for x in r[:0:-1]]
             operands.append(ptr(out32))
             dout, s, p = _head_rows(dout.to(q.dtype))
             operands += [p, s, ptr(lse)]
