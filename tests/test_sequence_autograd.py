@@ -89,3 +89,22 @@ def test_copies_of_saved_tensors_live_until_the_launch(calls, monkeypatch):
         given.clear()
         out.sum().backward()
     assert [n for n in calls if n.endswith("_bwd")] == ["dsw_band_attn_bwd", "dsw_qk_norm_rotary_bwd"]
+
+
+@pytest.mark.parametrize("shape,launched", [((1, 4, 5, 0, 2), True), ((1, 4, 5, 0, 0), False), ((1, 0, 5, 2, 1), True), ((1, 4, 0, 2, 1), True),
+                                            ((0, 4, 5, 2, 1), False), ((1, 0, 0, 2, 1), False)])
+def test_backward_is_launched_wherever_there_is_a_gradient_to_write(calls, shape, launched):
+    """also without query heads: the gradients of k and v are zeros then, which the library writes"""
+    B, Lq, Lk, Hq, Hkv = shape
+    leaves = [torch.randn(B, n, h, 8, requires_grad=True) for n, h in ((Lq, Hq), (Lk, Hkv), (Lk, Hkv))]
+    _attention(*leaves).sum().backward()
+    assert ("dsw_band_attn_bwd" in [n for n, _ in calls]) == launched
+
+
+def test_sizes_of_calls_without_query_heads():
+    """the C entries count workspaces of such a call as of any other"""
+    import ctypes
+    from visiontransformer_amd import _lib
+    for sinks in (0, 3):
+        d = _lib.BandDesc(dtype=1, B=1, Lq=4, Lk=8, Hq=0, Hkv=2, D=32, left=-1, right=0, sinks=sinks, scale=0.1)
+        assert _lib.load().dsw_band_attn_bwd_workspace(ctypes.byref(d)) == _lib.load().dsw_band_attn_fwd_workspace(ctypes.byref(d)) == 0

@@ -253,7 +253,7 @@ template <typename T, int V> __global__ __launch_bounds__(256) void band_attn_jo
 static BandChunks band_chunks(const BandArgs &a, int dtype) {
     BandChunks c = {0, 1, 1, 0};
     const long long nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS, heads = (long long)a.B * a.Hkv, tiles = (a.Lq + BAND_TILE - 1) / BAND_TILE;
-    if (nkb == 0 || heads == 0 || tiles == 0) return c;
+    if (nkb == 0 || heads == 0 || tiles == 0 || a.G == 0) return c;  // (nothing, or zeros, to write)
     const long long window = (long long)a.left + a.right + BAND_ROWS, reach = window >= a.Lq ? tiles : window / BAND_TILE + 2;
     const long long normal = (reach < tiles ? reach : tiles) * a.G;  // steps of a block in the middle
     const long long want = dtype == DSW_F32 ? 1024 : a.D > 64 ? 256 : 512, n = (want + heads * nkb - 1) / (heads * nkb), most = normal / (dtype == DSW_F32 ? 2 : 8);
@@ -570,7 +570,7 @@ static int band_dq_rows(const BandArgs &a) {
 template <typename T, int DP, int MODE, bool BIAS, bool DTABLE> static int launch_bwd(const BandArgs &a, hipStream_t st) {
     const size_t images = (size_t)band_t<T>::nbuf(DP) * 2 * band_t<T>::template elems<DP>(BAND_TILE) * sizeof(T);
     const size_t bl = BIAS ? (2 * (a.M + BAND_MARGIN) + 1) * sizeof(float) : 0;
-    if (a.Lq) {
+    if (a.Lq && a.Hq) {
         const size_t lds = images + (DTABLE ? ((bl + 15) & ~(size_t)15) + 4 * (32 * 64 * sizeof(float) + bl) : bl);
         const bool split = band_dq_rows(a) < BAND_ROWS;
         auto kern = split ? band_attn_dq_kernel<T, DP, MODE, BIAS, DTABLE, true> : band_attn_dq_kernel<T, DP, MODE, BIAS, DTABLE, false>;
@@ -620,8 +620,8 @@ extern "C" int dsw_band_attn_bwd(const dsw_band_desc *d, const void *q, const ds
     BandArgs a;
     int rc = band_make_args(who, d, a);
     if (rc) return rc;
-    if (a.B == 0 || a.Hq == 0) return DSW_OK;
-    const bool no_rows = a.Lq == 0, no_keys = a.Lk == 0;
+    if (a.B == 0 || a.Hkv == 0) return DSW_OK;
+    const bool no_rows = a.Lq == 0 || a.Hq == 0, no_keys = a.Lk == 0;  // (no query heads: dk and dv are zeros all the same)
     int mode = 0;
     if ((rc = band_tensor(who, "q", q, sq, d->dtype, a.D, no_rows, a.q, mode)) || (rc = band_tensor(who, "k", k, sk, d->dtype, a.D, no_keys, a.k, mode)) ||
         (rc = band_tensor(who, "v", v, sv, d->dtype, a.D, no_keys, a.v, mode)) || (rc = band_tensor(who, "out", out, so, d->dtype, a.D, no_rows, a.out, mode)) ||
@@ -650,7 +650,7 @@ extern "C" int dsw_band_attn_bwd(const dsw_band_desc *d, const void *q, const ds
         rc = d_table ? launch_bwd<T, DP, MODE, true, true>(a, st)
              : a.table ? launch_bwd<T, DP, MODE, true, false>(a, st) : launch_bwd<T, DP, MODE, false, false>(a, st);
     });
-    if (rc || d_table == nullptr) return rc;
+    if (rc || d_table == nullptr || a.Hq == 0) return rc;
     band_attn_table_kernel<<<dim3(a.n_buckets, a.Hq), 256, 0, st>>>(a.partial, a.buckets, (int)rows, n, a.n_buckets, a.Hq, d_table);
     return check_launch("dsw_band_attn_bwd (table)");
 }

@@ -2601,7 +2601,7 @@ class _BandAttnFn(torch.autograd.Function):
         made = [_new_rows(*t.shape, t.dtype, dev) for t in (q, k, v)]
         grads = [t[0] for t in made]
         d_tab = torch.empty_like(tab) if tab is not None and ctx.needs_input_grad[3] else None
-        if q.shape[0] * q.shape[2] * max(q.shape[1], k.shape[1]):
+        if q.numel() or k.numel():
             # (a hook may hand saved tensors back in other strides: a copy that is made of one has to live until the launch)
             rows = [_head_rows(t) for t in (q, k, v, out)]
             operands = [x for r in rows for x in r[:0:-1]]
