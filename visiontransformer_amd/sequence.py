@@ -84,8 +84,9 @@ class KVCache:
             raise RuntimeError("visiontransformer_amd: KVCache: %s %s tokens for a cache of %s %s" % (tuple(k.shape), k.dtype, tuple(self.k.shape), self.k.dtype))
         if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
             raise RuntimeError("visiontransformer_amd: KVCache: a cache is for inference (torch.no_grad())")
-        if lens is not None and tuple(lens.shape) != (B,):
-            raise RuntimeError("visiontransformer_amd: KVCache: lens must be [%d], got %s" % (B, tuple(lens.shape)))
+        if lens is not None and (tuple(lens.shape) != (B,) or lens.dtype not in (torch.int32, torch.int64) or lens.device != self.lens.device):
+            raise RuntimeError("visiontransformer_amd: KVCache: lens must be int32 or int64 [%d] on %s, got %s %s on %s" % (
+                B, self.lens.device, lens.dtype, tuple(lens.shape), lens.device))
         if self.longest + n > self.capacity:
             raise RuntimeError("visiontransformer_amd: KVCache: %d + %d tokens exceed the capacity of %d" % (self.longest, n, self.capacity))
         if n:
