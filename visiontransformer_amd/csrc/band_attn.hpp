@@ -268,6 +268,14 @@ template <int DP> __device__ __forceinline__ band_t<float>::frag band_cols(const
 // of the first LDS read of any image; m0, which carries their destination, is used by nothing else in these kernels.
 // Otherwise fetch() loads registers and put() writes the image; in mode 1 the last piece of a row is the one that ends
 // with it, and clear() has to have zeroed the columns past D once.
+// What lanes exchange through LDS: neither the barrier nor a wave's in-order LDS accesses are by themselves something that the
+// compiler keeps loads and stores on their side of.
+__device__ __forceinline__ void band_fence() { asm volatile("" ::: "memory"); }
+__device__ __forceinline__ void band_barrier() {
+    band_fence();
+    lds_barrier();
+    band_fence();
+}
 __device__ __forceinline__ void band_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ uint32_t band_lds_address(const void *p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p;

@@ -95,10 +95,10 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
     for (int step = begin; step < end; ++step) {
         T *const Q = lds + (NB == 2 ? ((step - begin) & 1) : 0) * 2 * ELEMS, *const G = Q + ELEMS;
         float *const S = stats + (NB == 2 ? ((step - begin) & 1) : 0) * STATS * BAND_TILE;
-        if constexpr (NB == 1) lds_barrier();
+        if constexpr (NB == 1) band_barrier();
         if constexpr (BIAS) {
             if (new_head) {
-                lds_barrier();  // the last head's readers are done
+                band_barrier();  // the last head's readers are done
                 band_stage_bias(a, hk * a.G + g, -1, bias, 256);
             }
         }
@@ -109,13 +109,13 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
             gs.put(G, a.D);
         }
         if (threadIdx.x < STATS * BAND_TILE) S[threadIdx.x] = st;
-        if constexpr (Stage::DIRECT) lds_barrier();
+        if constexpr (Stage::DIRECT) band_barrier();
         const int i0 = tile * BAND_TILE;
         new_head = tile + 1 == first + n_tiles;
         tile = new_head ? first : tile + 1;
         g += new_head;
         if (step + 1 < end) fetch(tile, hk * a.G + g, lds + (NB == 2 ? ((step + 1 - begin) & 1) : 0) * 2 * ELEMS);
-        if constexpr (!Stage::DIRECT) lds_barrier();
+        if constexpr (!Stage::DIRECT) band_barrier();
 #pragma unroll 1
         for (int u = 0; u < 2; ++u) {
             const int r0 = i0 + 32 * u, p_lo = sq.off + r0, p_hi = sq.off + min(r0 + 31, sq.qn - 1);
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
                         const int row = 32 * u + 4 * hh + rho(r), e = near ? p_lo + 4 * hh + rho(r) - j + a.M + BAND_MARGIN : j_lo > p_hi ? 0 : 2 * (a.M + BAND_MARGIN);
                         s[r] = band_exponent(s[r], a.c, bias[e], S[2 * BAND_TILE + row], true);
                         nl[r] = S[3 * BAND_TILE + row];
-                        asm volatile("" ::: "memory");
+                        band_fence();
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 } else if (near) {
@@ -376,9 +376,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
         T *const K = lds + (NB == 2 ? (it & 1) : 0) * 2 * ELEMS, *const V = K + ELEMS;
         if constexpr (Stage::DIRECT) {
             band_landed();
-            lds_barrier();
+            band_barrier();
         } else {
-            if constexpr (NB == 1) lds_barrier();
+            if constexpr (NB == 1) band_barrier();
             ks.put(K, D);
             vs.put(V, D);
         }
@@ -391,7 +391,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
             ks.fetch(kw.p, sq.kn - 1 - jt, D, K1);
             vs.fetch(vw.p, sq.kn - 1 - jt, D, K1 + ELEMS);
         }
-        if constexpr (!Stage::DIRECT) lds_barrier();
+        if constexpr (!Stage::DIRECT) band_barrier();
 #pragma unroll 1
         for (int u = SPLIT ? wave >> 1 : 0; u < (SPLIT ? (wave >> 1) + 1 : 2); ++u) {
             const int j0 = tile + 32 * u;
@@ -456,16 +456,16 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
                 // of LDS, in no order, took 140 cycles for each of the 16 registers.
                 if (near) {
                     float *const mine = slant + wave * 32 * 64;
-                    asm volatile("" ::: "memory");
+                    band_fence();
 #pragma unroll
                     for (int r = 0; r < 16; ++r) mine[l31 * 63 + 31 + 4 * hh + rho(r)] = s[r];
-                    asm volatile("" ::: "memory");  // (a wave's LDS accesses complete in order)
+                    band_fence();  // (a wave's LDS accesses complete in order)
                     float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int k = 0; k < 32; ++k) part[k & 3] += mine[64 * k + lane];
                     float *const at_distance = sums + wave * BL + (j0 - w_lo + lane - 31 + M + BAND_MARGIN);
                     *at_distance += (part[0] + part[1]) + (part[2] + part[3]);
-                    asm volatile("" ::: "memory");
+                    band_fence();
                 } else {
                     float t = 0.f;
 #pragma unroll

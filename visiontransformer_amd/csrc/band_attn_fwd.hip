@@ -78,9 +78,9 @@ __global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof
                 T *const K = lds + (NB == 2 ? (it & 1) : 0) * 2 * ELEMS, *const V = K + ELEMS;
                 if constexpr (Stage::DIRECT) {
                     band_landed();
-                    lds_barrier();
+                    band_barrier();
                 } else {
-                    if constexpr (NB == 1) lds_barrier();
+                    if constexpr (NB == 1) band_barrier();
                     ks.put(K, D);
                     vs.put(V, D);
                 }
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof
                     ks.fetch(kw.p, sq.kn - 1 - j1, D, K1);
                     vs.fetch(vw.p, sq.kn - 1 - j1, D, K1 + ELEMS);
                 }
-                if constexpr (!Stage::DIRECT) lds_barrier();
+                if constexpr (!Stage::DIRECT) band_barrier();
                 const int j = j0;
                 j0 = j1;
                 if (edges.none(j)) continue;

@@ -115,7 +115,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     if (t_begin < t_end) load(tiles.at(t_begin) * STEP_KEYS);
     for (int t = t_begin; t < t_end; t += 4) {
         const int j0 = tiles.at(t) * STEP_KEYS;
+        band_fence();  // (the last tile's reads of V come first, this one's after: a wave's LDS accesses complete in order)
         put();
+        band_fence();
         f32x16 s = band_zero();
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) s = band_mma(kf[c], qf[c], s);
