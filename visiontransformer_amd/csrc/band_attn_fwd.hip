@@ -224,14 +224,17 @@ __global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof
                         }
                     }
                 }
-                if (__any(l > 0x1p60f)) {  // far above the reference: move it up
-                    const float up = l > 0x1p60f ? 0x1p-60f : 1.f, both = fminf(up, __shfl_xor(up, 32, 64));
-                    m += both < 1.f ? 60.f : 0.f;
-                    l *= both;
+                if (__any(l > 0x1p60f)) {
+                    // far above the reference: move it up, by what the sum comes to (a large reference takes no step of 60
+                    // exactly, the largest ones none at all)
+                    const float up = l > 0x1p60f ? 60.f : 0.f, to = m + fmaxf(up, __shfl_xor(up, 32, 64));
+                    const float down = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
+                    m = to;
+                    l *= down;
 #pragma unroll
                     for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) o[db][r] *= both;
+                        for (int r = 0; r < 16; ++r) o[db][r] *= down;
                 }
             }
             float bad = l * 0.f;
