@@ -1,5 +1,7 @@
 """Attention over token sequences at the edges of what a call may be: sizes, biases and scores that a test of ordinary calls
 does not reach."""
+import math
+
 import pytest
 import torch
 
@@ -47,3 +49,66 @@ def test_equal_keys_weigh_the_same_wherever_they_stand(cuda0, dtype):
     for n in (L, 3):
         out = K.band_attention(on(torch.ones(1, L, 1, D), H)[:, L - n:], on(k, H), on(v, H), scale=1 / 1.4426950408889634).double().cpu()
         assert bool(((out - want).abs() <= want * (2.0 ** -8 if dtype == BF else 2.0 ** -22)).all())
+
+
+LEVELS = {"high": [0, 80, 160, 250], "higher": [250, 250, 0, 250], "low": [-250, -200, -220, -150], "lower": [-100, -250, -250, -200]}
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("value", [torch.finfo(FP).min, -1e30, -1e9, -1e6, -3e3, torch.finfo(FP).max, 1e9])
+@pytest.mark.parametrize("levels", list(LEVELS))
+@pytest.mark.parametrize("B,L,Hq,Hkv,D,table_grad", [(1, 250, 2, 1, 64, True), (2, 250, 4, 2, 30, False), (16, 250, 16, 8, 64, True), (16, 250, 16, 8, 30, False),
+                                                     (16, 250, 16, 16, 128, False)])
+def test_biases_far_from_zero_leave_the_softmax_of_large_scores(cuda0, B, L, Hq, Hkv, D, table_grad, levels, value, dtype):
+    """A table of one finite number, however far from zero: the softmax of the scores alone, and its gradients, also where the
+    scores (levels of base-2 logits by tile of 64 keys; whole numbers, exact in both types) leave fp32's exponents.  Small calls, with
+    their split form, and calls that fill the chip; without gradients as well."""
+    from oracle import sequence_oracle as S
+    from test_gpu_sequence import _within
+    K = _K()
+    gen = torch.Generator().manual_seed(D)
+    level = torch.tensor(LEVELS[levels], dtype=FP).repeat_interleave(64)[:L]
+    k = (level.view(1, L, 1, 1) + torch.randint(-3, 4, (1, L, Hkv, D), generator=gen)).to(dtype)
+    q, v, dout = torch.ones(1, L, Hq, D).to(dtype), torch.randn(1, L, Hkv, D, generator=gen).to(dtype), torch.randn(1, L, Hq, D, generator=gen).to(dtype)
+    bmap = torch.randint(0, 4, (2 * 40 + 1,), generator=gen, dtype=torch.int32)
+    scale = math.log(2) / D
+    ref = S.attention(q.double(), k.double(), v.double(), 150, 0, 20, scale, table=torch.zeros(4, Hq, dtype=torch.float64), buckets=bmap,
+                      dout=dout.double(), dtype=dtype, table_grad=table_grad)
+    on = lambda t: t.to(cuda0).expand(B, -1, -1, -1).contiguous()
+    leaves = [on(t).requires_grad_() for t in (q, k, v)] + [torch.full((4, Hq), value, device=cuda0).requires_grad_(table_grad)]
+    kw = dict(window=(150, 0), sinks=20, scale=scale, bias_table=leaves[3], bias_buckets=bmap.to(cuda0))
+    out = K.band_attention(*leaves[:3], **kw)
+    grads = torch.autograd.grad(out, leaves[:4 if table_grad else 3], on(dout))
+    with torch.no_grad():
+        again = K.band_attention(*leaves[:3], **kw)
+    for name, got in [("out", out), ("out (no grad)", again)] + list(zip(("dq", "dk", "dv"), grads)):
+        want, bound = ref[name.split(" ")[0]]
+        _within(name, got, want.expand(B, -1, -1, -1), bound.expand(B, -1, -1, -1))
+    if table_grad:      # (B equal sequences: their sum)
+        want, bound = ref["dtable"]
+        _within("dtable", grads[3], B * want, B * (bound + B * S.F * want.abs()))
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("value", [torch.finfo(FP).min, -1e9])
+@pytest.mark.parametrize("levels", list(LEVELS))
+@pytest.mark.parametrize("D", [30, 128])
+def test_new_tokens_whose_biases_are_all_far_from_zero(cuda0, D, levels, value, dtype):
+    """the same for single rows over long caches, whose keys are shared out"""
+    from oracle import sequence_oracle as S
+    from test_gpu_sequence import _within
+    K = _K()
+    gen = torch.Generator().manual_seed(D)
+    L = 4000
+    level = torch.tensor(LEVELS[levels], dtype=FP).repeat_interleave(1000)
+    k = (level.view(1, L, 1, 1) + torch.randint(-3, 4, (1, L, 2, D), generator=gen)).to(dtype)
+    q, v = torch.ones(1, 1, 4, D).to(dtype), torch.randn(1, L, 2, D, generator=gen).to(dtype)
+    bmap = torch.zeros(2 * 40 + 1, dtype=torch.int32)
+    scale = math.log(2) / D
+    lens = torch.tensor([4000, 0, 1, 1700], dtype=torch.int32)
+    four = lambda t: t.expand(4, -1, -1, -1).contiguous()
+    ref = S.attention(four(q).double(), four(k).double(), four(v).double(), None, 0, 0, scale, k_lens=lens, dtype=dtype)["out"]
+    with torch.no_grad():
+        out = K.band_attention(four(q).to(cuda0), four(k).to(cuda0), four(v).to(cuda0), window=(None, 0), scale=scale, k_lens=lens.to(cuda0),
+                               bias_table=torch.full((1, 4), value, device=cuda0), bias_buckets=bmap.to(cuda0))
+    _within("out", out, *ref)

@@ -436,9 +436,13 @@ __device__ __forceinline__ bool band_remote(float top) { return __any(fabsf(top)
 __device__ __forceinline__ float band_exponent(float s, float c, float bias, float top, bool remote) {
     return remote ? __builtin_fmaf(s, c, bias - top) : __builtin_fmaf(s, c, bias) - top;
 }
-// what a row leaves for its backward: top + log2(l), or with a bias the two apart
-__device__ __forceinline__ void band_keep(const BandArgs &a, size_t at, bool off, float top, float l) {
-    const float log_l = off ? INFINITY : __builtin_amdgcn_logf(l);
+// What is left of a score beside a reference that swallowed it (beyond 2^31 its rounding alone is a hundred) may overflow, or
+// leave nothing of any key.  Rows whose denominator comes out of the middle of fp32's range are done again by band_careful.
+// (The reference's own key gives 2^0 else, so that nothing is below and only what climbs above; rows without a key: m = -inf.)
+__device__ __forceinline__ bool band_strayed(float m, float l) { return m != -INFINITY && !(l >= 0x1p-64f && l <= 0x1p100f); }
+// what a row leaves for its backward: top + log2(l), or with a bias the two apart; l is the sum of 2^(exponent - lift)
+__device__ __forceinline__ void band_keep(const BandArgs &a, size_t at, bool off, float top, float lift, float l) {
+    const float log_l = off ? INFINITY : __builtin_amdgcn_logf(l) + lift;
     if (a.top) a.top[at] = off ? 0.f : top;
     a.lse[at] = a.top || off ? log_l : top + log_l;
 }
@@ -508,14 +512,15 @@ struct BandPlace {
 
 // Non-finite values in keys or values that a row does not see must not reach it: a probability of zero times an
 // infinity is not zero.  The tiles' products cannot tell, so a wave that ends with a non-finite result (seen nowhere
-// else) does its tiles again key by key, touching only what each row sees.  Lane = row as in the kernels; m, l and acc
-// as they leave them (l of one lane half).
+// else) does its tiles again key by key, touching only what each row sees.  So does one whose sums strayed (see there): with a
+// bias the reference has a second part here, `lift`, the largest exponent that is left beside m.  Lane = row as in the kernels;
+// m, l and acc as they leave them (l of one lane half).
 template <typename T, int DP, bool BIAS, int SIZE>
 __device__ __forceinline__ void band_careful(const BandArgs &a, const T *qrow, const T *kbase, const T *vbase, int head, int p,
                                              bool on, int kn, const BandTiles &tiles, int t_begin, int t_end, int t_step, int hh,
-                                             float &m, float &l, f32x16 *acc) {
+                                             float &m, float &lift, float &l, f32x16 *acc) {
     m = -INFINITY;
-    l = 0.f;
+    lift = l = 0.f;
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) acc[db] = band_zero();
     for (int t = t_begin; t < t_end; t += t_step)
@@ -528,10 +533,15 @@ __device__ __forceinline__ void band_careful(const BandArgs &a, const T *qrow, c
                 for (int d = hh; d < a.D; d += 2) s = __builtin_fmaf(io<T>::ld(qrow + d), io<T>::ld(kr + d), s);
             s += __shfl_xor(s, 32, 64);
             const float bias = BIAS && vis ? band_bias_at(a, head, j - p) : 0.f, x = __builtin_fmaf(s, a.c, bias);
-            const float mn = vis ? fmaxf(m, x) : m;
-            const float alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-            const float e = vis && x != -INFINITY ? __builtin_amdgcn_exp2f(band_exponent(s, a.c, bias, mn, band_remote(vis ? mn : 0.f))) : 0.f;
+            const bool counts = vis && x != -INFINITY;
+            const float mn = vis ? fmaxf(m, x) : m, left = band_exponent(s, a.c, bias, mn, BIAS && band_remote(vis ? mn : 0.f));
+            // (what the sums so far are worth beside mn, as an exponent; nothing at first)
+            const float before = m == -INFINITY ? -INFINITY : mn == m ? lift : lift + (m - mn);
+            const float ln = BIAS && counts ? fmaxf(before, left) : BIAS && m != -INFINITY ? before : 0.f;
+            const float alpha = before == ln ? 1.f : __builtin_amdgcn_exp2f(before - ln);
+            const float e = counts ? __builtin_amdgcn_exp2f(left - ln) : 0.f;
             m = mn;
+            lift = ln;
             l = l * alpha + (hh == 0 ? e : 0.f);
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db)
@@ -544,6 +554,9 @@ __device__ __forceinline__ void band_careful(const BandArgs &a, const T *qrow, c
                 }
         }
 }
+
+// floats of a row's share in the split forward: D sums, the reference, the denominator, with a bias the lift
+__host__ __device__ __forceinline__ int band_share_floats(const BandArgs &a) { return a.D + (a.table ? 3 : 2); }
 
 // Allows a kernel the LDS of its launch: always as much as any of these launches takes, so that calls of different sizes from
 // several threads leave each other's limit alone.

@@ -242,8 +242,8 @@ __global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof
             for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) bad = __builtin_fmaf(o[db][r], 0.f, bad);
-            spoiled = __any((int)row_on & (int)(bad != 0.f));
-            // a second time with the maximum over all keys so far as the reference, if anything overflowed
+            spoiled = __any((int)row_on & ((int)(bad != 0.f) | (int)band_strayed(m, l + __shfl_xor(l, 32, 64))));
+            // a second time with the maximum over all keys so far as the reference, if anything overflowed or strayed
             if (safe || !__syncthreads_or(spoiled)) break;
             safe = true;
         }
@@ -255,9 +255,10 @@ __global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof
     const BandArgs &a = *(const BandArgs *)again;
     const BandPlace at(a, block, gridDim.x);
     const bool row_on = at.i < at.sq.qn;
+    float lift = 0.f;
     if (spoiled && safe)
         band_careful<T, DP, BIAS, BAND_TILE>(a, band_row<T>(a.q, at.b, at.i, at.h), band_row<T>(a.k, at.b, 0, at.hk), band_row<T>(a.v, at.b, 0, at.hk),
-                                             at.h, at.sq.off + at.i, row_on, at.sq.kn, at.tiles, 0, at.tiles.count, 1, hh, m, l, o);
+                                             at.h, at.sq.off + at.i, row_on, at.sq.kn, at.tiles, 0, at.tiles.count, 1, hh, m, lift, l, o);
     l += __shfl_xor(l, 32, 64);
     const float inv = !row_on || l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -269,7 +270,7 @@ __global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof
     if constexpr (EXACT)  // (in mode 0 D is a multiple of 8)
         band_store_row<float, DP, MODE>(a.out32 + (((size_t)at.b * a.Lq + at.i) * a.Hq + at.h) * a.D, o, inv, a.D, hh, store);
     if (a.lse && store && hh == 0)
-        band_keep(a, ((size_t)at.b * a.Hq + at.h) * a.Lq + at.i, !row_on || l == 0.f, m, l);
+        band_keep(a, ((size_t)at.b * a.Hq + at.h) * a.Lq + at.i, !row_on || l == 0.f, m, lift, l);
 }
 
 template <typename T, int DP, int MODE, bool BIAS, bool EXACT> static int launch_fwd(const BandArgs &a, hipStream_t st) {
@@ -334,8 +335,7 @@ extern "C" size_t dsw_band_attn_fwd_workspace(const dsw_band_desc *d) {
     int nrb = 0, nsplit = 0;
     BandArgs a;
     if (band_make_args("dsw_band_attn_fwd_workspace", d, a) || !band_step_plan(*d, nrb, nsplit) || nsplit < 2) return 0;
-    // per split and row: D sums, the maximum and the denominator
-    return (size_t)d->B * d->Hkv * nrb * nsplit * 32 * (d->D + 2) * sizeof(float);
+    return (size_t)d->B * d->Hkv * nrb * nsplit * 32 * band_share_floats(a) * sizeof(float);
 }
 
 extern "C" int dsw_band_attn_fwd(const dsw_band_desc *d, const void *q, const dsw_strides *sq, const void *k, const dsw_strides *sk,

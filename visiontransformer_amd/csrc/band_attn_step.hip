@@ -165,21 +165,44 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) bad = __builtin_fmaf(o[db][r], 0.f, bad);
-    if (__any(bad != 0.f))
-        band_careful<T, DP, BIAS, STEP_KEYS>(a, qrow, kbase, vbase, h, p, row_on, sq.kn, tiles, t_begin, t_end, 4, hh, m, l, o);
+    float lift = 0.f;
+    if (__any(bad != 0.f || (BIAS && row_on && band_strayed(m, l + __shfl_xor(l, 32, 64)))))
+        band_careful<T, DP, BIAS, STEP_KEYS>(a, qrow, kbase, vbase, h, p, row_on, sq.kn, tiles, t_begin, t_end, 4, hh, m, lift, l, o);
 
     // the four waves meet: maxima and denominators first, then the sums, scaled to the common maximum
     l += __shfl_xor(l, 32, 64);
     __syncthreads();
     const int nrow = min(32, R - rb * 32);
-    float *const ml = reinterpret_cast<float *>(room);  // [4][32][2]
-    float *const os = ml + 4 * 32 * 2;                   // [4][nrow][D]
-    if (hh == 0) ml[(wave * 32 + l31) * 2] = m, ml[(wave * 32 + l31) * 2 + 1] = l;
-    __syncthreads();
-    float mt = -INFINITY;
+    constexpr int PART = BIAS ? 3 : 2;                   // reference, denominator, lift
+    float *const ml = reinterpret_cast<float *>(room);  // [4][32][PART]
+    float *const os = ml + 4 * 32 * PART;                // [4][nrow][D]
+    // the common reference of a row of the block, and the largest lift beside it
+    auto meet = [&](int r, float &mx, float &top) {
+        mx = -INFINITY, top = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, ml[(w * 32 + l31) * 2]);
-    const float mul = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mt);
+        for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[(w * 32 + r) * PART]);
+        if constexpr (BIAS) {
+            top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float *const x = ml + (w * 32 + r) * PART;
+                top = fmaxf(top, x[0] == -INFINITY ? -INFINITY : (x[0] - mx) + x[2]);
+            }
+            top = mx == -INFINITY ? 0.f : top;
+        }
+    };
+    auto weight = [&](float mw, float lw, float mx, float top) {
+        return mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(BIAS ? (mw - mx) + (lw - top) : mw - mx);
+    };
+    if (hh == 0) {
+        float *const x = ml + (wave * 32 + l31) * PART;
+        x[0] = m, x[1] = l;
+        if constexpr (BIAS) x[2] = lift;
+    }
+    __syncthreads();
+    float mt, top;
+    meet(l31, mt, top);
+    const float mul = weight(m, lift, mt, top);
     if (l31 < nrow) {
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
@@ -194,24 +217,27 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     const int n = nrow * a.D;
     for (int e = threadIdx.x; e < n; e += 256) {
         const int rl = e / a.D, d = e - rl * a.D;
-        float mx = -INFINITY, den = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[(w * 32 + rl) * 2]);
+        float mx, den = 0.f;
+        meet(rl, mx, top);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float mw = ml[(w * 32 + rl) * 2];
-            den += mw == -INFINITY ? 0.f : ml[(w * 32 + rl) * 2 + 1] * __builtin_amdgcn_exp2f(mw - mx);
+            const float *const x = ml + (w * 32 + rl) * PART;
+            den += x[0] == -INFINITY ? 0.f : x[1] * weight(x[0], BIAS ? x[PART - 1] : 0.f, mx, top);
         }
         const float sum = (os[e] + os[n + e]) + (os[2 * n + e] + os[3 * n + e]);
         if (a.nsplit == 1) {
             const int ro = rb * 32 + rl, io_ = ro / a.G, ho = hk * a.G + ro - io_ * a.G;
             const bool off = den == 0.f || io_ >= sq.qn;
             io<T>::st(const_cast<T *>(band_row<T>(a.out, b, io_, ho)) + d, off ? 0.f : sum / den);
-            if (a.lse && d == 0) band_keep(a, ((size_t)b * a.Hq + ho) * a.Lq + io_, off, mx, den);
+            if (a.lse && d == 0) band_keep(a, ((size_t)b * a.Hq + ho) * a.Lq + io_, off, mx, top, den);
         } else {
-            float *const ws = a.partial + (((size_t)bh * a.nrb + rb) * a.nsplit + sp) * 32 * (a.D + 2);
-            ws[rl * (a.D + 2) + d] = sum;
-            if (d == 0) ws[rl * (a.D + 2) + a.D] = mx, ws[rl * (a.D + 2) + a.D + 1] = den;
+            const int W = a.D + PART;
+            float *const ws = a.partial + ((((size_t)bh * a.nrb + rb) * a.nsplit + sp) * 32 + rl) * W;
+            ws[d] = sum;
+            if (d == 0) {
+                ws[a.D] = mx, ws[a.D + 1] = den;
+                if constexpr (BIAS) ws[a.D + 2] = top;
+            }
         }
     }
 }
@@ -222,14 +248,23 @@ template <typename T> __global__ __launch_bounds__(256) void band_attn_join_kern
     __shared__ float weight[STEP_MAX_SPLITS], red[8], sums[4][128];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, R = a.Lq * a.G;
     const int bh = blockIdx.x / R, row = blockIdx.x - bh * R, b = bh / a.Hkv, hk = bh % a.Hkv;
-    const int i = row / a.G, h = hk * a.G + row - i * a.G, W = a.D + 2;
+    const int i = row / a.G, h = hk * a.G + row - i * a.G, W = band_share_floats(a);
     const size_t step = (size_t)32 * W;
     const float *const ws = a.partial + ((size_t)bh * a.nrb + row / 32) * a.nsplit * step + (row & 31) * W;
     const int s0 = threadIdx.x, s1 = threadIdx.x + 256;
     const float m0 = s0 < a.nsplit ? ws[s0 * step + a.D] : -INFINITY, m1 = s1 < a.nsplit ? ws[s1 * step + a.D] : -INFINITY;
     const float d0 = s0 < a.nsplit ? ws[s0 * step + a.D + 1] : 0.f, d1 = s1 < a.nsplit ? ws[s1 * step + a.D + 1] : 0.f;
     const float mt = block_max(fmaxf(m0, m1), red);
-    const float w0 = m0 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m0 - mt), w1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - mt);
+    // exponents of the shares' weights beside the common reference; with a bias less the largest of them (the step kernel's lift)
+    float x0 = m0 == -INFINITY ? -INFINITY : m0 - mt, x1 = m1 == -INFINITY ? -INFINITY : m1 - mt, top = 0.f;
+    if (a.table) {
+        if (m0 != -INFINITY) x0 += ws[s0 * step + a.D + 2];
+        if (m1 != -INFINITY) x1 += ws[s1 * step + a.D + 2];
+        top = block_max(fmaxf(x0, x1), red);
+        top = mt == -INFINITY ? 0.f : top;
+        x0 -= top, x1 -= top;
+    }
+    const float w0 = __builtin_amdgcn_exp2f(x0), w1 = __builtin_amdgcn_exp2f(x1);
     if (s0 < a.nsplit) weight[s0] = w0;
     if (s1 < a.nsplit) weight[s1] = w1;
     const float den = block_sum(__builtin_fmaf(d0, w0, d1 * w1), red + 4);  // (its barriers cover the weights)
@@ -247,7 +282,7 @@ template <typename T> __global__ __launch_bounds__(256) void band_attn_join_kern
     const bool off = den == 0.f || i >= band_seq(a, b).qn;
     const int d = threadIdx.x;
     if (d < a.D) io<T>::st(const_cast<T *>(band_row<T>(a.out, b, i, h)) + d, off ? 0.f : ((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) / den);
-    if (a.lse && d == 0) band_keep(a, ((size_t)b * a.Hq + h) * a.Lq + i, off, mt, den);
+    if (a.lse && d == 0) band_keep(a, ((size_t)b * a.Hq + h) * a.Lq + i, off, mt, top, den);
 }
 
 // Few rows: at most 32 rows of a key head, or too few of the other kernel's workgroups (128 rows of a head) for the chip.
@@ -277,7 +312,7 @@ constexpr int STEP_BIAS_FLOATS = 3584;
 template <typename T, int DP, int MODE, bool BIAS> static int launch_step(BandArgs &a, hipStream_t st) {
     const int R = a.Lq * a.G, nrow = R < 32 ? R : 32;
     const size_t tile = (size_t)4 * band_t<T>::template elems<DP>(STEP_KEYS) * sizeof(T);
-    const size_t meet = (size_t)(4 * 32 * 2 + 4 * nrow * a.D) * sizeof(float), n_bias = (size_t)a.G * (2 * a.M + 1);
+    const size_t meet = (size_t)(4 * 32 * (BIAS ? 3 : 2) + 4 * nrow * a.D) * sizeof(float), n_bias = (size_t)a.G * (2 * a.M + 1);
     a.staged = BIAS && n_bias <= STEP_BIAS_FLOATS ? (int)((n_bias + 3) & ~(size_t)3) : 0;
     const size_t lds = (tile > meet ? tile : meet) + a.staged * sizeof(float);
     auto kern = band_attn_step_kernel<T, DP, MODE, BIAS>;
