@@ -112,3 +112,33 @@ def test_new_tokens_whose_biases_are_all_far_from_zero(cuda0, D, levels, value, 
         out = K.band_attention(four(q).to(cuda0), four(k).to(cuda0), four(v).to(cuda0), window=(None, 0), scale=scale, k_lens=lens.to(cuda0),
                                bias_table=torch.full((1, 4), value, device=cuda0), bias_buckets=bmap.to(cuda0))
     _within("out", out, *ref)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("B,Hq", [(1, 2), (16, 16)])
+def test_rows_that_see_one_not_a_number_key_show_it(cuda0, B, Hq, bias, dtype):
+    """windows of one key, and of a few: a row that sees the bad key is not finite, whether it sees another one or not; the
+    others are what they are without it"""
+    K = _K()
+    gen = torch.Generator().manual_seed(4)
+    L, at = 160, 70
+    q, k, v = (torch.randn(B, L, Hq, 32, generator=gen).to(dtype).to(cuda0) for _ in range(3))
+    kw = dict(bias_table=torch.zeros(1, Hq, device=cuda0), bias_buckets=torch.zeros(5, dtype=torch.int32, device=cuda0)) if bias else {}
+    bad = k.clone()
+    bad[:, at, :, 3] = float("nan")
+    for left in (0, 4):
+        clean, out = (K.band_attention(q, x, v, window=(left, 0), **kw) for x in (k, bad))
+        sees = torch.arange(L, device=cuda0)
+        sees = (sees >= at) & (sees <= at + left)
+        assert torch.isnan(out[:, sees]).all() and torch.isfinite(out[:, ~sees]).all()
+        assert float((out[:, ~sees] - clean[:, ~sees]).abs().max()) <= 2.0 ** -7 * float(v.abs().max())
+    # a new token whose only visible key of a share is the bad one
+    long = torch.randn(1, 4000, Hq, 32, generator=gen).to(dtype).to(cuda0)
+    one = long.clone()
+    one[:, 3999 - 128, :, 3] = float("nan")
+    assert torch.isnan(K.band_attention(q[:1, :1], one, long, window=(128, 0), **kw)).all()
+    one = long.clone()
+    one[:, 0, :, 3] = float("nan")
+    assert torch.isnan(K.band_attention(q[:1, :1], one, long, window=(64, 0), sinks=1, **kw)).all()
+    assert torch.isfinite(K.band_attention(q[:1, :1], one, long, window=(64, 0), **kw)).all()

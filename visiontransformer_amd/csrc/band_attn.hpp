@@ -534,7 +534,8 @@ __device__ __forceinline__ void band_careful(const BandArgs &a, const T *qrow, c
             s += __shfl_xor(s, 32, 64);
             const float bias = BIAS && vis ? band_bias_at(a, head, j - p) : 0.f, x = __builtin_fmaf(s, a.c, bias);
             const bool counts = vis && x != -INFINITY;
-            const float mn = vis ? fmaxf(m, x) : m, left = band_exponent(s, a.c, bias, mn, BIAS && band_remote(vis ? mn : 0.f));
+            // (not a number: the row has a reference all the same, so that its sums count, and show it)
+            const float mn = vis ? fmaxf(m, x != x ? 0.f : x) : m, left = band_exponent(s, a.c, bias, mn, BIAS && band_remote(vis ? mn : 0.f));
             // (what the sums so far are worth beside mn, as an exponent; nothing at first)
             const float before = m == -INFINITY ? -INFINITY : mn == m ? lift : lift + (m - mn);
             const float ln = BIAS && counts ? fmaxf(before, left) : BIAS && m != -INFINITY ? before : 0.f;
