@@ -180,3 +180,21 @@ def test_large_calls_over_rows_far_apart(cuda0, step, L, hkv):
         for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, dout.to(cuda0))):
             _within(name, g, *ref[name])
     del room
+
+
+@pytest.mark.parametrize("sinks", [3, 140])
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_sinks_of_many_sequences(cuda0, dtype, sinks):
+    """many short windows and rows far behind their sinks: the sinks' blocks are cut by what there is to do in all"""
+    K = _K()
+    B, L, D = 512, 4096, 8
+    q, k, v, dout, _ = _inputs((1, L, 1, D), (1, L, 1, D), dtype, 5)
+    ref = S.attention(q.double(), k.double(), v.double(), 20, 0, sinks, D ** -0.5, dout=dout.double(), dtype=dtype)
+    on = lambda t: t.to(cuda0).expand(B, -1, -1, -1).contiguous()
+    leaves = [on(t).requires_grad_() for t in (q, k, v)]
+    out = K.band_attention(*leaves, window=(20, 0), sinks=sinks)
+    grads = torch.autograd.grad(out, leaves, on(dout))
+    for name, got in zip(("out", "dq", "dk", "dv"), (out,) + grads):
+        got = got.detach()
+        assert bool((got == got[:1]).all())      # (equal sequences)
+        _within(name, got[B - 1:], *ref[name])

@@ -108,3 +108,21 @@ def test_sizes_of_calls_without_query_heads():
     for sinks in (0, 3):
         d = _lib.BandDesc(dtype=1, B=1, Lq=4, Lk=8, Hq=0, Hkv=2, D=32, left=-1, right=0, sinks=sinks, scale=0.1)
         assert _lib.load().dsw_band_attn_bwd_workspace(ctypes.byref(d)) == _lib.load().dsw_band_attn_fwd_workspace(ctypes.byref(d)) == 0
+
+
+def test_workspace_of_a_backward_with_sinks():
+    """Blocks of sinks are seen by every row; the shares of their runs must not outgrow the card's memory with the batch or the
+    number of sinks.  Four runs for each resident workgroup (512 of them for narrow heads in 16 bits, else 256), rounded up
+    block by block to twice as many at most; a share is 2 x 128 rows of fp32."""
+    import ctypes
+    from visiontransformer_amd import _lib
+
+    def size(sinks, B=4, L=32768, H=16, D=128, left=256, dtype=1):
+        d = _lib.BandDesc(dtype=dtype, B=B, Lq=L, Lk=L, Hq=H, Hkv=H, D=D, left=left, right=0, sinks=sinks, scale=0.1)
+        return _lib.load().dsw_band_attn_bwd_workspace(ctypes.byref(d))
+
+    for kw in ({}, dict(B=16), dict(B=1, H=1), dict(D=64, left=1024), dict(L=4096), dict(B=2, L=200000, H=8), dict(B=64, dtype=0)):
+        for sinks in (1, 4, 128, 129, 1000, 4096, 20000):
+            extra = size(sinks, **kw) - size(0, **kw)
+            assert 0 <= extra <= 2 * 128 << 20, (kw, sinks, extra)
+            assert sinks > 4 or extra <= 68 << 20, (kw, sinks, extra)

@@ -248,8 +248,10 @@ template <typename T, int V> __global__ __launch_bounds__(256) void band_attn_jo
 
 // Two workgroups a CU are wanted (one for wide heads, whose registers allow no more); a run of the work is at least 8
 // steps long, so that its share does not cost more than it brings.  In fp32, whose products take 16 times as long, runs of 2
-// steps pay, and so does a finer cut (4 a CU: 63 us for 68 for 3 x 1021 tokens, 6 heads of 32).  Blocks of
-// sinks are cut into runs as long as the others' ones.
+// steps pay, and so does a finer cut (4 a CU: 63 us for 68 for 3 x 1021 tokens, 6 heads of 32).  A block of
+// sinks, which every row sees, is cut into runs as long as the others' ones, or, where that would make more shares than balance
+// needs, a quarter of what each resident workgroup has to do in all, a thousand or two of them (4 x 32768 tokens, 16 heads of
+// 128, window 256: without that the workspace was 520 MiB with 4 sinks and 16 GiB with 4096, for 8 MiB with none).
 static BandChunks band_chunks(const BandArgs &a, int dtype) {
     BandChunks c = {0, 1, 1, 0};
     const long long nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS, heads = (long long)a.B * a.Hkv, tiles = (a.Lq + BAND_TILE - 1) / BAND_TILE;
@@ -262,7 +264,9 @@ static BandChunks band_chunks(const BandArgs &a, int dtype) {
     if (c.chunks > 64) c.chunks = 64;
     const long long sink_blocks = a.sinks > 0 && normal < tiles * a.G ? (a.sinks + BAND_ROWS - 1) / BAND_ROWS : 0;
     c.sink_blocks = (int)(sink_blocks < nkb ? sink_blocks : nkb);
-    const long long len = (normal + c.chunks - 1) / c.chunks, k = (tiles * a.G + len - 1) / len;
+    const long long run = (normal + c.chunks - 1) / c.chunks, all = heads * (c.sink_blocks * tiles * a.G + (nkb - c.sink_blocks) * normal);
+    const long long resident = dtype == DSW_F32 || a.D > 64 ? 256 : 512, part = all / (4 * resident);
+    const long long len = run > part ? run : part, k = (tiles * a.G + len - 1) / len;
     c.sink_chunks = c.sink_blocks ? (int)(k < 1024 ? k : 1024) : 1;
     c.shares = heads * ((c.sink_chunks > 1 ? (long long)c.sink_blocks * c.sink_chunks : 0));
     if (c.chunks > 1) c.shares = heads * ((long long)c.sink_blocks * c.sink_chunks + (nkb - c.sink_blocks) * c.chunks);
