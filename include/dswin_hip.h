@@ -693,6 +693,9 @@ typedef struct {
     const float *bias_table;   /* fp32 [n_buckets, Hq] or NULL: bias[j - p] = table[bias_buckets[clip(j - p, +-M) + M]] */
     const int *bias_buckets;   /* int32 [2 M + 1], values are clamped to 0..n_buckets - 1 */
     int n_buckets, max_distance; /* M <= 512 */
+    void *out_rest;            /* NULL, or (bf16) [B, Lq, Hq, D]: what the rounding of out left behind, itself rounded; the forward writes
+                                * it, and the backward, given the same, takes sum(dout * out) from both.  Without it the gradients
+                                * of scores carry the result's rounding, which for rows of one dominant key may be all of them. */
 } dsw_band_desc;
 
 /* lse: fp32 [B, Hq, Lq] for the backward ([2, B, Hq, Lq] where there is a bias table) or NULL; out32: NULL, or (bf16 calls

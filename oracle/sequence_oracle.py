@@ -42,7 +42,7 @@ def visible(Lq, Lk, qn, kn, left, right, sinks):
 
 
 def attention(q, k, v, left, right, sinks, scale, q_lens=None, k_lens=None, table=None, buckets=None, dout=None, dtype=torch.float32,
-              table_grad=True):
+              table_grad=True, score_roundings=None, whole_delta=False):
     """double tensors [B, L, H, D]; returns {"out": (value, bound), and with dout "dq", "dk", "dv", "dtable" likewise}.
 
     Bounds, entry by entry.  Scores: a sum of D products in fp32 and its scaling are off by at most
@@ -51,7 +51,13 @@ def attention(q, k, v, left, right, sinks, scale, q_lens=None, k_lens=None, tabl
     it enters a product in 16 bits, by u more.  The result then carries (u + e) sum P |v| and its own rounding u |out|.
     delta = dout . out inherits the result's error (where a table's gradient is wanted: that of the fp32 copy that the
     kernels keep then), and
-    dS = P (dP - delta) carries u |dS| + P |delta's error| + e P (|dP| + |delta|) + D F P sum|dout v|."""
+    dS = P (dP - delta) carries u |dS| + P |delta's error| + e P (|dP| + |delta|) + D F P sum|dout v|.
+
+    score_roundings: in the place of D + 4, for q and k whose products and sums are exact in fp32.
+    whole_delta: the result's own rounding does not enter delta (what it leaves behind is kept, rounded: u^2), and the rounded
+    probabilities are divided by their own sum: to first order delta is then off by sum_j P_j u_j (dP_j - delta), u_j the
+    rounding of P_j, at most u sum |dS|; (1 + 4 u) for the second.  An error e of P itself multiplies dP - delta.  The same sum
+    makes the backward's P = p / sum p (1 + u_j), off by the relative sum P_j u_j of at most u (1 + 2 u) in a whole row."""
     B, Lq, Hq, D = q.shape
     Lk, Hkv = k.shape[1:3]
     u = unit(dtype) if dtype != torch.float32 else 0.0     # rounding of probabilities and of dS
@@ -82,7 +88,7 @@ def attention(q, k, v, left, right, sinks, scale, q_lens=None, k_lens=None, tabl
             P = e / tot.masked_fill(tot == 0, 1.0)
             O = P @ V
             A = P @ V.abs()
-            rel_e = (2 * F * ((D + 4) * xabs.masked_fill(~vis, 0).amax(-1, keepdim=True) + vis.sum(-1, keepdim=True) + 16)
+            rel_e = (2 * F * ((D + 4 if score_roundings is None else score_roundings) * xabs.masked_fill(~vis, 0).amax(-1, keepdim=True) + vis.sum(-1, keepdim=True) + 16)
                      if Lk else torch.zeros(Lq, 1, dtype=q.dtype))
             out[b, :, h] = O
             b_out[b, :, h] = (u + rel_e) * A + uo * O.abs() + F * A * 8
@@ -101,6 +107,10 @@ def attention(q, k, v, left, right, sinks, scale, q_lens=None, k_lens=None, tabl
                 return P * d_delta + rel_e * P * (dP.abs() + delta.abs()) + (D + 8) * F * P * absGV
             exact = table is not None and table_grad and dtype != torch.float32
             raw = ds_bound(u ** 3, 0.0) if exact else ds_bound(u, uo)
+            if whole_delta and not exact:
+                d_delta = (u * (1 + 4 * u) * dS.abs().sum(-1, keepdim=True)
+                           + (G.abs() * ((rel_e + 8 * F) * A + u * u * O.abs())).sum(-1, keepdim=True) + (D + 4) * F * (G * O).abs().sum(-1, keepdim=True))
+                raw = P * d_delta + (rel_e + u * (1 + 2 * u)) * (1 + u) * dS.abs() + (D + 8) * F * P * absGV
             bS = u * dS.abs() + raw
             nrow = Lq * (Hq // Hkv)
             res["dq"][0][b, :, h] = dS @ Kb * scale
@@ -108,7 +118,7 @@ def attention(q, k, v, left, right, sinks, scale, q_lens=None, k_lens=None, tabl
             res["dk"][0][b, :, g] += dS.T @ Q * scale
             res["dk"][1][b, :, g] += (bS + (nrow + 8) * F * dS.abs()).T @ Q.abs() * scale
             res["dv"][0][b, :, g] += P.T @ G
-            res["dv"][1][b, :, g] += (P * (u + rel_e + (nrow + 8) * F)).T @ G.abs()
+            res["dv"][1][b, :, g] += (P * (u + rel_e + (nrow + 8) * F + (u * (1 + 2 * u) if whole_delta else 0.0))).T @ G.abs()
             if table is not None:
                 n = table.shape[0]
                 flat = bucket.flatten()

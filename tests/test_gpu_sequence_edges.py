@@ -142,3 +142,30 @@ def test_rows_that_see_one_not_a_number_key_show_it(cuda0, B, Hq, bias, dtype):
     one[:, 0, :, 3] = float("nan")
     assert torch.isnan(K.band_attention(q[:1, :1], one, long, window=(64, 0), sinks=1, **kw)).all()
     assert torch.isfinite(K.band_attention(q[:1, :1], one, long, window=(64, 0), **kw)).all()
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("left", [1, 2, 40])
+@pytest.mark.parametrize("B,L,Hq,Hkv,D", [(2, 150, 4, 2, 64), (1, 90, 2, 2, 30), (16, 150, 16, 4, 64), (8, 200, 16, 16, 30), (8, 140, 16, 8, 128),
+                                           (1, 150, 2, 1, 33)])
+def test_gradients_of_scores_under_one_dominant_key(cuda0, B, L, Hq, Hkv, D, left, dtype):
+    """Rows whose softmax is nearly one key: dS is small beside dP and delta, which have to agree far better than the result's own
+    rounding.  q and k are small whole numbers, so that scores carry the scaling's roundings alone; with and without a
+    bias that wants no gradient."""
+    from oracle import sequence_oracle as S
+    from test_gpu_sequence import _within
+    K = _K()
+    gen = torch.Generator().manual_seed(left)
+    ints = lambda h, n: torch.randint(-n, n + 1, (B, L, h, D), generator=gen).to(dtype)
+    q, k = ints(Hq, 1), ints(Hkv, 2)
+    v, dout = torch.randn(B, L, Hkv, D, generator=gen).to(dtype), torch.randn(B, L, Hq, D, generator=gen).to(dtype)
+    table, bmap = torch.randn(4, Hq, generator=gen), torch.randint(0, 4, (9,), generator=gen, dtype=torch.int32)
+    for bias in (False, True):
+        ref = S.attention(q.double(), k.double(), v.double(), left, 0, 0, 0.5, table=table.double() if bias else None, buckets=bmap if bias else None,
+                          dout=dout.double(), dtype=dtype, table_grad=False, score_roundings=4, whole_delta=True)
+        leaves = [t.to(cuda0).requires_grad_() for t in (q, k, v)]
+        kw = dict(bias_table=table.to(cuda0), bias_buckets=bmap.to(cuda0)) if bias else {}
+        out = K.band_attention(*leaves, window=(left, 0), scale=0.5, **kw)
+        _within("out", out, *ref["out"])
+        for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, dout.to(cuda0))):
+            _within(name, g, *ref[name])

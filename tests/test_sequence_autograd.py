@@ -126,3 +126,30 @@ def test_workspace_of_a_backward_with_sinks():
             extra = size(sinks, **kw) - size(0, **kw)
             assert 0 <= extra <= 2 * 128 << 20, (kw, sinks, extra)
             assert sinks > 4 or extra <= 68 << 20, (kw, sinks, extra)
+
+
+def test_refusals_of_what_the_rounding_leaves():
+    """out_rest with fp32 tensors, in both directions, before anything is launched"""
+    import ctypes
+    from visiontransformer_amd import _lib
+    lib = _lib.load()
+    p, s = ctypes.cast((ctypes.c_float * 64)(), ctypes.c_void_p), ctypes.byref(_lib.Strides(1, 1, 1))
+    d = _lib.BandDesc(dtype=0, B=1, Lq=4, Lk=8, Hq=4, Hkv=2, D=32, left=-1, right=0, sinks=0, scale=0.1, out_rest=p)
+    assert lib.dsw_band_attn_fwd(ctypes.byref(d), p, s, p, s, p, s, p, s, p, None, p, 1 << 40, None) == 1
+    assert b"out_rest" in lib.dswin_last_error_string()
+    assert lib.dsw_band_attn_bwd(ctypes.byref(d), p, s, p, s, p, s, p, s, None, p, s, p, p, s, p, s, p, s, None, p, 1 << 40, None) == 1
+    assert b"out_rest" in lib.dswin_last_error_string()
+
+
+@pytest.mark.parametrize("dtype,wants,table,kept", [(torch.bfloat16, "q", False, True), (torch.bfloat16, "v", False, False), (torch.float32, "q", False, False),
+                                                    (torch.bfloat16, "kt", True, False), (torch.bfloat16, "k", True, True)])
+def test_what_the_rounding_leaves_is_kept_where_scores_want_gradients(calls, dtype, wants, table, kept):
+    """(a table's gradient keeps the whole result in 32 bits instead)"""
+    import ctypes
+    ts = {n: torch.randn(1, 4, 2, 8).to(dtype).requires_grad_(n in wants) for n in "qkv"}
+    tab = torch.randn(3, 2).requires_grad_("t" in wants) if table else None
+    out = _attention(ts["q"], ts["k"], ts["v"], bias_table=tab, bias_buckets=torch.zeros(5, dtype=torch.int32) if table else None)
+    out.sum().backward()
+    from visiontransformer_amd._lib import BandDesc
+    descs = [ctypes.cast(ctypes.pointer(args[0]._obj), ctypes.POINTER(BandDesc)).contents for _, args in calls]
+    assert len(descs) == 2 and all(bool(d.out_rest) == kept for d in descs) and descs[0].out_rest == descs[1].out_rest

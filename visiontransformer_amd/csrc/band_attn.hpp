@@ -39,6 +39,7 @@ struct BandArgs {
     float *lse;          // [B][Hq][Lq], base 2; +inf for rows without a visible key (2^(x - inf) = 0 in the backward)
     float *top;          // with a bias table: [B][Hq][Lq], taken out of lse (see band_keep)
     float *out32;        // [B][Lq][Hq][D] or null
+    bf16_t *rest;        // [B][Lq][Hq][D] or null: out before its rounding, less out
     float *delta;        // [B][Hq][Lq]
     float *partial;      // step kernel: see there; dQ kernel: bias gradients by distance
     int nsplit, nrb, staged;  // step kernel; staged: floats of the bias by head and distance in LDS, or 0
@@ -211,6 +212,21 @@ __device__ __forceinline__ void band_store_row(T *row, const f32x16 *acc, float 
             }
             if (on) band_store8<MODE>(row, 32 * db + 16 * p + 8 * hh, v, D);
         }
+}
+
+// what the rounding of such a tile's rows left behind, rounded in its turn
+template <int DP, int MODE>
+__device__ __forceinline__ void band_store_rest(bf16_t *row, const f32x16 *acc, float mul, int D, int hh, bool on) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) {
+        f32x16 left;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float v = acc[db][r] * mul;
+            left[r] = v - bf16_to_f32(f32_to_bf16(v));
+        }
+        band_store_row<bf16_t, 32, MODE>(row + 32 * db, &left, 1.f, D - 32 * db, hh, on);
+    }
 }
 
 // ---- LDS images of [rows][DP] tiles --------------------------------------------------------------------------------
@@ -571,6 +587,8 @@ template <typename K> int band_allow_lds(const char *who, K kern, size_t lds) {
 int band_make_args(const char *who, const dsw_band_desc *d, BandArgs &a);
 // fills t and raises `mode` to what the tensor needs
 int band_tensor(const char *who, const char *name, const void *p, const dsw_strides *s, int dtype, int D, bool null_ok, BandTensor &t, int &mode);
+// likewise a.rest, where the description has it
+int band_rest_tensor(const char *who, const dsw_band_desc *d, BandArgs &a, int &mode);
 // (T, DP, MODE) for a call
 #define DSW_BAND_DISPATCH(dtype, D, mode, T, DP, MODE, ...)                                                           \
     DSW_DISPATCH_DTYPE(dtype, T, {                                                                                      \

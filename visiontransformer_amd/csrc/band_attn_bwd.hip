@@ -321,7 +321,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     const size_t stat = ((size_t)b * a.Hq + h) * a.Lq + i;
     const float nl = row_on ? -a.lse[stat] : -INFINITY, top = BIAS && row_on ? a.top[stat] : 0.f;
     const bool remote = BIAS && band_remote(top);
-    // delta = dout . out, from the result before its rounding where that was kept (in three parts of 8 bits).  It is the
+    // delta = dout . out, from the result before its rounding where that was kept (whole, in three parts of 8 bits, or as what the
+    // rounding left behind: with the rounded result alone dq and dk of a row of one dominant key were mostly its error).  It is the
     // diagonal of a product formed like dout v^T below: for a row that sees a single key, whose result is that key's value,
     // the two are then the same number and dS is exactly zero.
     float del = 0.f;
@@ -347,6 +348,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
                 band_clear(of);
                 if (row_on) of = band_load8<MODE>(orow, col, D);
                 d = band_mma(of, gf[c], d);
+                if constexpr (sizeof(T) == 2) {
+                    if (a.rest) {
+                        band_clear(of);
+                        if (row_on) of = band_load8<MODE>(a.rest + (((size_t)b * a.Lq + i) * a.Hq + h) * D, col, D);
+                        d = band_mma(of, gf[c], d);
+                    }
+                }
             }
         }
         float mine = 0.f;
@@ -632,6 +640,7 @@ extern "C" int dsw_band_attn_bwd(const dsw_band_desc *d, const void *q, const ds
         (rc = band_tensor(who, "dout", dout, sdo, d->dtype, a.D, no_rows, a.dout, mode)) || (rc = band_tensor(who, "dq", dq, sdq, d->dtype, a.D, no_rows, a.dq, mode)) ||
         (rc = band_tensor(who, "dk", dk, sdk, d->dtype, a.D, no_keys, a.dk, mode)) || (rc = band_tensor(who, "dv", dv, sdv, d->dtype, a.D, no_keys, a.dv, mode)))
         return rc;
+    if (!no_rows && (rc = band_rest_tensor(who, d, a, mode))) return rc;
     DSW_REQUIRE(no_rows || lse, "%s: null lse", who);
     DSW_REQUIRE(d_table == nullptr || a.table, "%s: a gradient for a table that is not there", who);
     DSW_REQUIRE(d_table == nullptr || no_rows || d->dtype == DSW_F32 || out32, "%s: the table's gradient needs the forward's out32", who);

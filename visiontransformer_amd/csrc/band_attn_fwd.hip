@@ -269,6 +269,9 @@ __global__ __launch_bounds__(256, (DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof
     band_store_row<T, DP, MODE>(const_cast<T *>(band_row<T>(a.out, at.b, at.i, at.h)), o, inv, a.D, hh, store);
     if constexpr (EXACT)  // (in mode 0 D is a multiple of 8)
         band_store_row<float, DP, MODE>(a.out32 + (((size_t)at.b * a.Lq + at.i) * a.Hq + at.h) * a.D, o, inv, a.D, hh, store);
+    if constexpr (sizeof(T) == 2) {
+        if (a.rest) band_store_rest<DP, MODE>(a.rest + (((size_t)at.b * a.Lq + at.i) * a.Hq + at.h) * a.D, o, inv, a.D, hh, store);
+    }
     if (a.lse && store && hh == 0)
         band_keep(a, ((size_t)at.b * a.Hq + at.h) * a.Lq + at.i, !row_on || l == 0.f, m, lift, l);
 }
@@ -296,6 +299,15 @@ int band_tensor(const char *who, const char *name, const void *p, const dsw_stri
     const int m = D < 8 || !fits(4) || t.s.l * size * BAND_TILE >= (1LL << 31) ? 2 : fits(16) ? 0 : 1;
     mode = m > mode ? m : mode;
     return DSW_OK;
+}
+
+int band_rest_tensor(const char *who, const dsw_band_desc *d, BandArgs &a, int &mode) {
+    if (d->out_rest == nullptr) return DSW_OK;
+    DSW_REQUIRE(d->dtype == DSW_BF16, "%s: out_rest goes with bf16 tensors", who);
+    BandTensor t;
+    const dsw_strides s = {(long long)a.Lq * a.Hq * a.D, (long long)a.Hq * a.D, a.D};
+    a.rest = static_cast<bf16_t *>(d->out_rest);
+    return band_tensor(who, "out_rest", d->out_rest, &s, d->dtype, a.D, false, t, mode);
 }
 
 int band_make_args(const char *who, const dsw_band_desc *d, BandArgs &a) {
@@ -352,6 +364,7 @@ extern "C" int dsw_band_attn_fwd(const dsw_band_desc *d, const void *q, const ds
         (rc = band_tensor(who, "v", v, sv, d->dtype, a.D, no_keys, a.v, mode)) || (rc = band_tensor(who, "out", out, so, d->dtype, a.D, false, a.out, mode)))
         return rc;
     DSW_REQUIRE(out32 == nullptr || (a.table && d->dtype == DSW_BF16), "%s: out32 goes with a bias table and bf16 tensors", who);
+    if ((rc = band_rest_tensor(who, d, a, mode))) return rc;
     a.lse = lse;
     a.top = lse && a.table ? lse + (size_t)a.B * a.Hq * a.Lq : nullptr;
     a.out32 = out32;

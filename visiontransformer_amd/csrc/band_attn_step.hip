@@ -15,6 +15,14 @@ namespace dsw {
 
 constexpr int STEP_KEYS = 32;
 
+// an element of the result, and what its rounding left behind
+template <typename T> __device__ __forceinline__ void step_store(const BandArgs &a, int b, int i, int h, int d, float v) {
+    io<T>::st(const_cast<T *>(band_row<T>(a.out, b, i, h)) + d, v);
+    if constexpr (sizeof(T) == 2) {
+        if (a.rest) a.rest[(((size_t)b * a.Lq + i) * a.Hq + h) * a.D + d] = f32_to_bf16(v - bf16_to_f32(f32_to_bf16(v)));
+    }
+}
+
 template <typename T, int DP, int MODE, bool BIAS>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void band_attn_step_kernel(const BandArgs a) {
     constexpr int ELEMS = band_t<T>::template elems<DP>(STEP_KEYS);
@@ -148,14 +156,12 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
         const float shift = m == -INFINITY ? 0.f : m;
         const bool remote = BIAS && band_remote(shift);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = __builtin_amdgcn_exp2f(band_exponent(s[r], a.c, bias[r], shift, remote));
-            l += s[r];
-        }
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(band_exponent(s[r], a.c, bias[r], shift, remote));
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             typename band_t<T>::frag pf;
             band_pack(s, k, pf);
+            l = band_sum(pf, l);  // (the weights as they enter the product: they then sum to one)
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db) o[db] = band_mma(band_cols<DP>(V, 16 * k, db, lane), pf, o[db]);
         }
@@ -228,7 +234,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
         if (a.nsplit == 1) {
             const int ro = rb * 32 + rl, io_ = ro / a.G, ho = hk * a.G + ro - io_ * a.G;
             const bool off = den == 0.f || io_ >= sq.qn;
-            io<T>::st(const_cast<T *>(band_row<T>(a.out, b, io_, ho)) + d, off ? 0.f : sum / den);
+            step_store<T>(a, b, io_, ho, d, off ? 0.f : sum / den);
             if (a.lse && d == 0) band_keep(a, ((size_t)b * a.Hq + ho) * a.Lq + io_, off, mx, top, den);
         } else {
             const int W = a.D + PART;
@@ -281,7 +287,7 @@ template <typename T> __global__ __launch_bounds__(256) void band_attn_join_kern
     __syncthreads();
     const bool off = den == 0.f || i >= band_seq(a, b).qn;
     const int d = threadIdx.x;
-    if (d < a.D) io<T>::st(const_cast<T *>(band_row<T>(a.out, b, i, h)) + d, off ? 0.f : ((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) / den);
+    if (d < a.D) step_store<T>(a, b, i, h, d, off ? 0.f : ((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) / den);
     if (a.lse && d == 0) band_keep(a, ((size_t)b * a.Hq + h) * a.Lq + i, off, mt, top, den);
 }
 

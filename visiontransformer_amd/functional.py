@@ -2563,10 +2563,10 @@ def _workspace(way, desc):
 
 class _BandAttnFn(torch.autograd.Function):
     @staticmethod
-    def _desc(q, k, tab, buckets, q_lens, k_lens, left, right, sinks, scale):
+    def _desc(q, k, tab, buckets, q_lens, k_lens, left, right, sinks, scale, rest=None):
         B, Lq, Hq, D = q.shape
         return _lib.BandDesc(dtype_code(q.dtype), B, Lq, k.shape[1], Hq, k.shape[2], D, left, right, sinks, scale, ptr(q_lens), ptr(k_lens),
-                             ptr(tab), ptr(buckets), 0 if tab is None else tab.shape[0], 0 if tab is None else buckets.numel() // 2)
+                             ptr(tab), ptr(buckets), 0 if tab is None else tab.shape[0], 0 if tab is None else buckets.numel() // 2, ptr(rest))
 
     @staticmethod
     def forward(ctx, q, k, v, table, buckets, q_lens, k_lens, left, right, sinks, scale):
@@ -2578,9 +2578,11 @@ class _BandAttnFn(torch.autograd.Function):
         tab = _as_f32(table)
         out, so, po = _new_rows(B, Lq, Hq, D, q.dtype, dev)
         settings = (left, right, sinks, scale)
-        desc = _BandAttnFn._desc(q, k, tab, buckets, q_lens, k_lens, *settings)
         train = any(ctx.needs_input_grad[:4])
         exact = train and ctx.needs_input_grad[3] and q.dtype == torch.bfloat16
+        # (what the rounding to 16 bits leaves of the result: the gradients of scores are taken from both)
+        rest = torch.empty_like(out) if train and not exact and q.dtype == torch.bfloat16 and any(ctx.needs_input_grad[:2]) else None
+        desc = _BandAttnFn._desc(q, k, tab, buckets, q_lens, k_lens, *settings, rest)
         lse = torch.empty(1 if tab is None else 2, B, Hq, Lq, dtype=torch.float32, device=dev) if train else None
         out32 = torch.empty(B, Lq, Hq, D, dtype=torch.float32, device=dev) if exact else None
         if B * Lq * Hq:
@@ -2588,7 +2590,7 @@ class _BandAttnFn(torch.autograd.Function):
             ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
             _call_on(dev, "dsw_band_attn_fwd", ctypes.byref(desc), pq, sq, pk, sk, pv, sv, po, so, ptr(lse), ptr(out32), ptr(ws), n, stream(dev))
         if train:
-            ctx.save_for_backward(q, k, v, tab, buckets, q_lens, k_lens, out, out32, lse)
+            ctx.save_for_backward(q, k, v, tab, buckets, q_lens, k_lens, out, rest, out32, lse)
             ctx.settings = settings
             ctx.table_dtype = None if table is None else table.dtype
         return out
@@ -2596,7 +2598,7 @@ class _BandAttnFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, tab, buckets, q_lens, k_lens, out, out32, lse = ctx.saved_tensors
+        q, k, v, tab, buckets, q_lens, k_lens, out, rest, out32, lse = ctx.saved_tensors
         dev = q.device
         made = [_new_rows(*t.shape, t.dtype, dev) for t in (q, k, v)]
         grads = [t[0] for t in made]
@@ -2610,7 +2612,7 @@ class _BandAttnFn(torch.autograd.Function):
             operands += [p, s, ptr(lse)]
             for t in made:
                 operands += t[:0:-1]
-            desc = _BandAttnFn._desc(q, k, tab, buckets, q_lens, k_lens, *ctx.settings)
+            desc = _BandAttnFn._desc(q, k, tab, buckets, q_lens, k_lens, *ctx.settings, rest)
             n = _workspace("bwd", desc)
             ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
             _call_on(dev, "dsw_band_attn_bwd", ctypes.byref(desc), *operands, ptr(d_tab), ptr(ws), n, stream(dev))
