@@ -1,4 +1,4 @@
-"""sequence.KVCache on the CPU: what a refused call leaves behind."""
+"""sequence.KVCache and sequence.BandedMSA on the CPU: calls that are refused, and what they leave behind."""
 import pytest
 import torch
 
@@ -13,3 +13,11 @@ def test_counts_of_other_types_are_refused_before_anything_is_written(lens):
     with pytest.raises(RuntimeError, match="KVCache: lens"):
         cache.append(torch.zeros(2, 3, 1, 4), torch.zeros(2, 3, 1, 4), lens)
     assert cache.lens.tolist() == [0, 0] and cache.longest == 0 and bool((cache.k == 7).all())
+
+
+@pytest.mark.parametrize("kw", [dict(rotary_axes=0), dict(rotary_axes=0, qk_norm=False), dict(rotary_pairs=0)])
+def test_positions_without_a_rotation_are_refused(kw):
+    """with the norm alone they were dropped"""
+    from visiontransformer_amd.sequence import BandedMSA
+    with pytest.raises(RuntimeError, match="without rotation"):
+        BandedMSA(64, **kw)(torch.zeros(1, 4, 64), positions=torch.arange(4))

@@ -146,6 +146,8 @@ class BandedMSA(nn.Module):
         it holds; with lens, the batch must be as long as its longest sequence."""
         B, L, C = x.shape
         h, g, d = self.num_heads, self.kv_heads, self.head_dim
+        if positions is not None and self.rotary_freqs is None:
+            raise RuntimeError("visiontransformer_amd: BandedMSA: positions given to a module without rotation")
         qkv = K.linear(x, self.qkv).unflatten(-1, (h + 2 * g, d))
         q, k, v = qkv.split((h, g, g), dim=2)
         if self.q_norm is not None:
@@ -156,9 +158,7 @@ class BandedMSA(nn.Module):
             freqs = self.rotary_freqs
             if freqs is not None and self.rotary_axes == 1:
                 freqs = freqs[0]
-            q, k = K.qk_norm_rotary(q, k, self.q_norm, self.k_norm, freqs, positions if freqs is not None else None, eps=self.eps)
-        elif positions is not None:
-            raise RuntimeError("visiontransformer_amd: BandedMSA: positions given to a module without rotation")
+            q, k = K.qk_norm_rotary(q, k, self.q_norm, self.k_norm, freqs, positions, eps=self.eps)
         q_lens = k_lens = lens
         if cache is not None:
             if torch.is_grad_enabled() and qkv.requires_grad:
