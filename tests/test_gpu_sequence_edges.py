@@ -169,3 +169,23 @@ def test_gradients_of_scores_under_one_dominant_key(cuda0, B, L, Hq, Hkv, D, lef
         _within("out", out, *ref["out"])
         for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, dout.to(cuda0))):
             _within(name, g, *ref[name])
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("B,H", [(16, 16), (1, 1)])
+@pytest.mark.parametrize("top", [2.0 ** 40, -2.0 ** 40, 2.0 ** 70])
+def test_scores_beyond_what_fp32_tells_apart(cuda0, top, B, H, dtype):
+    """Scores of `top` and, for every third key, lower by a 2^-7 of it: the mean of the others' values, though the scores' scaling
+    alone rounds by thousands.  Tolerance as for equal keys."""
+    K = _K()
+    L, D = 250, 64
+    k = torch.full((1, L, 1, D), top / D)
+    low = torch.arange(L) % 3 == 1
+    k[:, low] = (top - abs(top) / 128) / D
+    v = torch.randint(0, 8, (1, L, 1, D), generator=torch.Generator().manual_seed(2)).float()
+    on = lambda t: t.to(dtype).to(cuda0).expand(B, L, H, D).contiguous()
+    assert torch.equal(k.to(dtype).float(), k)
+    want = v[0, ~low, 0].double().mean(0)
+    for scale in (0.125, 1 / 3, 0.7):
+        out = K.band_attention(on(torch.ones(1, L, 1, D)), on(k), on(v), scale=scale).double().cpu()
+        assert bool(((out - want).abs() <= want * (2.0 ** -8 if dtype == BF else 2.0 ** -22)).all()), scale
