@@ -197,18 +197,16 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
             top = mx == -INFINITY ? 0.f : top;
         }
     };
-    auto weight = [&](float mw, float lw, float mx, float top) {
-        return mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(BIAS ? (mw - mx) + (lw - top) : mw - mx);
-    };
+    float *const mine = ml + (wave * 32 + l31) * PART;
     if (hh == 0) {
-        float *const x = ml + (wave * 32 + l31) * PART;
-        x[0] = m, x[1] = l;
-        if constexpr (BIAS) x[2] = lift;
+        mine[0] = m;
+        if constexpr (BIAS) mine[2] = lift;
     }
     __syncthreads();
     float mt, top;
     meet(l31, mt, top);
-    const float mul = weight(m, lift, mt, top);
+    const float mul = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(BIAS ? (m - mt) + (lift - top) : m - mt);
+    if (hh == 0) mine[1] = m == -INFINITY ? 0.f : l * mul;
     if (l31 < nrow) {
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
@@ -224,12 +222,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     for (int e = threadIdx.x; e < n; e += 256) {
         const int rl = e / a.D, d = e - rl * a.D;
         float mx, den = 0.f;
-        meet(rl, mx, top);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float *const x = ml + (w * 32 + rl) * PART;
-            den += x[0] == -INFINITY ? 0.f : x[1] * weight(x[0], BIAS ? x[PART - 1] : 0.f, mx, top);
-        }
+        for (int w = 0; w < 4; ++w) den += ml[(w * 32 + rl) * PART + 1];
+        if (d == 0) meet(rl, mx, top);
         const float sum = (os[e] + os[n + e]) + (os[2 * n + e] + os[3 * n + e]);
         if (a.nsplit == 1) {
             const int ro = rb * 32 + rl, io_ = ro / a.G, ho = hk * a.G + ro - io_ * a.G;
