@@ -690,7 +690,7 @@ __global__ __launch_bounds__(1024) void bias_grad_reduce_kernel(const float *__r
 template <typename T, int CH> struct LepeElem { using type = T; };
 template <> struct LepeElem<bf16_t, 2> { using type = uint32_t; };
 
-// CH floats side by side: with CH = 2 the arithmetic below is packed fp32 (v_pk_fma_f32) on the channel pair
+// CH floats side by side: with CH = 2 the arithmetic below goes over the channel pair
 template <int CH> struct LepeVec { typedef float type __attribute__((ext_vector_type(CH))); };
 
 // a window row of WS positions (16-byte aligned when the element has 4 bytes) as floats

@@ -8,10 +8,14 @@
 // share a key head are walked one after the other and meet in the accumulators).  Both recompute the scores.  Layouts as in
 // the forward: the 16 registers of a tile's P and dS are the second operand of the products that follow.
 //
-// Bound by the matrix instructions (four and three products per tile) and the exponentials between them, at two waves a SIMD,
-// which the accumulators' registers allow.  2 x 4096 tokens, 16 heads on 4 of 64, window 1024, bf16: dk and dv 100 us with 8 for
-// their join, 600 TFLOP/s of the visible pairs' products, dq 72 us, 625.  With a table's gradient, 2 x 2048 tokens, 8 heads of 64,
-// all visible: dq 70 us, dk and dv 61.
+// Rounding, for bf16 tensors: P and dS enter their products in bf16 (2^-8 each, as the matrix instructions take them); P is
+// divided by the sum of the rounded probabilities of the forward, which may put a row off by as much as one of them; dS itself,
+// delta and all sums are fp32.  dq, dk and dv are 2.3e-3 to 2.4e-3 (rms) from 64 bits, of which their own rounding is 1.7e-3.
+//
+// Neither pipe is full: products (four and three per tile) and the exponentials between them take turns at two waves a SIMD,
+// which the accumulators' registers allow.  2 x 4096 tokens, 16 heads on 4 of 64, window 1024, bf16: dk and dv 98 us, 610 TFLOP/s of the
+// visible pairs' products, matrix pipe 32 % and vector pipe 43 % busy, and 8 us for their join; dq 74 us, 610 TFLOP/s, 33 and
+// 49 %.  With a table's gradient, 2 x 2048 tokens, 8 heads of 64, all visible: dq 70 us (17 and 31 %), dk and dv 61 (27 and 42 %).
 #include "band_attn.hpp"
 
 namespace dsw {

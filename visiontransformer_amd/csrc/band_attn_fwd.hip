@@ -8,11 +8,18 @@
 // fp32 and bf16 reach 2^127 beyond it; sums that pass 2^60 move the reference up, and a workgroup that overflowed all
 // the same goes over its tiles again with the running maximum.  Tiles that every row sees whole carry no mask.
 //
-// Bound by the vector instructions around the products where heads are narrow (per score: an exponential of 4 plain
-// instructions' time, a multiply-add, half a conversion, half an addition), by the matrix instructions where they are wide.
-// Without bias, bf16: 16384 tokens, 8 heads of 128, window 4096: 270 us, 905 TFLOP/s of the visible scores' products (a large
-// matrix product reaches 1194); 4 maps of 4096 tokens, 6 heads of 30, window 1025: 39 us, of which 16 us remain with a
-// window of one key (launch, first loads, stores).  Tried without gain: tiles two ahead, two tiles between barriers, the next
+// Rounding, for bf16 tensors: the probabilities enter the product with V in bf16, one rounding of 2^-8 each, because the matrix
+// instructions take 16-bit operands (a second part would be a second product); they are divided by the sum of the rounded
+// ones, so that their weights sum to one.  Results are 2.1e-3 to 2.3e-3 (rms) from 64 bits, of which their own rounding is 1.7e-3.
+// Where a table wants its gradient (EXACT) the probabilities enter in three parts of 8 bits: 1.66e-3, as the rounding alone.
+// Scores, exponents, sums and the log-sum-exp are fp32; the latter is that of the rounded probabilities.
+//
+// Neither pipe is full: the matrix instructions and the vector instructions around them (per score: an exponential of 4 plain
+// instructions' time, a multiply-add, half a conversion, half an addition) take turns in the two or three waves of a SIMD.  Without
+// bias, bf16: 16384 tokens, 8 heads of 128, window 4096: 264 to 294 us by card and clock, 820 to 910 TFLOP/s of the visible
+// scores' products (a large matrix product reaches 1194), matrix pipe 50 % and vector pipe 44 % busy while an engine has waves,
+// and a fifth of the launch in which engines have run out of them; 4 maps of 4096 tokens, 6 heads of 30, window 1025: 39 us,
+// matrix 14 %, vector 48 %, of which 16 us remain with a window of one key (launch, first loads, stores).  Tried without gain: tiles two ahead, two tiles between barriers, the next
 // tile's products under this one's exponentials by hand, 4 waves a SIMD (registers spill).
 #include "band_attn.hpp"
 

@@ -8,7 +8,8 @@
 // the next tile under way meanwhile - and meet at the end.  With more than one share the sums, maxima and denominators
 // go to the workspace, and a second kernel joins them in the order of the shares.  One token over 8 caches of 4096 to 32768
 // keys, 16 heads on 4 of 64, bf16: 151 MB in 29 us, 5.2 TB/s, and 4 us for the join; over windows of 1028 keys of 128, 16
-// sequences of 8 key heads: 65 MB in 24 us, two tiles a wave, bound by latency.
+// sequences of 8 key heads: 65 MB in 24 us, two tiles a wave, bound by latency.  For bf16 tensors the probabilities enter the
+// product with V in bf16 and are divided by the sum of the rounded ones, as in the forward of many rows.
 #include "band_attn.hpp"
 
 namespace dsw {

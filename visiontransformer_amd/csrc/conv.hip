@@ -19,7 +19,7 @@ __device__ __forceinline__ float silu_grad(float v) {
     const float s = 1.f / (1.f + __expf(-v));
     return s * (1.f + v * (1.f - s));
 }
-// four fused multiply-adds as two packed ones (v_pk_fma_f32 does two lanes' worth per issue slot)
+// four fused multiply-adds, in pairs (the build has no packed fp32 instructions: see FLAGS in __graft_entry__.py)
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float4 fma4(float4 a, float4 b, float4 c) {
     const f32x2_t lo = __builtin_elementwise_fma(f32x2_t{a.x, a.y}, f32x2_t{b.x, b.y}, f32x2_t{c.x, c.y});
