@@ -153,3 +153,22 @@ def test_what_the_rounding_leaves_is_kept_where_scores_want_gradients(calls, dty
     from visiontransformer_amd._lib import BandDesc
     descs = [ctypes.cast(ctypes.pointer(args[0]._obj), ctypes.POINTER(BandDesc)).contents for _, args in calls]
     assert len(descs) == 2 and all(bool(d.out_rest) == kept for d in descs) and descs[0].out_rest == descs[1].out_rest
+
+
+def test_bucket_numbers_are_clamped_before_they_are_narrowed(calls, monkeypatch):
+    """int64 buckets beyond 32 bits: the table's ends, as for any other number outside it"""
+    import ctypes
+    from visiontransformer_amd import functional as K
+    from visiontransformer_amd._lib import BandDesc
+    seen = []
+
+    def launch(device, name, desc, *args):
+        d = ctypes.cast(ctypes.pointer(desc._obj), ctypes.POINTER(BandDesc)).contents
+        seen.append(list((ctypes.c_int * 5).from_address(d.bias_buckets)))
+
+    monkeypatch.setattr(K, "_call_on", launch)
+    x = torch.zeros(1, 4, 2, 8)
+    _attention(x, x, x, bias_table=torch.zeros(3, 2), bias_buckets=torch.tensor([2 ** 32, -2 ** 32 - 1, 1, 2 ** 33 + 1, -1]))
+    assert seen == [[2, 0, 1, 2, 0]]
+    _attention(x, x, x, bias_table=torch.zeros(3, 2), bias_buckets=torch.tensor([0, 1, 1, 2, 0], dtype=torch.int32))
+    assert seen[1] == [0, 1, 1, 2, 0]

@@ -2678,6 +2678,8 @@ def band_attention(q, k, v, window=(None, None), sinks=0, scale=None, q_lens=Non
         _device_ints(who, "bias_buckets", bias_buckets, q.device, ((n,),))
         if n % 2 == 0 or not 3 <= n <= 1025:
             _fail(who, "bias_buckets must have 2 M + 1 entries with 1 <= M <= 512, got %d" % n)
+        if bias_buckets.dtype == torch.int64:    # (clamped, as the kernels do, before they are narrowed)
+            bias_buckets = bias_buckets.clamp(0, bias_table.shape[0] - 1)
         bias_buckets = bias_buckets.to(torch.int32).contiguous()
     args = (q, k, v, bias_table, bias_buckets, q_lens, k_lens, -1 if left is None else int(left), -1 if right is None else int(right),
             int(sinks), scale)
