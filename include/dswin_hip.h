@@ -682,7 +682,8 @@ int dsw_qk_norm_rotary_bwd(const void *q, const dsw_strides *sq, const void *k, 
  * sequence b stands at p = k_len - q_len + i (q_len <= Lq rows, k_len <= Lk keys); key j < k_len is visible to it when
  * j <= p + right and (j >= p - left or j < sinks).  out = softmax over the visible keys of scale * q.k + bias, times v;
  * rows without a visible key and rows from q_len on are zeros, and so are their gradients.  Query head h reads key head
- * h / (Hq / Hkv).  The description is read before the call returns (it lies in HOST memory, the pointers in it do not). */
+ * h / (Hq / Hkv).  The description is read before the call returns (it lies in HOST memory, the pointers in it do not);
+ * start it from zeros, as fields may be added behind the last one (out_rest came with dswin_version() 101). */
 typedef struct {
     int dtype;                 /* of q, k, v, out and their gradients: DSW_F32 or DSW_BF16 */
     int B, Lq, Lk, Hq, Hkv, D; /* Hq a multiple of Hkv, 1 <= D <= 128 */

@@ -8,6 +8,6 @@ char *tls_error_buffer() {
 }
 }  // namespace dsw
 
-extern "C" int dswin_version(void) { return 100; }
+extern "C" int dswin_version(void) { return 101; }
 
 extern "C" const char *dswin_last_error_string(void) { return dsw::tls_error_buffer(); }
