@@ -683,7 +683,7 @@ int dsw_qk_norm_rotary_bwd(const void *q, const dsw_strides *sq, const void *k, 
  * j <= p + right and (j >= p - left or j < sinks).  out = softmax over the visible keys of scale * q.k + bias, times v;
  * rows without a visible key and rows from q_len on are zeros, and so are their gradients.  Query head h reads key head
  * h / (Hq / Hkv).  The description is read before the call returns (it lies in HOST memory, the pointers in it do not);
- * start it from zeros, as fields may be added behind the last one (out_rest came with dswin_version() 101). */
+ * start it from zeros, as fields may be added behind the last one (the last two came with dswin_version() 101). */
 typedef struct {
     int dtype;                 /* of q, k, v, out and their gradients: DSW_F32 or DSW_BF16 */
     int B, Lq, Lk, Hq, Hkv, D; /* Hq a multiple of Hkv, 1 <= D <= 128 */
@@ -697,6 +697,9 @@ typedef struct {
     void *out_rest;            /* NULL, or (bf16) [B, Lq, Hq, D]: what the rounding of out left behind, itself rounded; the forward writes
                                 * it, and the backward, given the same, takes sum(dout * out) from both.  Without it the gradients
                                 * of scores carry the result's rounding, which for rows of one dominant key may be all of them. */
+    float *lse_rest;           /* NULL, or (fp32 calls without a bias table; others leave it alone) [B, Hq, Lq]: what the rounding of lse
+                                * left behind, written and read like out_rest.  Without it, and in bf16, probabilities of the
+                                * backward carry 2^-25 of the logits' size. */
 } dsw_band_desc;
 
 /* lse: fp32 [B, Hq, Lq] for the backward ([2, B, Hq, Lq] where there is a bias table) or NULL; out32: NULL, or (bf16 calls

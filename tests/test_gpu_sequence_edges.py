@@ -189,3 +189,31 @@ def test_scores_beyond_what_fp32_tells_apart(cuda0, top, B, H, dtype):
     for scale in (0.125, 1 / 3, 0.7):
         out = K.band_attention(on(torch.ones(1, L, 1, D)), on(k), on(v), scale=scale).double().cpu()
         assert bool(((out - want).abs() <= want * (2.0 ** -8 if dtype == BF else 2.0 ** -22)).all()), scale
+
+
+# (bf16 calls keep a row's probability of 1 up to scores of 2^15: off by 2^-9 there, which is rounded away)
+@pytest.mark.parametrize("dtype,top", [(BF, 201 * 2.0 ** 7)] + [(FP, 201 * x) for x in (2.0 ** 7, 2.0 ** 13, 2.0 ** 33, -2.0 ** 13)])
+@pytest.mark.parametrize("B,L,Hq,Hkv,D", [(1, 150, 2, 1, 64), (16, 150, 16, 4, 64), (8, 140, 16, 16, 30), (8, 140, 16, 8, 128)])
+def test_gradients_of_rows_of_one_key_with_large_scores(cuda0, top, B, L, Hq, Hkv, D, dtype):
+    """Every row's softmax is one key, 2^9 and more above the others (their probabilities are below 2^-240, zero), however the
+    scaling rounds its score: the result is that key's value, dv its rows' dout added up, and the scores have no gradient at all."""
+    K = _K()
+    gen = torch.Generator().manual_seed(D)
+    k = torch.zeros(B, L, Hkv, D)
+    k[..., 0] = top - abs(top) / 201 * (25 if abs(top) < 2.0 ** 16 else 1)      # (bf16 has 8 bits: 176 and 200 of 201)
+    k[:, 17, :, 0] = top
+    assert torch.equal(k.to(dtype).float(), k)
+    q = torch.zeros(B, L, Hq, D)
+    q[..., 0] = 1.0
+    v, dout = torch.randn(B, L, Hkv, D, generator=gen).to(dtype), torch.randn(B, L, Hq, D, generator=gen).to(dtype)
+    G = Hq // Hkv
+    total = dout.double().sum(1).view(B, Hkv, G, D).sum(2)
+    bound = (L * G + 8) * 2.0 ** -24 * dout.double().abs().sum(1).view(B, Hkv, G, D).sum(2) + torch.finfo(dtype).eps / 2 * total.abs()
+    for scale in (0.7, 1 / 3):
+        leaves = [t.to(dtype).to(cuda0).requires_grad_() for t in (q, k, v)]
+        out = K.band_attention(*leaves, scale=scale)
+        assert torch.equal(out, leaves[2][:, 17:18].repeat_interleave(G, 2).expand_as(out))
+        dq, dk, dv = (g.double().cpu() for g in torch.autograd.grad(out, leaves, dout.to(cuda0)))
+        assert not dq.any() and not dk.any()
+        assert not dv[:, :17].any() and not dv[:, 18:].any()
+        assert bool(((dv[:, 17] - total).abs() <= bound).all())

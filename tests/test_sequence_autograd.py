@@ -172,3 +172,17 @@ def test_bucket_numbers_are_clamped_before_they_are_narrowed(calls, monkeypatch)
     assert seen == [[2, 0, 1, 2, 0]]
     _attention(x, x, x, bias_table=torch.zeros(3, 2), bias_buckets=torch.tensor([0, 1, 1, 2, 0], dtype=torch.int32))
     assert seen[1] == [0, 1, 1, 2, 0]
+
+
+@pytest.mark.parametrize("dtype,table,kept", [(torch.float32, False, True), (torch.bfloat16, False, False), (torch.float32, True, False)])
+def test_what_the_rounding_of_the_log_sum_exp_leaves_is_kept_in_fp32(calls, dtype, table, kept):
+    """(with a bias it is in two parts anyway)"""
+    import ctypes
+    from visiontransformer_amd._lib import BandDesc
+    x = torch.randn(2, 4, 3, 8).to(dtype).requires_grad_()
+    kw = dict(bias_table=torch.zeros(3, 3), bias_buckets=torch.zeros(5, dtype=torch.int32)) if table else {}
+    _attention(x, x, x, **kw).sum().backward()
+    for name, args in calls:
+        d = ctypes.cast(ctypes.pointer(args[0]._obj), ctypes.POINTER(BandDesc)).contents
+        lse = args[9 if name.endswith("fwd") else 12]
+        assert d.lse_rest == (lse + 4 * 2 * 3 * 4 if kept else None), name

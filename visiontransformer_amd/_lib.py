@@ -32,7 +32,7 @@ class BandDesc(ctypes.Structure):
     """dsw_band_desc"""
     _fields_ = [("dtype", _I), ("B", _I), ("Lq", _I), ("Lk", _I), ("Hq", _I), ("Hkv", _I), ("D", _I), ("left", _I), ("right", _I),
                 ("sinks", _I), ("scale", _F), ("q_lens", _P), ("k_lens", _P), ("bias_table", _P), ("bias_buckets", _P),
-                ("n_buckets", _I), ("max_distance", _I), ("out_rest", _P)]
+                ("n_buckets", _I), ("max_distance", _I), ("out_rest", _P), ("lse_rest", _P)]
 
 
 # name -> (restype, argtypes); must list every symbol include/dswin_hip.h declares

@@ -38,6 +38,7 @@ struct BandArgs {
     int n_buckets, M;
     float *lse;          // [B][Hq][Lq], base 2; +inf for rows without a visible key (2^(x - inf) = 0 in the backward)
     float *top;          // with a bias table: [B][Hq][Lq], taken out of lse (see band_keep)
+    float *lse_rest;     // fp32 calls without a bias table: [B][Hq][Lq] or null, what the rounding of lse left behind
     float *out32;        // [B][Lq][Hq][D] or null
     bf16_t *rest;        // [B][Lq][Hq][D] or null: out before its rounding, less out
     float *delta;        // [B][Hq][Lq]
@@ -460,8 +461,16 @@ __device__ __forceinline__ bool band_strayed(float m, float l) { return m != -IN
 __device__ __forceinline__ void band_keep(const BandArgs &a, size_t at, bool off, float top, float lift, float l) {
     const float log_l = off ? INFINITY : __builtin_amdgcn_logf(l) + lift;
     if (a.top) a.top[at] = off ? 0.f : top;
-    a.lse[at] = a.top || off ? log_l : top + log_l;
+    const float sum = top + log_l, part = sum - top;
+    a.lse[at] = a.top || off ? log_l : sum;
+    if (a.lse_rest) a.lse_rest[at] = off ? 0.f : (top - (sum - part)) + (log_l - part);
 }
+// Without a bias an exponent of the backward is one multiply-add, scale * s - lse: the product is not rounded, as the reference
+// was, and lse is rounded once more, which puts probabilities off by 2^-25 of the logits' size.  For fp32 calls, whose matrix
+// instructions leave the time, the product is rounded first and what the rounding of lse left is taken off as well: a row's
+// only key then has the probability 1, whatever its score.  (For bf16 the size has to pass 2^16 before it is seen, and the
+// same costs dk and dv 15 %.)
+template <typename T> constexpr bool band_whole(bool bias) { return !bias && sizeof(T) == 4; }
 __device__ __forceinline__ void band_stage_bias(const BandArgs &a, int head, int sign, float *dst, int threads) {
     const int n = 2 * (a.M + BAND_MARGIN) + 1;
     for (int e = threadIdx.x; e < n; e += threads) dst[e] = band_bias_at(a, head, sign * (e - a.M - BAND_MARGIN));

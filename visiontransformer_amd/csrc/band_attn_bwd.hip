@@ -29,11 +29,12 @@ template <typename T, int DP, int MODE, bool BIAS>
 __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void band_attn_dkv_kernel(const BandArgs a) {
     constexpr int NB = band_t<T>::nbuf(DP), ELEMS = band_t<T>::template elems<DP>(BAND_TILE), C = DP / 16;
     constexpr bool AHEAD = DP < 128 && (sizeof(T) == 2 || DP == 32);  // registers for LDS reads well ahead of the products that need them
-    constexpr int STATS = BIAS ? 4 : 2;
+    constexpr bool WHOLE = band_whole<T>(BIAS);
+    constexpr int STATS = BIAS ? 4 : WHOLE ? 3 : 2;
     using Stage = BandStage<T, DP, MODE>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     T *const lds = reinterpret_cast<T *>(smem);                        // [NB][Q | dO]
-    float *const stats = reinterpret_cast<float *>(lds + NB * 2 * ELEMS);  // [NB][-lse - top | delta | top | -lse][64]
+    float *const stats = reinterpret_cast<float *>(lds + NB * 2 * ELEMS);  // [NB][-lse - top | delta | top | -lse][64], WHOLE: [-lse | delta | -lse_rest]
     float *const bias = stats + NB * STATS * BAND_TILE;
 
     const int nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS, units = a.sink_blocks * a.sink_chunks + (nkb - a.sink_blocks) * a.chunks;
@@ -86,9 +87,13 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
             const int i = i0 + (threadIdx.x & (BAND_TILE - 1));
             const int stat = threadIdx.x / BAND_TILE;
             const size_t at = ((size_t)b * a.Hq + h) * a.Lq + min(i, sq.qn - 1);
-            st = (stat == 1 ? a.delta : stat == 2 ? a.top : a.lse)[at];
-            if (BIAS && stat == 0) st += a.top[at];
-            if (stat == 0 || stat == 3) st = i < sq.qn ? -st : -INFINITY;
+            if (WHOLE && stat == 2) {
+                st = a.lse_rest ? -a.lse_rest[at] : 0.f;
+            } else {
+                st = (stat == 1 ? a.delta : stat == 2 ? a.top : a.lse)[at];
+                if (BIAS && stat == 0) st += a.top[at];
+                if (stat == 0 || stat == 3) st = i < sq.qn ? -st : -INFINITY;
+            }
         }
         qs.fetch(reinterpret_cast<const char *>(band_row<T>(a.q, b, i0, h)), sq.qn - 1 - i0, a.D, image);
         gs.fetch(reinterpret_cast<const char *>(band_row<T>(a.dout, b, i0, h)), sq.qn - 1 - i0, a.D, image + ELEMS);
@@ -158,6 +163,14 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void ba
             };
             if (AHEAD && !BIAS) columns_ahead();
             float cs = a.c;
+            if constexpr (WHOLE) {
+                cs = 1.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[r] = s[r] * a.c + nl[r];
+                    nl[r] = S[2 * BAND_TILE + 32 * u + 4 * hh + rho(r)];
+                }
+            }
             if constexpr (BIAS) {
                 const bool near = j_lo - p_hi < a.M && j_hi - p_lo > -a.M;
                 if (band_remote(S[2 * BAND_TILE + 32 * u + l31])) {
@@ -325,6 +338,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
     const size_t stat = ((size_t)b * a.Hq + h) * a.Lq + i;
     const float nl = row_on ? -a.lse[stat] : -INFINITY, top = BIAS && row_on ? a.top[stat] : 0.f;
     const bool remote = BIAS && band_remote(top);
+    constexpr bool WHOLE = band_whole<T>(BIAS);
+    const float low = WHOLE && row_on && a.lse_rest ? -a.lse_rest[stat] : 0.f;
     // delta = dout . out, from the result before its rounding where that was kept (whole, in three parts of 8 bits, or as what the
     // rounding left behind: with the rounded result alone dq and dk of a row of one dominant key were mostly its error).  It is the
     // diagonal of a product formed like dout v^T below: for a row that sees a single key, whose result is that key's value,
@@ -448,9 +463,18 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ba
 #pragma unroll
                         for (int r = 0; r < 16; ++r) s[r] = band_exponent(s[r], scale, bias[e0 + rho(r)], top, false);
                     }
+                } else if (remote) {
+                    const float left = bias[j0 > w_hi ? BL - 1 : 0] - top;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], scale, left);
+                    cs = 1.f;
                 } else {
                     shift += bias[j0 > w_hi ? BL - 1 : 0] - top;
                 }
+            } else if constexpr (WHOLE) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = s[r] * scale + nl;
+                cs = 1.f, shift = low;
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], cs, shift));
@@ -595,7 +619,7 @@ template <typename T, int DP, int MODE, bool BIAS, bool DTABLE> static int launc
         if (int rc = check_launch("dsw_band_attn_bwd (dq)")) return rc;
     }
     if (a.Lk) {
-        const size_t lds = images + (size_t)band_t<T>::nbuf(DP) * (BIAS ? 4 : 2) * BAND_TILE * sizeof(float) + bl;
+        const size_t lds = images + (size_t)band_t<T>::nbuf(DP) * (BIAS ? 4 : band_whole<T>(BIAS) ? 3 : 2) * BAND_TILE * sizeof(float) + bl;
         auto kern = band_attn_dkv_kernel<T, DP, MODE, BIAS>;
         if (int rc = band_allow_lds("dsw_band_attn_bwd", kern, lds)) return rc;
         const long long nkb = (a.Lk + BAND_ROWS - 1) / BAND_ROWS, heads = (long long)a.B * a.Hkv;
@@ -655,6 +679,7 @@ extern "C" int dsw_band_attn_bwd(const dsw_band_desc *d, const void *q, const ds
     const size_t need = dsw_band_attn_bwd_workspace(d);
     DSW_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "%s: workspace of %zu bytes, %zu are needed", who, workspace_bytes, need);
     a.lse = const_cast<float *>(lse);
+    a.lse_rest = a.table || d->dtype != DSW_F32 ? nullptr : d->lse_rest;
     a.top = a.table && lse ? a.lse + (size_t)a.B * a.Hq * a.Lq : nullptr;
     a.out32 = const_cast<float *>(out32);
     a.delta = static_cast<float *>(workspace);

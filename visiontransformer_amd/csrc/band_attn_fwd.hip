@@ -373,6 +373,7 @@ extern "C" int dsw_band_attn_fwd(const dsw_band_desc *d, const void *q, const ds
     DSW_REQUIRE(out32 == nullptr || (a.table && d->dtype == DSW_BF16), "%s: out32 goes with a bias table and bf16 tensors", who);
     if ((rc = band_rest_tensor(who, d, a, mode))) return rc;
     a.lse = lse;
+    a.lse_rest = a.table || d->dtype != DSW_F32 ? nullptr : d->lse_rest;
     a.top = lse && a.table ? lse + (size_t)a.B * a.Hq * a.Lq : nullptr;
     a.out32 = out32;
     hipStream_t st = as_stream(stream);

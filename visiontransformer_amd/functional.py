@@ -2562,10 +2562,11 @@ def _workspace(way, desc):
 
 class _BandAttnFn(torch.autograd.Function):
     @staticmethod
-    def _desc(q, k, tab, buckets, q_lens, k_lens, left, right, sinks, scale, rest=None):
+    def _desc(q, k, tab, buckets, q_lens, k_lens, left, right, sinks, scale, rest=None, lse=None):
         B, Lq, Hq, D = q.shape
         return _lib.BandDesc(dtype_code(q.dtype), B, Lq, k.shape[1], Hq, k.shape[2], D, left, right, sinks, scale, ptr(q_lens), ptr(k_lens),
-                             ptr(tab), ptr(buckets), 0 if tab is None else tab.shape[0], 0 if tab is None else buckets.numel() // 2, ptr(rest))
+                             ptr(tab), ptr(buckets), 0 if tab is None else tab.shape[0], 0 if tab is None else buckets.numel() // 2, ptr(rest),
+                             ptr(lse[1]) if lse is not None and tab is None and len(lse) == 2 else None)
 
     @staticmethod
     def forward(ctx, q, k, v, table, buckets, q_lens, k_lens, left, right, sinks, scale):
@@ -2581,8 +2582,9 @@ class _BandAttnFn(torch.autograd.Function):
         exact = train and ctx.needs_input_grad[3] and q.dtype == torch.bfloat16
         # (what the rounding to 16 bits leaves of the result: the gradients of scores are taken from both)
         rest = torch.empty_like(out) if train and not exact and q.dtype == torch.bfloat16 and any(ctx.needs_input_grad[:2]) else None
-        desc = _BandAttnFn._desc(q, k, tab, buckets, q_lens, k_lens, *settings, rest)
-        lse = torch.empty(1 if tab is None else 2, B, Hq, Lq, dtype=torch.float32, device=dev) if train else None
+        # (with a bias the rows' references and log2 of their sums; without, the sum of the two and, in fp32, what its rounding leaves)
+        lse = torch.empty(1 if tab is None and q.dtype != torch.float32 else 2, B, Hq, Lq, dtype=torch.float32, device=dev) if train else None
+        desc = _BandAttnFn._desc(q, k, tab, buckets, q_lens, k_lens, *settings, rest, lse)
         out32 = torch.empty(B, Lq, Hq, D, dtype=torch.float32, device=dev) if exact else None
         if B * Lq * Hq:
             n = 0 if exact else _workspace("fwd", desc)
@@ -2611,7 +2613,7 @@ class _BandAttnFn(torch.autograd.Function):
             operands += [p, s, ptr(lse)]
             for t in made:
                 operands += t[:0:-1]
-            desc = _BandAttnFn._desc(q, k, tab, buckets, q_lens, k_lens, *ctx.settings, rest)
+            desc = _BandAttnFn._desc(q, k, tab, buckets, q_lens, k_lens, *ctx.settings, rest, lse)
             n = _workspace("bwd", desc)
             ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
             _call_on(dev, "dsw_band_attn_bwd", ctypes.byref(desc), *operands, ptr(d_tab), ptr(ws), n, stream(dev))
@@ -2638,7 +2640,8 @@ def band_attention(q, k, v, window=(None, None), sinks=0, scale=None, q_lens=Non
     product with v, and in the backward those and the scores' gradients where they enter theirs (2^-8 each, as the matrix
     instructions take them), besides each result: outputs end some 2.2e-3 (rms) from 64 bits and gradients 2.4e-3, where the
     results' own rounding is 1.7e-3.  A bias table's gradient is fp32, 1.2e-6 from 64 bits in bf16 calls.  fp32 calls round nothing
-    further.  The backward computes probabilities anew from a log-sum-exp in fp32, so they carry 2^-24 of the logits' size.
+    further.  The backward of bf16 calls computes probabilities anew from a log-sum-exp in fp32: they are off by 2^-25 of the
+    logits' size, and logits beyond 2^30 leave no finite gradients.
 
     bias_table [n, Hq] with bias_buckets int32 [2 M + 1], M <= 512: table[bias_buckets[clip(j - p, -M, M) + M], head] is
     added to the scaled logits (sequence.BucketedPositionBias holds both).  scale: D ** -0.5 by default, positive.
